@@ -445,6 +445,157 @@ snn_status_t snn_b200_step_noalloc(int device, void *stream, snn_size_t neuron_c
                                    uint32_t *refractory, uint8_t *spikes, const snn_size_t *row_ptr,
                                    const uint32_t *col_idx, const float *weights, float *next_current);
 
+/* ============ Part 4: sequence operators over device arrays ============= */
+/* The two halves of a step for whole sequences and dense layers, over device
+ * arrays the caller owns: the propagation of a dense layer as a product with
+ * packed 4-bit weights, and the leaky integration (no threshold, no reset) of
+ * many steps at once, with its gradient and a single-step form. No
+ * counterpart in the reference's CUDA API.
+ *
+ * Common to all of them: work is enqueued on `stream` (a cudaStream_t, NULL =
+ * legacy default) of `device`, which need not be the current device; nothing
+ * is allocated and nothing synchronises, so every call can be captured into
+ * a CUDA graph. All pointers are device pointers aligned to their element
+ * size unless said otherwise, strides count elements, and input arrays do not
+ * overlap output arrays unless said otherwise. Workspaces need no
+ * initialisation; calls (or graphs) that may overlap on the GPU need
+ * workspaces of their own. An empty problem (a count of zero) reads and
+ * writes only what it still defines. Counts above 2^31 - 1 return
+ * SNN_ERR_OVERFLOW, a combination of element types that is not listed
+ * SNN_ERR_UNSUPPORTED, everything else that is wrong with an argument
+ * SNN_ERR_INVALID_ARGUMENT. */
+typedef enum snn_b200_dtype {
+    SNN_B200_F32 = 0,
+    SNN_B200_F16 = 1,
+    SNN_B200_BF16 = 2,
+    SNN_B200_SPIKES = 3 /* a byte per element, non-zero = one spike (1.0), as snn_cuda_step writes them */
+} snn_b200_dtype_t;
+
+/* ---- Microscaled 4-bit floating point (MXFP4) ----
+ * A packed matrix of `rows` x `cols` keeps each row in blocks of 32 elements
+ * that share a scale 2^X, X = max(floor(log2(largest magnitude)) - 2, -127)
+ * (-127 for a block of zeros), each element as the nearest of 0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 times the scale with its sign (ties to the even code, larger
+ * magnitudes to 6). Spikes and blocks of equal magnitudes are kept exactly. A
+ * block that holds a NaN or an infinity reads back as NaN throughout.
+ *
+ * codes: row r at r * pitch, pitch = ceil(cols / 32) * 16 bytes, two elements
+ * a byte, the even one in the low half; elements behind the last column are
+ * zero. scales: one byte X + 127 a block (255: NaN), in tiles of 128 rows x 4
+ * blocks: the byte of row r, block b lies at
+ *   512 * ((r / 128) * ceil(ceil(cols / 32) / 4) + b / 4) + 16 * (r % 32) + 4 * (r % 128 / 32) + b % 4;
+ * bytes without a row or a block are zero. Both arrays 16-byte aligned. */
+snn_status_t snn_b200_mx4_sizes(snn_size_t rows, snn_size_t cols, snn_size_t *out_code_bytes,
+                                snn_size_t *out_scale_bytes);
+
+/* Packs src (any snn_b200_dtype_t; element (r, c) at r * row_stride + c *
+ * col_stride, strides >= 0). With row_stride 1 the source is a transposed
+ * matrix, e.g. a dense layer stored one row per presynaptic neuron. */
+snn_status_t snn_b200_mx4_quantize_async(int device, void *stream, const void *src, int src_dtype, snn_size_t rows,
+                                         snn_size_t cols, int64_t row_stride, int64_t col_stride, void *codes,
+                                         void *scales);
+
+/* Writes the values that a packed matrix stands for (F32, F16, BF16; exact
+ * in F32 and BF16) as rows of row_stride >= cols elements. */
+snn_status_t snn_b200_mx4_dequantize_async(int device, void *stream, const void *codes, const void *scales,
+                                           snn_size_t rows, snn_size_t cols, void *dst, int dst_dtype,
+                                           int64_t row_stride);
+
+/* out[i, j] = sum over k of x[i, k] * w[j, k], plus bias[j] where bias (n
+ * floats) is not NULL: x (m x k) and w (n x k) packed, sums in 32 bits, one
+ * rounding to F32, F16 or BF16. Row i of out starts at i * out_row_stride
+ * (>= n). The sums' order depends on m, n and k only, so results repeat. */
+snn_status_t snn_b200_mx4_matmul_async(int device, void *stream, const void *x_codes, const void *x_scales,
+                                       snn_size_t m, const void *w_codes, const void *w_scales, snn_size_t n,
+                                       snn_size_t k, const float *bias, void *out, int out_dtype,
+                                       int64_t out_row_stride);
+
+/* The same with x (m x k, any snn_b200_dtype_t, strides as for quantize)
+ * packed on the way: equal to quantize followed by matmul. The workspace holds
+ * snn_b200_mx4_linear_workspace(m, k) bytes, 16-byte aligned. */
+snn_size_t snn_b200_mx4_linear_workspace(snn_size_t m, snn_size_t k);
+snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, int x_dtype, snn_size_t m,
+                                       snn_size_t k, int64_t x_row_stride, int64_t x_col_stride, const void *w_codes,
+                                       const void *w_scales, snn_size_t n, const float *bias, void *out,
+                                       int out_dtype, int64_t out_row_stride, void *workspace,
+                                       snn_size_t workspace_bytes);
+
+/* ---- Leaky recurrence ----
+ * For every sequence b < batch and channel c < channels
+ *   h[t] = a[t] * h[t-1] + u[t],   y[t] = h[t],   t = 0 .. steps-1,   h[-1] = h0[b, c],
+ * the update of the membrane (src/snn.c:773-790) without its threshold. The
+ * gate array holds a itself, or its logits (logit != 0: a = 1 / (1 + exp(-gate)));
+ * without a gate array a = decay. u = input_scale * x, or with complement != 0
+ * u = input_scale * (1 - a) * x.
+ *
+ * Element (b, t, c) of an array lies at b * batch_stride + t * step_stride + c,
+ * so rasters (steps first) and activations (sequences first) both work; a
+ * gate stride of 0 shares the gate over the sequences or over the steps.
+ * States (h0, h_last, dh_last, dh0) are floats [batch, channels].
+ *
+ * lengths (batch values, NULL: all `steps`; larger ones count as steps): rows
+ * at or behind lengths[b] are not read, their outputs are zero, and the state
+ * passes them unchanged.
+ *
+ * Types (x, gate, y): SPIKES, F32, F32; F32, F32, F32; and for T of F16 and
+ * BF16: T with gate T or F32 and y T or F32. A gate without step stride is F32.
+ * States, sums and products are in 32 bits. Products of gates over
+ * consecutive steps are formed, so gates above one must not overflow there. */
+typedef struct snn_b200_leaky {
+    snn_size_t batch, steps, channels;
+    int x_dtype, gate_dtype, y_dtype; /* snn_b200_dtype_t */
+    int logit;                        /* the gate array holds logits */
+    int complement;                   /* the input is weighted with 1 - a */
+    float decay;                      /* a, where there is no gate array */
+    float input_scale;
+    int64_t x_batch_stride, x_step_stride;
+    int64_t gate_batch_stride, gate_step_stride;
+    int64_t y_batch_stride, y_step_stride;
+    /* backward only */
+    int64_t dy_batch_stride, dy_step_stride;
+    int64_t dx_batch_stride, dx_step_stride;
+    int64_t dgate_batch_stride, dgate_step_stride;
+} snn_b200_leaky_t;
+
+/* What the backward pass needs beside x and the gate: the state before every
+ * 16th step, floats [batch, ceil(steps / 16), channels]. */
+#define SNN_B200_LEAKY_BLOCK 16u
+snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_size_t channels);
+/* Bytes of workspace (16-byte aligned) of the forward and of the backward call. */
+snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *leaky);
+
+/* h0 may be NULL (zero); h_last and saved may be NULL (not wanted). */
+snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,
+                                       const void *gate, const float *h0, const uint32_t *lengths, void *y,
+                                       float *h_last, float *saved, void *workspace, snn_size_t workspace_bytes);
+
+/* Gradients of the same call, given dy (type y_dtype) and dh_last (may be
+ * NULL: zero): dx (type x_dtype, F32 for SPIKES), dh0, and dgate. With a gate
+ * step stride dgate has the gate's type and layout [b, t, c] with its own
+ * strides, and the gate must not be shared over the sequences (batch > 1 with
+ * gate_batch_stride 0: SNN_ERR_UNSUPPORTED). Without one, dgate is the sum
+ * over the steps in F32: [batch, channels] rows of dgate_batch_stride, or
+ * with gate_batch_stride 0 the sum over everything, [channels]. dx, dgate and
+ * dh0 may be NULL (not wanted). Sums are taken in a fixed order. */
+snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const snn_b200_leaky_t *leaky,
+                                                const void *x, const void *gate, const uint32_t *lengths,
+                                                const float *saved, const void *dy, const float *dh_last, void *dx,
+                                                void *dgate, float *dh0, void *workspace,
+                                                snn_size_t workspace_bytes);
+
+/* One step of `batch` rows whose states sit in a pool: row i updates pool row
+ * slots[i] (slots NULL: row i; then batch <= slot_count) in place and writes
+ * the new state to y. x, gate and y rows have their own strides, a
+ * gate_row_stride of 0 shares the gate; types as above. Rows whose slot is
+ * outside [0, slot_count) are padding: y is zero and no state changes. Rows
+ * that name the same slot are applied in row order. */
+snn_status_t snn_b200_leaky_step_async(int device, void *stream, snn_size_t batch, snn_size_t slot_count,
+                                       snn_size_t channels, const void *x, int x_dtype, int64_t x_row_stride,
+                                       const void *gate, int gate_dtype, int64_t gate_row_stride, int logit,
+                                       int complement, float decay, float input_scale, float *pool,
+                                       int64_t pool_row_stride, const int32_t *slots, void *y, int y_dtype,
+                                       int64_t y_row_stride);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libsnn_b200.so")
 
 u64 = C.c_uint64
+i64 = C.c_int64
 f32 = C.c_float
 P = C.c_void_p
 
@@ -154,6 +155,19 @@ ENTRY_POINTS = [
     ("snn_b200_network_unwrap", None, [P]),
     ("snn_b200_network_save", C.c_int, [P, C.c_char_p]),
     ("snn_b200_network_map", C.c_int, [C.c_char_p, P]),
+    ("snn_b200_mx4_sizes", C.c_int, [u64, u64, P, P]),
+    ("snn_b200_mx4_quantize_async", C.c_int, [C.c_int, P, P, C.c_int, u64, u64, i64, i64, P, P]),
+    ("snn_b200_mx4_dequantize_async", C.c_int, [C.c_int, P, P, P, u64, u64, P, C.c_int, i64]),
+    ("snn_b200_mx4_matmul_async", C.c_int, [C.c_int, P, P, P, u64, P, P, u64, u64, P, P, C.c_int, i64]),
+    ("snn_b200_mx4_linear_workspace", u64, [u64, u64]),
+    ("snn_b200_mx4_linear_async", C.c_int, [C.c_int, P, P, C.c_int, u64, u64, i64, i64, P, P, u64, P, P, C.c_int,
+                                            i64, P, u64]),
+    ("snn_b200_leaky_saved_floats", u64, [u64, u64, u64]),
+    ("snn_b200_leaky_workspace", u64, [P]),
+    ("snn_b200_leaky_scan_async", C.c_int, [C.c_int, P, P, P, P, P, P, P, P, P, P, u64]),
+    ("snn_b200_leaky_scan_backward_async", C.c_int, [C.c_int, P, P, P, P, P, P, P, P, P, P, P, P, u64]),
+    ("snn_b200_leaky_step_async", C.c_int, [C.c_int, P, u64, u64, u64, P, C.c_int, i64, P, C.c_int, i64, C.c_int,
+                                            C.c_int, f32, f32, P, i64, P, P, C.c_int, i64]),
 ]
 
 _LIB = None
@@ -464,3 +478,8 @@ class CudaContext:
             self.free()
         except Exception:
             pass
+
+
+# The sequence operators over CUDA tensors (torch is imported when one is called).
+from .sequence import (Leaky, Mx4, leaky_scan, leaky_scan_backward, leaky_step, mx4_dequantize,  # noqa: E402,F401
+                       mx4_linear, mx4_matmul, mx4_quantize, mx4_sizes)

@@ -21,6 +21,7 @@
 #include "b200_binfold.h"
 #include "b200_kernels.h"
 #include "b200_network.h"
+#include "b200_ops.h"
 
 #include <cuda_runtime.h>
 #include <nccl.h>
@@ -2053,6 +2054,10 @@ snn_status_t group_step(snn_cuda_context_t *g, const float *ext, uint8_t *spikes
 // ======================================================================
 //                              C ABI
 // ======================================================================
+namespace b200 {
+snn_status_t op_status(cudaError_t e, const char *where) { return cuda_status_at(e, where); }
+}  // namespace b200
+
 extern "C" {
 
 snn_cuda_config_t snn_cuda_default_config(void) {

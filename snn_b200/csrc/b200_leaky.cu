@@ -1,182 +1,42 @@
-// The leaky recurrence over device arrays: scan, gradient and single step.
-#include "b200_ops.h"
+// The leaky recurrence over device arrays: the calls, their checks and how the
+// work is split, the sum of a shared gate's gradient, and the single step.
+#include "b200_leaky.h"
+
+#include <algorithm>
 
 namespace b200 {
+namespace leaky {
 namespace {
 
-constexpr uint32_t kBlockSteps = SNN_B200_LEAKY_BLOCK;
-
-__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
-    switch (dtype) {
-        case SNN_B200_F32: return ((const float *)p)[i];
-        case SNN_B200_F16: return to_float(((const __half *)p)[i]);
-        case SNN_B200_BF16: return to_float(((const __nv_bfloat16 *)p)[i]);
-        default: return to_float(((const Spike *)p)[i]);
-    }
-}
-__device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
-    switch (dtype) {
-        case SNN_B200_F32: ((float *)p)[i] = v; break;
-        case SNN_B200_F16: ((__half *)p)[i] = from_float<__half>(v); break;
-        default: ((__nv_bfloat16 *)p)[i] = from_float<__nv_bfloat16>(v); break;
-    }
-}
-
-struct Leak {
-    float a, rest;  // the gate and one minus it
-};
-// Both from one exponential of a non-positive number, so that neither is a
-// difference of nearly equal values.
-__device__ __forceinline__ Leak leak_of(float z, int logit) {
-    if (!logit) return {z, __fsub_rn(1.0f, z)};
-    const float t = expf(-fabsf(z));
-    const float r = __fdividef(1.0f, __fadd_rn(1.0f, t)), q = __fmul_rn(t, r);
-    return z >= 0.0f ? Leak{r, q} : Leak{q, r};
-}
-
-struct Args {
-    snn_b200_leaky_t p;
-    const void *x, *gate;
-    const float *h0;
-    const uint32_t *lengths;
-    void *y;
-    float *h_last, *saved;
-    const void *dy;
-    const float *dh_last;
-    void *dx, *dgate;
-    float *dh0;
-    float *partial;  // [batch, channels] sums of a shared gate's gradient
-};
-
-__device__ __forceinline__ uint64_t length_of(const Args &g, uint64_t b) {
-    return g.lengths ? min((uint64_t)g.lengths[b], (uint64_t)g.p.steps) : g.p.steps;
-}
-__device__ __forceinline__ Leak leak_at(const Args &g, uint64_t b, uint64_t t, uint64_t c) {
-    if (!g.gate) return {g.p.decay, __fsub_rn(1.0f, g.p.decay)};
-    return leak_of(load_any(g.gate, g.p.gate_dtype,
-                            (int64_t)b * g.p.gate_batch_stride + (int64_t)t * g.p.gate_step_stride + (int64_t)c),
-                   g.p.logit);
-}
-
-// One thread a channel, step by step.
-__global__ void leaky_scan_kernel(Args g) {
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= g.p.batch * g.p.channels) return;
-    const uint64_t b = i / g.p.channels, c = i % g.p.channels, len = length_of(g, b);
-    const uint64_t blocks = (g.p.steps + kBlockSteps - 1) / kBlockSteps;
-    float h = g.h0 ? g.h0[i] : 0.0f;
-    for (uint64_t t = 0; t < g.p.steps; ++t) {
-        if (g.saved && t % kBlockSteps == 0) g.saved[(b * blocks + t / kBlockSteps) * g.p.channels + c] = h;
-        float y = 0.0f;
-        if (t < len) {
-            const Leak l = leak_at(g, b, t, c);
-            float u = __fmul_rn(g.p.input_scale,
-                                load_any(g.x, g.p.x_dtype,
-                                         (int64_t)b * g.p.x_batch_stride + (int64_t)t * g.p.x_step_stride + (int64_t)c));
-            if (g.p.complement) u = __fmul_rn(u, l.rest);
-            y = h = __fmaf_rn(l.a, h, u);
+// ---- a shared gate's gradient ----
+// out[r][c] = the sum of partial[t][b][c] over the tiles and, where the gate
+// is shared over the sequences (rows of out: 1), over b. A CTA takes 32
+// channels of a row; its warps share the terms, in an order that depends on
+// the counts only. Terms are few (a tile each), so they are summed in 64 bits.
+constexpr uint32_t kSumWarps = 16;
+__global__ void __launch_bounds__(kSumWarps * 32) gate_sum_kernel(const float *partial, uint32_t tiles, uint32_t batch,
+                                                                  uint32_t channels, float *out, int64_t row_stride) {
+    __shared__ double s_sum[kSumWarps][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint32_t c = blockIdx.x * 32 + lane;
+    const uint64_t flat = (uint64_t)batch * channels;
+    for (uint32_t r = blockIdx.y; r < (row_stride ? batch : 1u); r += gridDim.y) {
+        const uint64_t terms = row_stride ? tiles : (uint64_t)tiles * batch;
+        // Term n of row r: tile n, sequence r; or n-th of all [tiles][batch].
+        const float *p = partial + (row_stride ? (uint64_t)r * channels : 0) + c;
+        const uint64_t step = row_stride ? flat : channels;
+        double sum = 0.0;
+        if (c < channels)
+#pragma unroll 4
+            for (uint64_t n = warp; n < terms; n += kSumWarps) sum += (double)p[n * step];
+        s_sum[warp][lane] = sum;
+        __syncthreads();
+        if (warp == 0 && c < channels) {
+            for (uint32_t w = 1; w < kSumWarps; ++w) sum += s_sum[w][lane];
+            out[(int64_t)r * row_stride + c] = (float)sum;
         }
-        store_any(g.y, g.p.y_dtype, (int64_t)b * g.p.y_batch_stride + (int64_t)t * g.p.y_step_stride + (int64_t)c, y);
+        __syncthreads();
     }
-    if (g.h_last) g.h_last[i] = h;
-}
-
-__global__ void leaky_backward_kernel(Args g) {
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= g.p.batch * g.p.channels) return;
-    const uint64_t b = i / g.p.channels, c = i % g.p.channels, len = length_of(g, b);
-    const uint64_t blocks = (g.p.steps + kBlockSteps - 1) / kBlockSteps;
-    const int dx_type = g.p.x_dtype == SNN_B200_SPIKES ? SNN_B200_F32 : g.p.x_dtype;
-    float e = g.dh_last ? g.dh_last[i] : 0.0f, total = 0.0f;
-    for (uint64_t k = blocks; k-- > 0;) {
-        float before[kBlockSteps], u[kBlockSteps];
-        float h = g.saved[(b * blocks + k) * g.p.channels + c], sum = 0.0f;
-        const uint64_t t0 = k * kBlockSteps;
-        for (uint32_t j = 0; j < kBlockSteps && t0 + j < len; ++j) {
-            const Leak l = leak_at(g, b, t0 + j, c);
-            before[j] = h;
-            u[j] = __fmul_rn(g.p.input_scale, load_any(g.x, g.p.x_dtype, (int64_t)b * g.p.x_batch_stride +
-                                                                               (int64_t)(t0 + j) * g.p.x_step_stride +
-                                                                               (int64_t)c));
-            h = __fmaf_rn(l.a, h, g.p.complement ? __fmul_rn(u[j], l.rest) : u[j]);
-        }
-        for (uint32_t j = kBlockSteps; j-- > 0;) {
-            const uint64_t t = t0 + j;
-            if (t >= g.p.steps) continue;
-            float dx = 0.0f, dz = 0.0f;
-            if (t < len) {
-                const Leak l = leak_at(g, b, t, c);
-                const float d = __fadd_rn(
-                    load_any(g.dy, g.p.y_dtype,
-                             (int64_t)b * g.p.dy_batch_stride + (int64_t)t * g.p.dy_step_stride + (int64_t)c),
-                    e);
-                e = __fmul_rn(l.a, d);
-                dx = __fmul_rn(g.p.input_scale, g.p.complement ? __fmul_rn(d, l.rest) : d);
-                dz = __fmul_rn(d, g.p.complement ? __fsub_rn(before[j], u[j]) : before[j]);
-                if (g.p.logit) dz = __fmul_rn(dz, __fmul_rn(l.a, l.rest));
-                sum = __fadd_rn(sum, dz);
-            }
-            if (g.dx)
-                store_any(g.dx, dx_type,
-                          (int64_t)b * g.p.dx_batch_stride + (int64_t)t * g.p.dx_step_stride + (int64_t)c, dx);
-            if (g.dgate && g.p.gate_step_stride)
-                store_any(g.dgate, g.p.gate_dtype,
-                          (int64_t)b * g.p.dgate_batch_stride + (int64_t)t * g.p.dgate_step_stride + (int64_t)c, dz);
-        }
-        total = __fadd_rn(total, sum);
-    }
-    if (g.dh0) g.dh0[i] = e;
-    if (g.dgate && !g.p.gate_step_stride) {
-        if (g.p.gate_batch_stride) ((float *)g.dgate)[(int64_t)b * g.p.dgate_batch_stride + (int64_t)c] = total;
-        else g.partial[i] = total;
-    }
-}
-
-// A gate shared over the sequences: their sums, added in order.
-__global__ void leaky_gate_sum_kernel(const float *partial, uint64_t batch, uint64_t channels, float *dgate) {
-    const uint64_t c = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= channels) return;
-    float sum = 0.0f;
-    for (uint64_t b = 0; b < batch; ++b) sum = __fadd_rn(sum, partial[b * channels + c]);
-    dgate[c] = sum;
-}
-
-struct StepArgs {
-    uint64_t batch, slot_count, channels;
-    const void *x, *gate;
-    int x_dtype, gate_dtype, y_dtype, logit, complement;
-    int64_t x_stride, gate_stride, pool_stride, y_stride;
-    float decay, input_scale;
-    float *pool;
-    const int32_t *slots;
-    void *y;
-};
-
-// A thread does the row that names a slot first, and in order the later
-// rows that name it too.
-__global__ void leaky_step_kernel(StepArgs g) {
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= g.batch * g.channels) return;
-    const uint64_t row = i / g.channels, c = i % g.channels;
-    const int64_t slot = g.slots ? (int64_t)g.slots[row] : (int64_t)row;
-    if (slot < 0 || (uint64_t)slot >= g.slot_count) {
-        store_any(g.y, g.y_dtype, (int64_t)row * g.y_stride + (int64_t)c, 0.0f);
-        return;
-    }
-    if (g.slots)
-        for (uint64_t r = 0; r < row; ++r)
-            if (g.slots[r] == (int32_t)slot) return;
-    float h = g.pool[slot * g.pool_stride + (int64_t)c];
-    for (uint64_t r = row; r < g.batch; ++r) {
-        if (r != row && (!g.slots || g.slots[r] != (int32_t)slot)) continue;
-        const Leak l = g.gate ? leak_of(load_any(g.gate, g.gate_dtype, (int64_t)r * g.gate_stride + (int64_t)c), g.logit)
-                              : Leak{g.decay, __fsub_rn(1.0f, g.decay)};
-        float u = __fmul_rn(g.input_scale, load_any(g.x, g.x_dtype, (int64_t)r * g.x_stride + (int64_t)c));
-        if (g.complement) u = __fmul_rn(u, l.rest);
-        h = __fmaf_rn(l.a, h, u);
-        store_any(g.y, g.y_dtype, (int64_t)r * g.y_stride + (int64_t)c, h);
-    }
-    g.pool[slot * g.pool_stride + (int64_t)c] = h;
 }
 
 // The listed combinations of types. Without a gate array its type is not looked at.
@@ -211,23 +71,86 @@ snn_status_t check_common(int device, const snn_b200_leaky_t *q, const void *x, 
     return SNN_OK;
 }
 
-uint32_t grid_of(uint64_t threads) { return (uint32_t)((threads + 127) / 128); }
+// Where the work lies in the workspace, for the split form.
+struct Plan {
+    uint64_t flat;
+    uint32_t tiles;
+    uint64_t zeroed;  // bytes of ticket and flags, at the start
+    uint64_t aggregates, states, partial, bytes;
+};
+// `width` channels a thread; the workspace is sized for either width.
+Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
+    Plan p = {};
+    p.flat = q.batch * q.channels;
+    p.tiles = (uint32_t)((q.steps + kTile - 1) / kTile);
+    const uint64_t supers = p.tiles / kSuper, columns = (p.flat + 32 * width - 1) / (32 * width);
+    const auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
+    p.zeroed = round((1 + ((uint64_t)p.tiles + supers) * columns) * 4);
+    p.aggregates = p.zeroed;
+    p.states = p.aggregates + round(p.tiles * columns * 32 * width * 8);
+    p.partial = p.states + round(supers * columns * 32 * width * 4);
+    p.bytes = p.partial + round((p.tiles ? p.tiles : 1) * p.flat * 4);
+    return p;
+}
+
+// Split along the steps when whole walks would leave the SMs short of loads
+// in flight, and when there are steps to split.
+bool wants_split(int device, const Plan &p, uint32_t width, snn_size_t steps) {
+    const uint64_t warps = (p.flat + 32 * width - 1) / (32 * width);
+    if (steps <= 2 * kSteps || warps * p.tiles > kMaxCount) return false;
+    return warps < (uint64_t)sm_count(device) * 16;
+}
+
+void fill(Args &g, const snn_b200_leaky_t &q, const Plan &p, uint32_t width, void *workspace) {
+    g.flat = p.flat;
+    g.batch = (uint32_t)q.batch, g.steps = (uint32_t)q.steps, g.channels = (uint32_t)q.channels;
+    g.xb = q.x_batch_stride, g.xt = q.x_step_stride, g.gb = q.gate_batch_stride, g.gt = q.gate_step_stride;
+    g.yb = q.y_batch_stride, g.yt = q.y_step_stride, g.dyb = q.dy_batch_stride, g.dyt = q.dy_step_stride;
+    g.dxb = q.dx_batch_stride, g.dxt = q.dx_step_stride, g.dgb = q.dgate_batch_stride, g.dgt = q.dgate_step_stride;
+    g.decay = q.decay, g.scale = q.input_scale, g.logit = q.logit, g.complement = q.complement;
+    g.tiles = p.tiles;
+    g.columns = (uint32_t)((p.flat + 32 * width - 1) / (32 * width));
+    char *w = (char *)workspace;
+    g.ticket = (uint32_t *)w;
+    g.tile_flags = g.ticket + 1;
+    g.state_flags = g.tile_flags + (uint64_t)p.tiles * g.columns;
+    g.aggregates = (float2 *)(w + p.aggregates);
+    g.states = (float *)(w + p.states);
+}
+
+// Two channels a thread where every array can be read in pairs.
+bool pairs(const void *p, uint32_t bytes, int64_t sb, int64_t st) {
+    return !p || (aligned_to(p, 2 * bytes) && sb % 2 == 0 && st % 2 == 0);
+}
+bool float_pairs(const float *p) { return aligned_to(p, 8); }
+
+cudaError_t run(cudaStream_t s, int x_dtype, const Form &f, const Args &g, bool back) {
+    switch (x_dtype) {
+        case SNN_B200_F32: return back ? backward_f32(s, f, g) : forward_f32(s, f, g);
+        case SNN_B200_F16: return back ? backward_f16(s, f, g) : forward_f16(s, f, g);
+        case SNN_B200_BF16: return back ? backward_bf16(s, f, g) : forward_bf16(s, f, g);
+        default: return back ? backward_spikes(s, f, g) : forward_spikes(s, f, g);
+    }
+}
 
 }  // namespace
+}  // namespace leaky
 }  // namespace b200
 
 using namespace b200;
+using namespace b200::leaky;
 
 extern "C" {
 
 snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_size_t channels) {
     if (batch > kMaxCount || steps > kMaxCount || channels > kMaxCount) return 0;
-    return batch * ((steps + kBlockSteps - 1) / kBlockSteps) * channels;
+    return batch * ((steps + kSteps - 1) / kSteps) * channels;
 }
 
 snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *q) {
     if (q == nullptr || q->batch > kMaxCount || q->steps > kMaxCount || q->channels > kMaxCount) return 0;
-    return q->batch * q->channels * 4;
+    const uint64_t one = plan_of(*q, 1).bytes, two = plan_of(*q, 2).bytes;
+    return one > two ? one : two;
 }
 
 snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,
@@ -244,10 +167,26 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
     if (q.batch * q.channels > kMaxCount) return SNN_ERR_OVERFLOW;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (q.steps == 0) {  // the state passes through
+        if (!h_last) return SNN_OK;
+        const cudaError_t e = h0 ? cudaMemcpyAsync(h_last, h0, q.batch * q.channels * 4, cudaMemcpyDeviceToDevice, s)
+                                 : cudaMemsetAsync(h_last, 0, q.batch * q.channels * 4, s);
+        return op_status(e, __func__);
+    }
+    const bool even = q.channels % 2 == 0 && pairs(x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
+                      pairs(gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
+                      pairs(y, dtype_bytes(q.y_dtype), q.y_batch_stride, q.y_step_stride) && float_pairs(h0) &&
+                      float_pairs(h_last) && float_pairs(saved);
+    const uint32_t width = even ? 2 : 1;
+    const Plan p = plan_of(q, width);
+    const Form f = {q.gate_dtype, q.y_dtype, gate && q.gate_step_stride, wants_split(device, p, width, q.steps), width};
     Args g = {};
-    g.p = q, g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
-    leaky_scan_kernel<<<grid_of(q.batch * q.channels), 128, 0, (cudaStream_t)stream>>>(g);
-    return op_status(cudaGetLastError(), __func__);
+    fill(g, q, p, width, workspace);
+    g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
+    cudaError_t e = f.split ? cudaMemsetAsync(workspace, 0, p.zeroed, s) : cudaSuccess;
+    if (e == cudaSuccess) e = run(s, q.x_dtype, f, g, false);
+    return op_status(e, __func__);
 }
 
 snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const snn_b200_leaky_t *leaky,
@@ -279,14 +218,42 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
     if (q.batch * q.channels > kMaxCount) return SNN_ERR_OVERFLOW;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
-    Args g = {};
-    g.p = q, g.x = x, g.gate = gate, g.lengths = lengths, g.saved = const_cast<float *>(saved), g.dy = dy;
-    g.dh_last = dh_last, g.dx = dx, g.dgate = dgate, g.dh0 = dh0, g.partial = (float *)workspace;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (q.batch) leaky_backward_kernel<<<grid_of(q.batch * q.channels), 128, 0, s>>>(g);
-    if (dgate && shared)
-        leaky_gate_sum_kernel<<<grid_of(q.channels), 128, 0, s>>>(g.partial, q.batch, q.channels, (float *)dgate);
-    return op_status(cudaGetLastError(), __func__);
+    const bool sums = dgate && !every;
+    if (q.steps == 0 || q.batch == 0) {  // no steps: the state's gradient passes through, the gate's is zero
+        cudaError_t e = cudaSuccess;
+        if (dh0 && q.batch)
+            e = dh_last ? cudaMemcpyAsync(dh0, dh_last, q.batch * q.channels * 4, cudaMemcpyDeviceToDevice, s)
+                        : cudaMemsetAsync(dh0, 0, q.batch * q.channels * 4, s);
+        if (e == cudaSuccess && sums)
+            e = shared ? cudaMemsetAsync(dgate, 0, q.channels * 4, s)
+                       : cudaMemset2DAsync(dgate, 4 * std::max<size_t>(q.dgate_batch_stride, q.channels), 0, q.channels * 4, q.batch, s);
+        return op_status(e, __func__);
+    }
+    const bool even = q.channels % 2 == 0 && pairs(x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
+                      pairs(gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
+                      pairs(dy, dtype_bytes(q.y_dtype), q.dy_batch_stride, q.dy_step_stride) &&
+                      pairs(dx, dtype_bytes(dx_type), q.dx_batch_stride, q.dx_step_stride) &&
+                      (!every || pairs(dgate, dtype_bytes(q.gate_dtype), q.dgate_batch_stride, q.dgate_step_stride)) &&
+                      float_pairs(dh_last) && float_pairs(dh0) && float_pairs(saved);
+    const uint32_t width = even ? 2 : 1;
+    const Plan p = plan_of(q, width);
+    const Form f = {q.gate_dtype, q.y_dtype, every, wants_split(device, p, width, q.steps), width};
+    Args g = {};
+    fill(g, q, p, width, workspace);
+    g.x = x, g.gate = gate, g.lengths = lengths, g.saved = const_cast<float *>(saved), g.dy = dy;
+    g.dh_last = dh_last, g.dx = dx, g.dgate = every ? dgate : nullptr, g.dh0 = dh0;
+    g.partial = sums ? (float *)((char *)workspace + p.partial) : nullptr;
+    cudaError_t e = f.split ? cudaMemsetAsync(workspace, 0, p.zeroed, s) : cudaSuccess;
+    if (e == cudaSuccess) e = run(s, q.x_dtype, f, g, true);
+    if (e == cudaSuccess && sums) {
+        const uint32_t rows = shared ? 1u : (uint32_t)(q.batch < 65535 ? q.batch : 65535);
+        gate_sum_kernel<<<dim3((uint32_t)((q.channels + 31) / 32), rows), kSumWarps * 32, 0, s>>>(
+            g.partial, f.split ? p.tiles : 1u, (uint32_t)q.batch, (uint32_t)q.channels, (float *)dgate,
+            shared ? 0 : q.dgate_batch_stride);
+        e = cudaGetLastError();
+    }
+    return op_status(e, __func__);
 }
 
 snn_status_t snn_b200_leaky_step_async(int device, void *stream, snn_size_t batch, snn_size_t slot_count,
@@ -312,10 +279,30 @@ snn_status_t snn_b200_leaky_step_async(int device, void *stream, snn_size_t batc
     if (batch * channels > kMaxCount) return SNN_ERR_OVERFLOW;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
-    const StepArgs g = {batch, slot_count, channels, x, gate, x_dtype, gate_dtype, y_dtype, logit, complement,
-                        x_row_stride, gate_row_stride, pool_row_stride, y_row_stride, decay, input_scale, pool, slots, y};
-    leaky_step_kernel<<<grid_of(batch * channels), 128, 0, (cudaStream_t)stream>>>(g);
-    return op_status(cudaGetLastError(), __func__);
+    StepArgs g = {(uint32_t)batch, (uint32_t)slot_count, (uint32_t)channels, x, gate, x_row_stride, gate_row_stride,
+                  pool_row_stride, y_row_stride, logit, complement, decay, input_scale, pool, slots, y, 0};
+    // Four channels a thread where every array can be read in fours.
+    const auto fours = [&](const void *p, uint32_t bytes, int64_t stride) {
+        return !p || (aligned_to(p, 4 * bytes) && stride % 4 == 0);
+    };
+    const bool wide = channels % 4 == 0 && fours(x, dtype_bytes(x_dtype), x_row_stride) &&
+                      fours(gate, dtype_bytes(gate_dtype), gate_row_stride) && fours(pool, 4, pool_row_stride) &&
+                      fours(y, dtype_bytes(y_dtype), y_row_stride);
+    const Form f = {gate ? gate_dtype : SNN_B200_F32, y_dtype, true, false, wide ? 4u : 1u};
+    const uint32_t pieces = (uint32_t)((channels + f.width - 1) / f.width);  // thread-sized pieces of a row
+    // A warp a row, or the whole CTA where that would leave SMs without work.
+    const bool many = batch >= (snn_size_t)sm_count(device) * 4;
+    g.rows = many ? 8 : 1;
+    const uint32_t across = 256 / g.rows;
+    const dim3 grid((uint32_t)((batch + g.rows - 1) / g.rows), std::min(many ? 2u : 64u, (pieces + across - 1) / across));
+    cudaError_t e;
+    switch (x_dtype) {
+        case SNN_B200_F32: e = step_f32((cudaStream_t)stream, f, g, grid); break;
+        case SNN_B200_F16: e = step_f16((cudaStream_t)stream, f, g, grid); break;
+        case SNN_B200_BF16: e = step_bf16((cudaStream_t)stream, f, g, grid); break;
+        default: e = step_spikes((cudaStream_t)stream, f, g, grid); break;
+    }
+    return op_status(e, __func__);
 }
 
 }  // extern "C"

@@ -1,13 +1,10 @@
 // Packed 4-bit matrices (MXFP4): packing, reading back and the product.
-#include "b200_ops.h"
+#include "b200_mx4.h"
 
 namespace b200 {
+namespace mx4 {
 namespace {
 
-constexpr uint32_t kBlock = 32;
-
-__host__ __device__ inline uint64_t blocks_of(uint64_t cols) { return (cols + kBlock - 1) / kBlock; }
-__host__ __device__ inline uint64_t scale_tiles(uint64_t cols) { return (blocks_of(cols) + 3) / 4; }
 __host__ __device__ inline uint64_t scale_offset(uint64_t r, uint64_t b, uint64_t tiles) {
     return 512 * ((r / 128) * tiles + b / 4) + 16 * (r % 32) + 4 * (r % 128 / 32) + b % 4;
 }
@@ -95,46 +92,17 @@ __global__ void mx4_dequantize_kernel(const uint8_t *codes, const uint8_t *scale
     }
 }
 
-// 32 x 32 outputs a CTA, a block of k at a time through shared memory.
-__global__ void mx4_matmul_kernel(const uint8_t *xc, const uint8_t *xs, uint64_t m, const uint8_t *wc,
-                                  const uint8_t *ws, uint64_t n, uint64_t k, const float *bias, void *out, int dtype,
-                                  int64_t rs) {
-    __shared__ float sx[32][33], sw[32][33];
-    const uint64_t nb = blocks_of(k), tiles = scale_tiles(k);
-    const uint32_t tx = threadIdx.x, ty = threadIdx.y;
-    const uint64_t j = (uint64_t)blockIdx.x * 32 + tx;
-    for (uint64_t i0 = (uint64_t)blockIdx.y * 32; i0 < m; i0 += (uint64_t)gridDim.y * 32) {
-        float acc[4] = {};
-        for (uint64_t b = 0; b < nb; ++b) {
-            for (uint32_t r = ty; r < 32; r += 8) {
-                const uint64_t xi = i0 + r, wj = (uint64_t)blockIdx.x * 32 + r;
-                sx[r][tx] = xi < m ? __fmul_rn(decode(xc[(xi * nb + b) * 16 + tx / 2] >> (4 * (tx & 1)) & 15u),
-                                               scale_value(xs[scale_offset(xi, b, tiles)]))
-                                   : 0.0f;
-                sw[r][tx] = wj < n ? __fmul_rn(decode(wc[(wj * nb + b) * 16 + tx / 2] >> (4 * (tx & 1)) & 15u),
-                                               scale_value(ws[scale_offset(wj, b, tiles)]))
-                                   : 0.0f;
-            }
-            __syncthreads();
-            for (uint32_t q = 0; q < 32; ++q)
-                for (uint32_t r = 0; r < 4; ++r) acc[r] = __fmaf_rn(sx[ty + 8 * r][q], sw[tx][q], acc[r]);
-            __syncthreads();
-        }
-        for (uint32_t r = 0; r < 4; ++r) {
-            const uint64_t i = i0 + ty + 8 * r;
-            if (i < m && j < n)
-                store_any(out, dtype, (int64_t)i * rs + (int64_t)j, bias ? __fadd_rn(acc[r], bias[j]) : acc[r]);
-        }
-    }
+// A product over no columns: the bias, or zero.
+__global__ void mx4_no_columns_kernel(uint64_t m, uint64_t n, const float *bias, void *out, int dtype, int64_t rs) {
+    const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < m * n; i += step)
+        store_any(out, dtype, (int64_t)(i / n) * rs + (int64_t)(i % n), bias ? bias[i % n] : 0.0f);
 }
 
 int grid_for(int device, uint64_t threads, uint32_t block) {
     const uint64_t want = (threads + block - 1) / block, most = (uint64_t)sm_count(device) * 16;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
-
-uint64_t code_bytes(uint64_t rows, uint64_t cols) { return rows * blocks_of(cols) * 16; }
-uint64_t scale_bytes(uint64_t rows, uint64_t cols) { return (rows + 127) / 128 * scale_tiles(cols) * 512; }
 
 snn_status_t check_source(const void *src, int dtype, snn_size_t rows, snn_size_t cols, int64_t rs, int64_t cs) {
     if (!is_dtype(dtype) || !offset_fits(rows, rs) || !offset_fits(cols, cs)) return SNN_ERR_INVALID_ARGUMENT;
@@ -161,18 +129,19 @@ void enqueue_quantize(int device, cudaStream_t s, const void *src, int dtype, ui
                                                                       (uint8_t *)scales);
 }
 
-void enqueue_matmul(cudaStream_t s, const void *xc, const void *xs, uint64_t m, const void *wc, const void *ws,
-                    uint64_t n, uint64_t k, const float *bias, void *out, int dtype, int64_t rs) {
-    const uint64_t rows = (m + 31) / 32;
-    const dim3 grid((uint32_t)((n + 31) / 32), (uint32_t)(rows < 65535 ? rows : 65535));
-    mx4_matmul_kernel<<<grid, dim3(32, 8), 0, s>>>((const uint8_t *)xc, (const uint8_t *)xs, m, (const uint8_t *)wc,
-                                                   (const uint8_t *)ws, n, k, bias, out, dtype, rs);
+cudaError_t enqueue_matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,
+                           void *out, int dtype, int64_t rs) {
+    if (k) return matmul(device, s, x, w, k, bias, out, dtype, rs);
+    mx4_no_columns_kernel<<<grid_for(device, x.rows * w.rows, 256), 256, 0, s>>>(x.rows, w.rows, bias, out, dtype, rs);
+    return cudaGetLastError();
 }
 
 }  // namespace
+}  // namespace mx4
 }  // namespace b200
 
 using namespace b200;
+using namespace b200::mx4;
 
 extern "C" {
 
@@ -227,9 +196,10 @@ snn_status_t snn_b200_mx4_matmul_async(int device, void *stream, const void *x_c
     if (m == 0 || n == 0) return SNN_OK;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
-    enqueue_matmul((cudaStream_t)stream, x_codes, x_scales, m, w_codes, w_scales, n, k, bias, out, out_dtype,
-                   out_row_stride);
-    return op_status(cudaGetLastError(), __func__);
+    const Packed x = {(const uint8_t *)x_codes, (const uint8_t *)x_scales, m};
+    const Packed w = {(const uint8_t *)w_codes, (const uint8_t *)w_scales, n};
+    return op_status(enqueue_matmul(device, (cudaStream_t)stream, x, w, k, bias, out, out_dtype, out_row_stride),
+                     __func__);
 }
 
 snn_size_t snn_b200_mx4_linear_workspace(snn_size_t m, snn_size_t k) {
@@ -253,11 +223,13 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
     if (m == 0 || n == 0) return SNN_OK;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
-    void *codes = workspace, *scales = (char *)workspace + code_bytes(m, k);
+    uint8_t *codes = (uint8_t *)workspace, *scales = codes + code_bytes(m, k);
     if (k) enqueue_quantize(device, (cudaStream_t)stream, x, x_dtype, m, k, x_row_stride, x_col_stride, codes, scales);
-    enqueue_matmul((cudaStream_t)stream, codes, scales, m, w_codes, w_scales, n, k, bias, out, out_dtype,
-                   out_row_stride);
-    return op_status(cudaGetLastError(), __func__);
+    cudaError_t e = cudaGetLastError();
+    const Packed xq = {codes, scales, m}, w = {(const uint8_t *)w_codes, (const uint8_t *)w_scales, n};
+    if (e == cudaSuccess)
+        e = enqueue_matmul(device, (cudaStream_t)stream, xq, w, k, bias, out, out_dtype, out_row_stride);
+    return op_status(e, __func__);
 }
 
 }  // extern "C"

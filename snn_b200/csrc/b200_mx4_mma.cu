@@ -1,0 +1,527 @@
+// The product of two packed 4-bit matrices on the tensor cores.
+//
+// tcgen05.mma kind::mxf4 multiplies 4-bit operands with a scale byte for every
+// 32 of them and adds in 32 bits in tensor memory, 64 of k an instruction. The
+// weights are the operand of 128 rows, x the one of BN rows, so an accumulator
+// lane is an output feature and a column a row of x: a warp reads 32
+// neighbouring features of a column at a time and writes them as one run, and
+// few rows of x cost a narrow instruction, not a padded one.
+//
+// A stage holds 256 of k: 128 bytes a row for both operands (TMA, 128-byte
+// swizzle) and their scales, which lie in memory as the 512-byte tiles that
+// tcgen05.cp spreads over the lanes (row r of a 128-row tile: lane r % 32,
+// column r / 32, a byte for each of 4 blocks). Rows and columns behind the
+// matrices are zero (TMA's fill, and the packer's for scales); a scale tile
+// that is not loaded belongs to k or rows that no instruction or store uses.
+//
+// One warp issues the loads, one the instructions; the others read the
+// accumulators and write. Two forms share this:
+//  * wide: BN = 256, a CTA an SM, tiles in turn; the accumulators are moved to
+//    registers and given back before they are written, so that the writes of
+//    a tile overlap the next one's instructions.
+//  * skinny: one tile a CTA and BN down to 16, the k of a tile split over the
+//    CTAs of a cluster, which add their parts through shared memory in the
+//    order of their ranks.
+// Every wait is bounded; one that gives up makes its tile NaN.
+#include "b200_mx4.h"
+
+#include <cuda.h>
+
+#include <algorithm>
+
+namespace b200 {
+namespace mx4 {
+namespace {
+
+constexpr uint32_t kRows = 128;        // weight rows of a tile
+constexpr uint32_t kStageK = 256;      // k of a stage
+constexpr uint32_t kStageBytes = 128;  // of a row
+constexpr uint32_t kScaleTile = 512;
+constexpr uint32_t kPolls = 1u << 24;
+
+__device__ __forceinline__ uint32_t smem_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- barriers ----
+__device__ __forceinline__ void bar_init(uint64_t *b, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_of(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_of(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
+    const uint32_t at = smem_of(b);
+    for (uint32_t i = 0; i < kPolls; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(at), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
+// ---- copies ----
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
+            "r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_of(bar))
+        : "memory");
+}
+__device__ __forceinline__ void load_run(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(smem_of(bar))
+                 : "memory");
+}
+
+// ---- tensor memory and instructions ----
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_of(slot)), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_of(bar))
+                 : "memory");
+}
+// Rows of 128 bytes in 8-row groups of 1024, swizzled by 128 bytes.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem) {
+    return (uint64_t)((smem & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+// 32 rows of 16 bytes, one behind the other.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
+    return (uint64_t)((smem & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_desc(smem)) : "memory");
+}
+// Both operands e2m1, K-major; scales ue8m0; 128 x n. The scale bytes of 64 of
+// k are the low or the high half of a scale column's word.
+__device__ __forceinline__ uint32_t instruction(uint32_t n, uint32_t half) {
+    return (half * 2u) << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (kRows >> 7) << 27 | (half * 2u) << 29;
+}
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                         bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"((uint32_t)add)
+        : "memory");
+}
+// 16 accumulator columns of the warp's 32 lanes.
+__device__ __forceinline__ void read_columns(uint32_t at, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void read_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Behind read_done: nothing that uses the columns moves before it.
+__device__ __forceinline__ void settle(float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[i]));
+}
+
+// ---- a tile's k loop ----
+template <uint32_t BN>
+struct Shape {
+    static constexpr uint32_t kScaleRows = (BN + 127) / 128;  // scale tiles across x's rows
+    static constexpr uint32_t kW = kRows * kStageBytes, kX = BN * kStageBytes;
+    static constexpr uint32_t kWScales = 2 * kScaleTile, kXScales = 2 * kScaleTile * kScaleRows;
+    static constexpr uint32_t kStage = kW + kX + kWScales + kXScales;  // a multiple of 1024
+    static constexpr uint32_t kScaleColumns = 8 + 8 * kScaleRows;      // tensor memory columns of a stage's scales
+    // Offsets of a stage's parts.
+    static constexpr uint32_t kAtX = kW, kAtWScales = kW + kX, kAtXScales = kW + kX + kWScales;
+};
+
+struct Problem {
+    const uint8_t *x_scales, *w_scales;
+    uint32_t m, n, k, scale_tiles;  // scale tiles along k
+    const float *bias;
+    void *out;
+    int64_t row_stride;
+    uint32_t tiles_n, tiles_m, splits, stages;  // stages along k
+};
+
+// Loads stage `at` (of k) of a tile into slot memory.
+template <uint32_t BN>
+__device__ __forceinline__ void load_stage(const Problem &p, const CUtensorMap *wm, const CUtensorMap *xm,
+                                           uint32_t slot, uint64_t *full, uint32_t at, uint32_t j0, uint32_t i0) {
+    using S = Shape<BN>;
+    const uint32_t tile = at * 2, bytes = kScaleTile * min(2u, p.scale_tiles - tile);
+    const uint32_t row_tiles = min(S::kScaleRows, (p.m + 127) / 128 - i0 / 128);
+    bar_expect(full, S::kW + S::kX + bytes * (1 + row_tiles));
+    load_box(slot, wm, (int32_t)(at * kStageBytes), (int32_t)j0, full);
+    load_box(slot + S::kAtX, xm, (int32_t)(at * kStageBytes), (int32_t)i0, full);
+    load_run(slot + S::kAtWScales, p.w_scales + ((uint64_t)(j0 / 128) * p.scale_tiles + tile) * kScaleTile, bytes, full);
+    for (uint32_t r = 0; r < row_tiles; ++r)
+        load_run(slot + S::kAtXScales + r * 2 * kScaleTile,
+                 p.x_scales + ((uint64_t)(i0 / 128 + r) * p.scale_tiles + tile) * kScaleTile, bytes, full);
+}
+
+// Issues a loaded stage's instructions. sf: tensor memory columns of its scales.
+template <uint32_t BN>
+__device__ __forceinline__ void multiply_stage(const Problem &p, uint32_t slot, uint32_t at, uint32_t d, uint32_t sf,
+                                               bool &add) {
+    using S = Shape<BN>;
+    const uint32_t pieces = min(kStageK / 64, (p.k - at * kStageK + 63) / 64);
+#pragma unroll
+    for (uint32_t t = 0; t < 2; ++t) {
+        copy_scales(sf + 4 * t, slot + S::kAtWScales + t * kScaleTile);
+#pragma unroll
+        for (uint32_t r = 0; r < S::kScaleRows; ++r)
+            copy_scales(sf + 8 + 4 * (t * S::kScaleRows + r), slot + S::kAtXScales + (r * 2 + t) * kScaleTile);
+    }
+    const uint64_t a = operand_desc(slot), b = operand_desc(slot + S::kAtX);
+    for (uint32_t q = 0; q < pieces; ++q) {
+        multiply(d, a + q * 2, b + q * 2, instruction(BN, q & 1), sf + 4 * (q / 2), sf + 8 + 4 * S::kScaleRows * (q / 2),
+                 add);
+        add = true;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void put(const Problem &p, uint32_t i, uint32_t j, float v) {
+    ((T *)p.out)[(int64_t)i * p.row_stride + j] = from_float<T>(v);
+}
+
+constexpr uint32_t kNoValue = 0x7fffffffu;
+
+// ---- wide form ----
+constexpr uint32_t kWideN = 256, kWideStages = 4, kWideThreads = 384;
+constexpr uint32_t kWideSmem = 1024 + kWideStages * Shape<kWideN>::kStage;
+
+template <typename T>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap wm, const __grid_constant__ CUtensorMap xm, Problem p) {
+    using S = Shape<kWideN>;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ uint64_t s_full[kWideStages], s_empty[kWideStages], s_ready, s_free;
+    __shared__ uint32_t s_tmem;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_of(s_raw) + 1023) & ~1023u;
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kWideStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
+        bar_init(&s_ready, 1);
+        bar_init(&s_free, 256);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(&s_tmem, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem, tiles = p.tiles_n * p.tiles_m;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t n = 0;  // stages so far
+            for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                const uint32_t j0 = tile % p.tiles_n * kRows, i0 = tile / p.tiles_n * kWideN;
+                for (uint32_t at = 0; ok && at < p.stages; ++at, ++n) {
+                    const uint32_t s = n % kWideStages, turn = n / kWideStages;
+                    ok = turn == 0 || bar_wait(&s_empty[s], (turn - 1) & 1);
+                    if (ok) load_stage<kWideN>(p, &wm, &xm, base + s * S::kStage, &s_full[s], at, j0, i0);
+                    else --n;
+                }
+            }
+            // Let the last copies land before the CTA may end.
+            for (uint32_t d = 1; d <= kWideStages && d <= n; ++d)
+                bar_wait(&s_full[(n - d) % kWideStages], ((n - d) / kWideStages) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t n = 0, count = 0;
+            for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++count) {
+                ok = count == 0 || bar_wait(&s_free, (count - 1) & 1);
+                fence_after();
+                bool add = false;
+                for (uint32_t at = 0; ok && at < p.stages; ++at, ++n) {
+                    const uint32_t s = n % kWideStages;
+                    ok = bar_wait(&s_full[s], (n / kWideStages) & 1);
+                    fence_after();
+                    if (!ok) break;
+                    multiply_stage<kWideN>(p, base + s * S::kStage, at, tmem, tmem + kWideN + s * S::kScaleColumns, add);
+                    commit(&s_empty[s]);
+                }
+                if (ok) commit(&s_ready);
+            }
+        }
+    } else if (warp >= 4) {
+        // Four warps share the lanes, two share the columns.
+        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+        uint32_t count = 0;
+        for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++count) {
+            const uint32_t j0 = tile % p.tiles_n * kRows, i0 = tile / p.tiles_n * kWideN;
+            const uint32_t j = j0 + quarter * 32 + lane;
+            const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
+            ok = ok && bar_wait(&s_ready, count & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            fence_after();
+            float v[kWideN / 2 / 16][16];
+#pragma unroll
+            for (uint32_t c = 0; c < kWideN / 2 / 16; ++c)
+                read_columns(tmem + (quarter * 32 << 16) + half * (kWideN / 2) + c * 16, v[c]);
+            read_done();
+#pragma unroll
+            for (uint32_t c = 0; c < kWideN / 2 / 16; ++c) settle(v[c]);
+            fence_before();
+            bar_arrive(&s_free);
+            if (j < p.n) {
+#pragma unroll
+                for (uint32_t c = 0; c < kWideN / 2 / 16; ++c)
+#pragma unroll
+                    for (uint32_t q = 0; q < 16; ++q) {
+                        const uint32_t i = i0 + half * (kWideN / 2) + c * 16 + q;
+                        if (i < p.m) put<T>(p, i, j, ok ? __fadd_rn(v[c][q], bias) : __uint_as_float(kNoValue));
+                    }
+            }
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+// ---- skinny form ----
+template <uint32_t BN>
+struct Skinny {
+    static constexpr uint32_t kStages = BN >= 128 ? 3 : BN >= 64 ? 4 : 5;  // two CTAs an SM
+    static constexpr uint32_t kSmem = 1024 + kStages * Shape<BN>::kStage;
+    static constexpr uint32_t kColumns = BN + kStages * Shape<BN>::kScaleColumns <= 128 ? 128 : 256;
+    static_assert(BN + kStages * Shape<BN>::kScaleColumns <= kColumns, "tensor memory");
+    static_assert(BN * kRows * 4 <= kStages * Shape<BN>::kStage, "the parts lie where the stages were");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float read_remote(uint32_t smem, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+template <typename T, uint32_t BN>
+__global__ void __launch_bounds__(128)
+    skinny_kernel(const __grid_constant__ CUtensorMap wm, const __grid_constant__ CUtensorMap xm, Problem p) {
+    using S = Shape<BN>;
+    using K = Skinny<BN>;
+    extern __shared__ uint8_t s_raw[];
+    __shared__ uint64_t s_full[K::kStages], s_empty[K::kStages], s_ready;
+    __shared__ uint32_t s_tmem;
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t base = (smem_of(s_raw) + 1023) & ~1023u;
+    const uint32_t rank = p.splits > 1 ? cluster_rank() : 0;
+    const uint32_t tile = blockIdx.x / p.splits;
+    const uint32_t j0 = tile % p.tiles_n * kRows, i0 = tile / p.tiles_n * BN;
+    // This CTA's stages along k.
+    const uint32_t first = (uint32_t)((uint64_t)p.stages * rank / p.splits);
+    const uint32_t count = (uint32_t)((uint64_t)p.stages * (rank + 1) / p.splits) - first;
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < K::kStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
+        bar_init(&s_ready, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(&s_tmem, K::kColumns);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem;
+    bool ok = true;
+    if (warp == 0 && lane == 0) {
+        uint32_t n = 0;
+        for (; ok && n < count; ++n) {
+            const uint32_t s = n % K::kStages, turn = n / K::kStages;
+            ok = turn == 0 || bar_wait(&s_empty[s], (turn - 1) & 1);
+            if (!ok) break;
+            load_stage<BN>(p, &wm, &xm, base + s * S::kStage, &s_full[s], first + n, j0, i0);
+        }
+        for (uint32_t d = 1; d <= K::kStages && d <= n; ++d)
+            bar_wait(&s_full[(n - d) % K::kStages], ((n - d) / K::kStages) & 1);
+    } else if (warp == 1 && lane == 0) {
+        bool add = false;
+        for (uint32_t n = 0; ok && n < count; ++n) {
+            const uint32_t s = n % K::kStages;
+            ok = bar_wait(&s_full[s], (n / K::kStages) & 1);
+            fence_after();
+            if (!ok) break;
+            multiply_stage<BN>(p, base + s * S::kStage, first + n, tmem, tmem + BN + s * S::kScaleColumns, add);
+            commit(&s_empty[s]);
+        }
+        if (ok) commit(&s_ready);
+    }
+    __syncwarp();
+    const uint32_t feature = warp * 32 + lane, j = j0 + feature;
+    const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
+    ok = bar_wait(&s_ready, 0);
+    ok = __all_sync(0xffffffffu, ok);
+    fence_after();
+    // All instructions are done, so the stages' memory is free.
+#pragma unroll 1
+    for (uint32_t c = 0; c < BN; c += 16) {
+        float v[16];
+        read_columns(tmem + (warp * 32 << 16) + c, v);
+        read_done();
+        settle(v);
+#pragma unroll
+        for (uint32_t q = 0; q < 16; ++q) {
+            const float part = ok ? v[q] : __uint_as_float(kNoValue);
+            if (p.splits > 1)
+                asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + ((c + q) * kRows + feature) * 4), "f"(part) : "memory");
+            else if (j < p.n && i0 + c + q < p.m)
+                put<T>(p, i0 + c + q, j, __fadd_rn(part, bias));
+        }
+    }
+    if (p.splits > 1) {
+        // Rank r adds up rows r, r + splits, ... of x.
+        cluster_sync();
+        for (uint32_t c = rank; c < BN && i0 + c < p.m; c += p.splits) {
+            float sum = 0.0f;
+            for (uint32_t r = 0; r < p.splits; ++r)
+                sum = __fadd_rn(sum, read_remote(base + (c * kRows + feature) * 4, r));
+            if (j < p.n) put<T>(p, i0 + c, j, __fadd_rn(sum, bias));
+        }
+        cluster_sync();
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        tmem_free(tmem, K::kColumns);
+    }
+}
+
+// ---- host side ----
+using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                            const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+    static Encode f = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (Encode)p;
+    }();
+    return f;
+}
+
+// Boxes of `box` rows and 128 bytes of a packed matrix.
+cudaError_t map_of(CUtensorMap *map, const Packed &q, uint64_t k, uint32_t box) {
+    const Encode f = encoder();
+    if (f == nullptr) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {blocks_of(k) * 16, q.rows}, strides[1] = {blocks_of(k) * 16};
+    const cuuint32_t boxes[2] = {kStageBytes, box}, steps[2] = {1, 1};
+    return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(q.codes), dims, strides, boxes, steps,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+template <typename T>
+cudaError_t launch_wide(int device, cudaStream_t s, const CUtensorMap &wm, const CUtensorMap &xm, const Problem &p) {
+    const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+    if (e != cudaSuccess) return e;
+    const uint32_t grid = std::min<uint64_t>((uint64_t)p.tiles_n * p.tiles_m, (uint64_t)sm_count(device));
+    wide_kernel<T><<<grid, kWideThreads, kWideSmem, s>>>(wm, xm, p);
+    return cudaGetLastError();
+}
+
+template <typename T, uint32_t BN>
+cudaError_t launch_skinny(cudaStream_t s, const CUtensorMap &wm, const CUtensorMap &xm, const Problem &p) {
+    using K = Skinny<BN>;
+    const cudaError_t e =
+        cudaFuncSetAttribute(skinny_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(p.tiles_n * p.tiles_m * p.splits);
+    c.blockDim = dim3(128);
+    c.dynamicSmemBytes = K::kSmem;
+    c.stream = s;
+    cudaLaunchAttribute cluster = {};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = p.splits;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    c.attrs = &cluster;
+    c.numAttrs = p.splits > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&c, skinny_kernel<T, BN>, wm, xm, p);
+}
+
+template <typename T>
+cudaError_t run(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, Problem &p) {
+    const uint64_t sms = (uint64_t)sm_count(device);
+    p.tiles_n = (uint32_t)((w.rows + kRows - 1) / kRows);
+    const uint64_t wide_tiles = p.tiles_n * ((x.rows + kWideN - 1) / kWideN);
+    CUtensorMap wm, xm;
+    cudaError_t e = map_of(&wm, w, k, kRows);
+    if (e != cudaSuccess) return e;
+    // Wide tiles where they fill the SMs, else narrower ones with k split.
+    if (x.rows > 128 && wide_tiles * 4 >= sms * 3) {
+        p.tiles_m = (uint32_t)((x.rows + kWideN - 1) / kWideN);
+        p.splits = 1;
+        e = map_of(&xm, x, k, kWideN);
+        return e != cudaSuccess ? e : launch_wide<T>(device, s, wm, xm, p);
+    }
+    const uint32_t bn = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : x.rows <= 64 ? 64 : 128;
+    p.tiles_m = (uint32_t)((x.rows + bn - 1) / bn);
+    // As many parts of k (of two stages at least) as two CTAs an SM hold at once.
+    uint32_t splits = 1;
+    while (splits < 8 && (uint64_t)p.tiles_n * p.tiles_m * splits * 2 <= sms * 2 && p.stages >= splits * 4) splits *= 2;
+    p.splits = splits;
+    e = map_of(&xm, x, k, bn);
+    if (e != cudaSuccess) return e;
+    switch (bn) {
+        case 16: return launch_skinny<T, 16>(s, wm, xm, p);
+        case 32: return launch_skinny<T, 32>(s, wm, xm, p);
+        case 64: return launch_skinny<T, 64>(s, wm, xm, p);
+        default: return launch_skinny<T, 128>(s, wm, xm, p);
+    }
+}
+
+}  // namespace
+
+cudaError_t matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,
+                   void *out, int dtype, int64_t row_stride) {
+    Problem p = {};
+    p.x_scales = x.scales, p.w_scales = w.scales;
+    p.m = (uint32_t)x.rows, p.n = (uint32_t)w.rows, p.k = (uint32_t)k;
+    p.scale_tiles = (uint32_t)scale_tiles(k);
+    p.bias = bias, p.out = out, p.row_stride = row_stride;
+    p.stages = (uint32_t)((k + kStageK - 1) / kStageK);
+    switch (dtype) {
+        case SNN_B200_F32: return run<float>(device, s, x, w, k, p);
+        case SNN_B200_F16: return run<__half>(device, s, x, w, k, p);
+        default: return run<__nv_bfloat16>(device, s, x, w, k, p);
+    }
+}
+
+}  // namespace mx4
+}  // namespace b200

@@ -558,8 +558,8 @@ typedef struct snn_b200_leaky {
 } snn_b200_leaky_t;
 
 /* What the backward pass needs beside x and the gate: the state before every
- * 16th step, floats [batch, ceil(steps / 16), channels]. */
-#define SNN_B200_LEAKY_BLOCK 16u
+ * 8th step, floats [batch, ceil(steps / 8), channels]. */
+#define SNN_B200_LEAKY_BLOCK 8u
 snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_size_t channels);
 /* Bytes of workspace (16-byte aligned) of the forward and of the backward call. */
 snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *leaky);

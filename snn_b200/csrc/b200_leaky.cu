@@ -78,11 +78,12 @@ struct Plan {
     uint64_t zeroed;  // bytes of ticket and flags, at the start
     uint64_t aggregates, states, partial, bytes;
 };
-// `width` channels a thread; the workspace is sized for either width.
-Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
+// `width` channels a thread, `warps` in a tile; the workspace is sized for the largest.
+Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, uint32_t warps) {
+    const uint32_t tile = warps * kSteps;
     Plan p = {};
     p.flat = q.batch * q.channels;
-    p.tiles = (uint32_t)((q.steps + kTile - 1) / kTile);
+    p.tiles = (uint32_t)((q.steps + tile - 1) / tile);
     const uint64_t supers = p.tiles / kSuper, columns = (p.flat + 32 * width - 1) / (32 * width);
     const auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
     p.zeroed = round((1 + ((uint64_t)p.tiles + supers) * columns) * 4);
@@ -149,8 +150,10 @@ snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_s
 
 snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *q) {
     if (q == nullptr || q->batch > kMaxCount || q->steps > kMaxCount || q->channels > kMaxCount) return 0;
-    const uint64_t one = plan_of(*q, 1).bytes, two = plan_of(*q, 2).bytes;
-    return one > two ? one : two;
+    uint64_t most = 0;
+    for (uint32_t width = 1; width <= 2; ++width)
+        for (const uint32_t warps : {kScanWarps, kBackWarps}) most = std::max(most, plan_of(*q, width, warps).bytes);
+    return most;
 }
 
 snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,
@@ -179,7 +182,7 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
                       pairs(y, dtype_bytes(q.y_dtype), q.y_batch_stride, q.y_step_stride) && float_pairs(h0) &&
                       float_pairs(h_last) && float_pairs(saved);
     const uint32_t width = even ? 2 : 1;
-    const Plan p = plan_of(q, width);
+    const Plan p = plan_of(q, width, kScanWarps);
     const Form f = {q.gate_dtype, q.y_dtype, gate && q.gate_step_stride, wants_split(device, p, width, q.steps), width};
     Args g = {};
     fill(g, q, p, width, workspace);
@@ -237,7 +240,7 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
                       (!every || pairs(dgate, dtype_bytes(q.gate_dtype), q.dgate_batch_stride, q.dgate_step_stride)) &&
                       float_pairs(dh_last) && float_pairs(dh0) && float_pairs(saved);
     const uint32_t width = even ? 2 : 1;
-    const Plan p = plan_of(q, width);
+    const Plan p = plan_of(q, width, kBackWarps);
     const Form f = {q.gate_dtype, q.y_dtype, every, wants_split(device, p, width, q.steps), width};
     Args g = {};
     fill(g, q, p, width, workspace);

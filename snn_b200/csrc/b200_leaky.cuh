@@ -7,8 +7,7 @@
 //
 //  * whole: a warp walks through all steps of its channels, kSteps at a time,
 //    with the state in registers.
-//  * split: a CTA takes one tile of kTile steps (its warps one block of kSteps
-//    each). Steps compose as affine maps h -> A h + H, so each tile publishes
+//  * split: a CTA takes one tile of steps (its warps one block of kSteps each). Steps compose as affine maps h -> A h + H, so each tile publishes
 //    its (A, H) at once and then folds the maps of the tiles before it onto
 //    the last published state. States are published every kSuper tiles, so a
 //    tile waits for fewer than kSuper neighbours and one state, always in the
@@ -33,6 +32,105 @@ struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
 
+// Arithmetic on a thread's channels, two at a time where there are two: the
+// kernels' instruction count, not their arithmetic, is what is scarce.
+template <int V>
+using Row = Vec<float, V>;
+template <int V>
+__device__ __forceinline__ uint64_t two(const Row<V> &a, int q) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[q]), "f"(a.v[q + 1]));
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void split(uint64_t r, Row<V> &o, int q) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(o.v[q]), "=f"(o.v[q + 1]) : "l"(r));
+}
+template <int V>
+__device__ __forceinline__ Row<V> fma(const Row<V> &a, const Row<V> &b, const Row<V> &c) {
+    Row<V> o;
+    if constexpr (V == 1) {
+        o.v[0] = __fmaf_rn(a.v[0], b.v[0], c.v[0]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < V; q += 2) {
+            uint64_t r;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a, q)), "l"(two(b, q)), "l"(two(c, q)));
+            split(r, o, q);
+        }
+    }
+    return o;
+}
+template <int V>
+__device__ __forceinline__ Row<V> mul(const Row<V> &a, const Row<V> &b) {
+    Row<V> o;
+    if constexpr (V == 1) {
+        o.v[0] = __fmul_rn(a.v[0], b.v[0]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < V; q += 2) {
+            uint64_t r;
+            asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a, q)), "l"(two(b, q)));
+            split(r, o, q);
+        }
+    }
+    return o;
+}
+template <int V>
+__device__ __forceinline__ Row<V> add(const Row<V> &a, const Row<V> &b) {
+    Row<V> o;
+    if constexpr (V == 1) {
+        o.v[0] = __fadd_rn(a.v[0], b.v[0]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < V; q += 2) {
+            uint64_t r;
+            asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a, q)), "l"(two(b, q)));
+            split(r, o, q);
+        }
+    }
+    return o;
+}
+template <int V>
+__device__ __forceinline__ Row<V> all(float f) {
+    Row<V> o;
+#pragma unroll
+    for (int q = 0; q < V; ++q) o.v[q] = f;
+    return o;
+}
+template <typename T, int V>
+__device__ __forceinline__ Row<V> widen(const Vec<T, V> &a) {
+    Row<V> o;
+#pragma unroll
+    for (int q = 0; q < V; ++q) o.v[q] = to_float(a.v[q]);
+    return o;
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow(const Row<V> &a) {
+    Vec<T, V> o;
+    if constexpr (V > 1 && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int q = 0; q < V; q += 2)
+            *reinterpret_cast<__nv_bfloat162 *>(&o.v[q]) = __floats2bfloat162_rn(a.v[q], a.v[q + 1]);
+    } else if constexpr (V > 1 && std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int q = 0; q < V; q += 2)
+            *reinterpret_cast<__half2 *>(&o.v[q]) = __floats2half2_rn(a.v[q], a.v[q + 1]);
+    } else {
+#pragma unroll
+        for (int q = 0; q < V; ++q) o.v[q] = from_float<T>(a.v[q]);
+    }
+    return o;
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load(const T *p) {
+    return *reinterpret_cast<const Vec<T, V> *>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
+    *reinterpret_cast<Vec<T, V> *>(p) = v;
+}
+
 // No gate array, or one without a step stride: the gate is a constant of the thread.
 struct Fixed {};
 
@@ -40,12 +138,24 @@ struct Leak {
     float a, rest;  // the gate and one minus it
 };
 // Both from one exponential of a non-positive number, so that neither is a
-// difference of nearly equal values.
+// difference of nearly equal values. A 16-bit logit has a rounding of 2^-9 of
+// itself, so for it the product with log2(e) is rounded once to 32 bits (2^-20
+// of the exponential up to logits of 22).
+template <bool Narrow>
 __device__ __forceinline__ Leak leak_of(float z, int logit) {
     if (!logit) return {z, __fsub_rn(1.0f, z)};
-    const float t = expf(-fabsf(z));
+    float t;
+    if (Narrow) {
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmul_rn(-fabsf(z), 1.44269504f)));
+    } else {
+        t = expf(-fabsf(z));
+    }
     const float r = __fdividef(1.0f, __fadd_rn(1.0f, t)), q = __fmul_rn(t, r);
     return z >= 0.0f ? Leak{r, q} : Leak{q, r};
+}
+template <typename G>
+__device__ __forceinline__ Leak leak_from(G z, int logit) {
+    return leak_of<sizeof(G) == 2>(to_float(z), logit);
 }
 
 __device__ __forceinline__ uint32_t load_acquire(const uint32_t *p) {
@@ -87,51 +197,56 @@ __device__ __forceinline__ int live_steps(uint32_t len, uint32_t t0) {
     return len <= t0 ? 0 : (int)min(len - t0, kSteps);
 }
 
+// kSteps rows, all of them wanted by most threads.
 template <typename T, int V>
 __device__ __forceinline__ void load_steps(Vec<T, V> (&r)[kSteps], const T *p, int64_t stride, int live) {
+    if (live == (int)kSteps) {
 #pragma unroll
-    for (int j = 0; j < (int)kSteps; ++j)
-        if (j < live) r[j] = *reinterpret_cast<const Vec<T, V> *>(p + j * stride);
-        else r[j] = Vec<T, V>{};
+        for (int j = 0; j < (int)kSteps; ++j) r[j] = load<T, V>(p + j * stride);
+    } else {
+#pragma unroll
+        for (int j = 0; j < (int)kSteps; ++j) r[j] = j < live ? load<T, V>(p + j * stride) : Vec<T, V>{};
+    }
 }
 
 // The gates of a thread's steps. Fixed gates are kept once.
 template <typename G, int V>
 struct Gates {
     Vec<G, V> raw[kSteps];
+    __device__ __forceinline__ void init(const Args &, const Place &) {}
     __device__ __forceinline__ void load(const Args &g, const Place &p, uint32_t t0, int live) {
         load_steps<G, V>(raw, (const G *)g.gate + p.b * g.gb + (int64_t)t0 * g.gt + p.c, g.gt, live);
     }
-    __device__ __forceinline__ Leak at(const Args &g, int j, int q) const {
-        return leak_of(to_float(raw[j].v[q]), g.logit);
+    __device__ __forceinline__ void at(const Args &g, int j, Row<V> &a, Row<V> &rest) const {
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const Leak l = leak_from(raw[j].v[q], g.logit);
+            a.v[q] = l.a, rest.v[q] = l.rest;
+        }
     }
 };
 template <int V>
 struct Gates<Fixed, V> {
-    Leak leak[V];
+    Row<V> a_, rest_;
     __device__ __forceinline__ void init(const Args &g, const Place &p) {
 #pragma unroll
-        for (int q = 0; q < V; ++q)
-            leak[q] = !g.gate ? Leak{g.decay, __fsub_rn(1.0f, g.decay)}
-                              : p.on ? leak_of(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit) : Leak{1.0f, 0.0f};
+        for (int q = 0; q < V; ++q) {
+            const Leak l = !g.gate ? Leak{g.decay, __fsub_rn(1.0f, g.decay)}
+                           : p.on  ? leak_from(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit)
+                                   : Leak{1.0f, 0.0f};
+            a_.v[q] = l.a, rest_.v[q] = l.rest;
+        }
     }
     __device__ __forceinline__ void load(const Args &, const Place &, uint32_t, int) {}
-    __device__ __forceinline__ Leak at(const Args &, int, int q) const { return leak[q]; }
+    __device__ __forceinline__ void at(const Args &, int, Row<V> &a, Row<V> &rest) const { a = a_, rest = rest_; }
 };
-template <typename G, int V>
-__device__ __forceinline__ void init_gates(Gates<G, V> &, const Args &, const Place &) {}
-template <int V>
-__device__ __forceinline__ void init_gates(Gates<Fixed, V> &k, const Args &g, const Place &p) {
-    k.init(g, p);
-}
 
 template <int V>
-__device__ __forceinline__ Vec<float, V> load_state(const float *p, uint64_t i, bool on) {
-    return on && p ? *reinterpret_cast<const Vec<float, V> *>(p + i) : Vec<float, V>{};
+__device__ __forceinline__ Row<V> load_state(const float *p, uint64_t i, bool on) {
+    return on && p ? load<float, V>(p + i) : Row<V>{};
 }
 
 // The state before a block of steps, kept for the backward pass.
-template <int V>
 __device__ __forceinline__ float *saved_at(const Args &g, const Place &p, uint32_t t0) {
     const uint32_t blocks = (g.steps + kSteps - 1) / kSteps;
     return g.saved + ((uint64_t)p.b * blocks + t0 / kSteps) * g.channels + p.c;
@@ -139,57 +254,70 @@ __device__ __forceinline__ float *saved_at(const Args &g, const Place &p, uint32
 
 // Walks a thread's steps from state h on, writing y.
 template <typename Y, int V>
-__device__ __forceinline__ void emit(const Args &g, const Place &p, uint32_t t0, int live,
-                                     const float (&a)[kSteps][V], const float (&u)[kSteps][V], Vec<float, V> &h) {
+__device__ __forceinline__ void emit(const Args &g, const Place &p, uint32_t t0, int live, const Row<V> (&a)[kSteps],
+                                     const Row<V> (&u)[kSteps], Row<V> &h) {
     if (!p.on) return;
-    if (g.saved) *reinterpret_cast<Vec<float, V> *>(saved_at<V>(g, p, t0)) = h;
+    if (g.saved) store<float, V>(saved_at(g, p, t0), h);
     Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
-    const int rows = (int)min(g.steps - t0, kSteps);
+    if (live == (int)kSteps) {
 #pragma unroll
-    for (int j = 0; j < (int)kSteps; ++j) {
-        Vec<Y, V> o;
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            h.v[q] = __fmaf_rn(a[j][q], h.v[q], u[j][q]);
-            o.v[q] = from_float<Y>(j < live ? h.v[q] : 0.0f);
+        for (int j = 0; j < (int)kSteps; ++j) {
+            h = fma(a[j], h, u[j]);
+            store<Y, V>(y + j * g.yt, narrow<Y, V>(h));
         }
-        if (j < rows) *reinterpret_cast<Vec<Y, V> *>(y + j * g.yt) = o;
+    } else {
+        const int rows = (int)min(g.steps - t0, kSteps);
+#pragma unroll
+        for (int j = 0; j < (int)kSteps; ++j) {
+            h = fma(a[j], h, u[j]);
+            if (j < rows) store<Y, V>(y + j * g.yt, j < live ? narrow<Y, V>(h) : Vec<Y, V>{});
+        }
     }
 }
 
-// Gates and inputs of a thread's steps; rows behind the sequence keep the state (a = 1, u = 0).
+// What a block reads, before it is worked on.
 template <typename X, typename G, int V>
-__device__ __forceinline__ void gather(const Args &g, const Place &p, uint32_t t0, int live, Gates<G, V> &gates,
-                                       float (&a)[kSteps][V], float (&u)[kSteps][V]) {
+struct Inputs {
+    Gates<G, V> gates;
     Vec<X, V> x[kSteps];
-    gates.load(g, p, t0, live);
-    load_steps<X, V>(x, (const X *)g.x + p.b * g.xb + (int64_t)t0 * g.xt + p.c, g.xt, live);
+    __device__ __forceinline__ void load(const Args &g, const Place &p, uint32_t t0, int live) {
+        gates.load(g, p, t0, live);
+        load_steps<X, V>(x, (const X *)g.x + p.b * g.xb + (int64_t)t0 * g.xt + p.c, g.xt, live);
+    }
+    // Gates and inputs of the steps; rows behind the sequence keep the state (a = 1, u = 0).
+    __device__ __forceinline__ void maps(const Args &g, int live, Row<V> (&a)[kSteps], Row<V> (&u)[kSteps]) const {
+        const Row<V> scale = all<V>(g.scale);
 #pragma unroll
-    for (int j = 0; j < (int)kSteps; ++j)
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            const Leak l = gates.at(g, j, q);
-            float v = __fmul_rn(g.scale, to_float(x[j].v[q]));
-            if (g.complement) v = __fmul_rn(v, l.rest);
-            a[j][q] = j < live ? l.a : 1.0f;
-            u[j][q] = j < live ? v : 0.0f;
+        for (int j = 0; j < (int)kSteps; ++j) {
+            Row<V> rest;
+            gates.at(g, j, a[j], rest);
+            u[j] = mul(scale, widen(x[j]));
+            if (g.complement) u[j] = mul(u[j], rest);
         }
-}
+        if (live < (int)kSteps) {
+#pragma unroll
+            for (int j = 0; j < (int)kSteps; ++j)
+                if (j >= live) a[j] = all<V>(1.0f), u[j] = all<V>(0.0f);
+        }
+    }
+};
 
 template <typename X, typename G, typename Y, int V>
 __global__ void __launch_bounds__(128) scan_whole_kernel(Args g) {
     const Place p = place_of<V>(g, (uint64_t)blockIdx.x * 4 + threadIdx.x / 32);
     if (!p.on) return;
-    Gates<G, V> gates;
-    init_gates(gates, g, p);
-    Vec<float, V> h = load_state<V>(g.h0, p.i, true);
+    Inputs<X, G, V> in;
+    in.gates.init(g, p);
+    Row<V> h = load_state<V>(g.h0, p.i, true);
+    in.load(g, p, 0, live_steps(p.len, 0));
     for (uint32_t t0 = 0; t0 < g.steps; t0 += kSteps) {
-        float a[kSteps][V], u[kSteps][V];
+        Row<V> a[kSteps], u[kSteps];
         const int live = live_steps(p.len, t0);
-        gather<X, G, V>(g, p, t0, live, gates, a, u);
+        in.maps(g, live, a, u);
+        if (t0 + kSteps < g.steps) in.load(g, p, t0 + kSteps, live_steps(p.len, t0 + kSteps));  // on the way while this block is written
         emit<Y, V>(g, p, t0, live, a, u, h);
     }
-    if (g.h_last) *reinterpret_cast<Vec<float, V> *>(g.h_last + p.i) = h;
+    if (g.h_last) store<float, V>(g.h_last + p.i, h);
 }
 
 // ---- split form ----
@@ -204,9 +332,9 @@ __device__ __forceinline__ Tile take_tile(const Args &g) {
     return {s_ticket / g.columns, s_ticket % g.columns};
 }
 
-template <int V>
+template <int V, uint32_t W>
 struct Exchange {
-    float2 map[kWarps][32 * V];  // each warp's (A, H)
+    float2 map[W][32 * V];  // each warp's (A, H)
     float state[32 * V];         // the state that enters the tile
 };
 
@@ -214,8 +342,8 @@ struct Exchange {
 // the state that enters tile 0. Warp w's own map is in ex.map[w]; `order`
 // gives the warps in the direction of the walk. On return (after a barrier)
 // ex.state is set.
-template <int V, bool Reverse>
-__device__ __forceinline__ void link_tiles(const Args &g, const Tile &tile, Exchange<V> &ex, const float *first,
+template <int V, uint32_t W, bool Reverse>
+__device__ __forceinline__ void link_tiles(const Args &g, const Tile &tile, Exchange<V, W> &ex, const float *first,
                                            bool on, uint64_t i) {
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const uint64_t width = (uint64_t)g.columns * 32 * V, at = tile.column * 32 * V + lane * V;
@@ -228,8 +356,8 @@ __device__ __forceinline__ void link_tiles(const Args &g, const Tile &tile, Exch
         for (int q = 0; q < V; ++q) {
             m[q] = make_float2(1.0f, 0.0f);
 #pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) {
-                const float2 n = ex.map[Reverse ? kWarps - 1 - w : w][lane * V + q];
+            for (uint32_t w = 0; w < W; ++w) {
+                const float2 n = ex.map[Reverse ? W - 1 - w : w][lane * V + q];
                 m[q] = make_float2(__fmul_rn(n.x, m[q].x), __fmaf_rn(n.x, m[q].y, n.y));
             }
         }
@@ -276,28 +404,28 @@ __device__ __forceinline__ void link_tiles(const Args &g, const Tile &tile, Exch
 }
 
 template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(kWarps * 32, 2) scan_split_kernel(Args g) {
-    __shared__ Exchange<V> ex;
+__global__ void __launch_bounds__(kScanWarps * 32) scan_split_kernel(Args g) {
+    __shared__ Exchange<V, kScanWarps> ex;
     const Tile tile = take_tile(g);
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const Place p = place_of<V>(g, tile.column);
-    const uint32_t t0 = tile.k * kTile + warp * kSteps;
-    Gates<G, V> gates;
-    init_gates(gates, g, p);
-    float a[kSteps][V], u[kSteps][V];
+    const uint32_t t0 = (tile.k * kScanWarps + warp) * kSteps;
+    Row<V> a[kSteps], u[kSteps];
     const int live = live_steps(p.len, t0);
-    gather<X, G, V>(g, p, t0, live, gates, a, u);
-#pragma unroll
-    for (int q = 0; q < V; ++q) {
-        float2 m = make_float2(1.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j)
-            m = make_float2(__fmul_rn(a[j][q], m.x), __fmaf_rn(a[j][q], m.y, u[j][q]));
-        ex.map[warp][lane * V + q] = m;
+    {
+        Inputs<X, G, V> in;
+        in.gates.init(g, p);
+        in.load(g, p, t0, live);
+        in.maps(g, live, a, u);
     }
+    Row<V> A = all<V>(1.0f), H = all<V>(0.0f);
+#pragma unroll
+    for (int j = 0; j < (int)kSteps; ++j) A = mul(a[j], A), H = fma(a[j], H, u[j]);
+#pragma unroll
+    for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q] = make_float2(A.v[q], H.v[q]);
     __syncthreads();
-    link_tiles<V, false>(g, tile, ex, g.h0, p.on, p.i);
-    Vec<float, V> h;
+    link_tiles<V, kScanWarps, false>(g, tile, ex, g.h0, p.on, p.i);
+    Row<V> h;
 #pragma unroll
     for (int q = 0; q < V; ++q) {
         h.v[q] = ex.state[lane * V + q];
@@ -307,8 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_split_kernel(Args g) {
         }
     }
     if (t0 < g.steps) emit<Y, V>(g, p, t0, live, a, u, h);
-    if (g.h_last && p.on && tile.k + 1 == g.tiles && warp + 1 == kWarps)
-        *reinterpret_cast<Vec<float, V> *>(g.h_last + p.i) = h;
+    if (g.h_last && p.on && tile.k + 1 == g.tiles && warp + 1 == kScanWarps) store<float, V>(g.h_last + p.i, h);
 }
 
 // ---- gradient ----
@@ -327,63 +454,69 @@ struct GradientOf<Spike> {
 
 template <typename X, typename G, typename Y, int V>
 struct Back {
-    Gates<G, V> gates;
-    float a[kSteps][V], rest[kSteps][V], dy[kSteps][V], k[kSteps][V];  // k: what d is multiplied with
+    Inputs<X, G, V> in;
+    Vec<Y, V> dy[kSteps];
+    Row<V> h;
+    Row<V> a[kSteps], rest[kSteps], k[kSteps];  // k: what d is multiplied with
 
-    __device__ __forceinline__ void gather(const Args &g, const Place &p, uint32_t t0, int live) {
-        Vec<X, V> x[kSteps];
-        Vec<Y, V> d[kSteps];
-        gates.load(g, p, t0, live);
-        load_steps<X, V>(x, (const X *)g.x + p.b * g.xb + (int64_t)t0 * g.xt + p.c, g.xt, live);
-        load_steps<Y, V>(d, (const Y *)g.dy + p.b * g.dyb + (int64_t)t0 * g.dyt + p.c, g.dyt, live);
-        Vec<float, V> h = live ? *reinterpret_cast<const Vec<float, V> *>(saved_at<V>(g, p, t0)) : Vec<float, V>{};
+    __device__ __forceinline__ void load(const Args &g, const Place &p, uint32_t t0, int live) {
+        in.load(g, p, t0, live);
+        load_steps<Y, V>(dy, (const Y *)g.dy + p.b * g.dyb + (int64_t)t0 * g.dyt + p.c, g.dyt, live);
+        h = live ? leaky::load<float, V>(saved_at(g, p, t0)) : Row<V>{};
+    }
+    __device__ __forceinline__ void maps(const Args &g, int live) {
+        const Row<V> scale = all<V>(g.scale);
 #pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j)
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                const Leak l = gates.at(g, j, q);
-                const float v = __fmul_rn(g.scale, to_float(x[j].v[q]));
-                k[j][q] = g.complement ? __fsub_rn(h.v[q], v) : h.v[q];
-                h.v[q] = __fmaf_rn(l.a, h.v[q], g.complement ? __fmul_rn(v, l.rest) : v);
-                a[j][q] = j < live ? l.a : 1.0f;
-                rest[j][q] = l.rest;
-                dy[j][q] = to_float(d[j].v[q]);
+        for (int j = 0; j < (int)kSteps; ++j) {
+            in.gates.at(g, j, a[j], rest[j]);
+            const Row<V> v = mul(scale, widen(in.x[j]));
+            if (g.complement) {
+                k[j] = add(h, mul(all<V>(-1.0f), v));
+                h = fma(a[j], h, mul(v, rest[j]));
+            } else {
+                k[j] = h;
+                h = fma(a[j], h, v);
             }
+        }
+        if (live < (int)kSteps) {
+#pragma unroll
+            for (int j = 0; j < (int)kSteps; ++j)
+                if (j >= live) a[j] = all<V>(1.0f);
+        }
+    }
+    // One step back: d and e before it.
+    __device__ __forceinline__ Row<V> step(int j, int live, Row<V> &e) const {
+        const Row<V> d = add(widen(dy[j]), e);
+        if (j < live) e = mul(a[j], d);
+        return d;
     }
     // Walks back from e, writes dx and the gradient of a gate with a value
     // for every step, and returns the block's sum of da in sum.
-    __device__ __forceinline__ void emit(const Args &g, const Place &p, uint32_t t0, int live, Vec<float, V> &e,
-                                         float (&sum)[V]) {
+    __device__ __forceinline__ void emit(const Args &g, const Place &p, uint32_t t0, int live, Row<V> &e,
+                                         Row<V> &sum) {
         using D = typename GradientOf<X>::type;
         constexpr bool every = !std::is_same<G, Fixed>::value;
         D *dx = (D *)g.dx + p.b * g.dxb + (int64_t)t0 * g.dxt + p.c;
-        const int rows = t0 < g.steps ? (int)min(g.steps - t0, kSteps) : 0;
-#pragma unroll
-        for (int q = 0; q < V; ++q) sum[q] = 0.0f;
+        const int rows = !p.on || t0 >= g.steps ? 0 : (int)min(g.steps - t0, kSteps);
+        const Row<V> scale = all<V>(g.scale);
+        sum = all<V>(0.0f);
 #pragma unroll
         for (int j = (int)kSteps - 1; j >= 0; --j) {
-            Vec<D, V> ox;
-            Vec<float, V> oz;
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                const bool on = j < live;
-                const float d = __fadd_rn(dy[j][q], e.v[q]);
-                e.v[q] = __fmul_rn(a[j][q], on ? d : e.v[q]);
-                const float f = g.complement ? __fmul_rn(d, rest[j][q]) : d;
-                ox.v[q] = from_float<D>(on ? __fmul_rn(g.scale, f) : 0.0f);
-                const float z = on ? __fmul_rn(d, k[j][q]) : 0.0f;
-                if (every) oz.v[q] = g.logit && on ? __fmul_rn(z, __fmul_rn(a[j][q], rest[j][q])) : z;
-                else sum[q] = __fadd_rn(sum[q], z);
+            const bool on = j < live;
+            const Row<V> d = step(j, live, e);
+            Row<V> z = mul(d, k[j]);
+            if (!every && on) sum = add(sum, z);
+            if (j >= rows) continue;
+            if (g.dx) {
+                Row<V> f = mul(scale, d);
+                if (g.complement) f = mul(f, rest[j]);
+                store<D, V>(dx + j * g.dxt, on ? narrow<D, V>(f) : Vec<D, V>{});
             }
-            if (p.on && j < rows) {
-                if (g.dx) *reinterpret_cast<Vec<D, V> *>(dx + j * g.dxt) = ox;
-                if constexpr (every) {
-                    if (g.dgate) {
-                        Vec<G, V> o;
-#pragma unroll
-                        for (int q = 0; q < V; ++q) o.v[q] = from_float<G>(oz.v[q]);
-                        *reinterpret_cast<Vec<G, V> *>((G *)g.dgate + p.b * g.dgb + (int64_t)(t0 + j) * g.dgt + p.c) = o;
-                    }
+            if constexpr (every) {
+                if (g.dgate) {
+                    if (g.logit) z = mul(z, mul(a[j], rest[j]));
+                    store<G, V>((G *)g.dgate + p.b * g.dgb + (int64_t)(t0 + j) * g.dgt + p.c,
+                                on ? narrow<G, V>(z) : Vec<G, V>{});
                 }
             }
         }
@@ -393,90 +526,85 @@ struct Back {
 // A shared gate's sum for one thread: of logits, the gate's own slope is a common factor.
 template <int V>
 __device__ __forceinline__ void put_partial(const Args &g, const Place &p, const Gates<Fixed, V> &gates, uint32_t tile,
-                                            const float (&sum)[V]) {
-#pragma unroll
-    for (int q = 0; q < V; ++q)
-        g.partial[tile * g.flat + p.i + q] =
-            g.logit && g.gate ? __fmul_rn(sum[q], __fmul_rn(gates.leak[q].a, gates.leak[q].rest)) : sum[q];
+                                            const Row<V> &sum) {
+    store<float, V>(g.partial + tile * g.flat + p.i, g.logit ? mul(sum, mul(gates.a_, gates.rest_)) : sum);
 }
 template <typename G, int V>
 __device__ __forceinline__ void put_partial(const Args &, const Place &, const Gates<G, V> &, uint32_t,
-                                            const float (&)[V]) {}
+                                            const Row<V> &) {}
 
 template <typename X, typename G, typename Y, int V>
 __global__ void __launch_bounds__(128) back_whole_kernel(Args g) {
     const Place p = place_of<V>(g, (uint64_t)blockIdx.x * 4 + threadIdx.x / 32);
     if (!p.on) return;
     Back<X, G, Y, V> w;
-    init_gates(w.gates, g, p);
-    Vec<float, V> e = load_state<V>(g.dh_last, p.i, true);
+    w.in.gates.init(g, p);
+    Row<V> e = load_state<V>(g.dh_last, p.i, true);
     double total[V] = {};
     for (uint32_t n = (g.steps + kSteps - 1) / kSteps; n-- > 0;) {
         const uint32_t t0 = n * kSteps;
         const int live = live_steps(p.len, t0);
-        float sum[V];
-        w.gather(g, p, t0, live);
+        Row<V> sum;
+        w.load(g, p, t0, live);
+        w.maps(g, live);
         w.emit(g, p, t0, live, e, sum);
         if (std::is_same<G, Fixed>::value)
 #pragma unroll
-            for (int q = 0; q < V; ++q) total[q] += (double)sum[q];
+            for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
     }
-    if (g.dh0) *reinterpret_cast<Vec<float, V> *>(g.dh0 + p.i) = e;
+    if (g.dh0) store<float, V>(g.dh0 + p.i, e);
     if (g.partial) {
-        float sum[V];
+        Row<V> sum;
 #pragma unroll
-        for (int q = 0; q < V; ++q) sum[q] = (float)total[q];
-        put_partial(g, p, w.gates, 0, sum);
+        for (int q = 0; q < V; ++q) sum.v[q] = (float)total[q];
+        put_partial(g, p, w.in.gates, 0, sum);
     }
 }
 
 template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(kWarps * 32) back_split_kernel(Args g) {
-    __shared__ Exchange<V> ex;
+__global__ void __launch_bounds__(kBackWarps * 32) back_split_kernel(Args g) {
+    __shared__ Exchange<V, kBackWarps> ex;
     const Tile tile = take_tile(g);
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const Place p = place_of<V>(g, tile.column);
-    const uint32_t t0 = (g.tiles - 1 - tile.k) * kTile + warp * kSteps;
+    const uint32_t t0 = ((g.tiles - 1 - tile.k) * kBackWarps + warp) * kSteps;
     Back<X, G, Y, V> w;
-    init_gates(w.gates, g, p);
+    w.in.gates.init(g, p);
     const int live = live_steps(p.len, t0);
-    w.gather(g, p, t0, live);
+    w.load(g, p, t0, live);
+    w.maps(g, live);
+    Row<V> A = all<V>(1.0f), E = all<V>(0.0f);
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-        float2 m = make_float2(1.0f, 0.0f);
+    for (int j = (int)kSteps - 1; j >= 0; --j) A = mul(w.a[j], A), w.step(j, live, E);
 #pragma unroll
-        for (int j = (int)kSteps - 1; j >= 0; --j)
-            m = make_float2(__fmul_rn(w.a[j][q], m.x),
-                            __fmul_rn(w.a[j][q], j < live ? __fadd_rn(m.y, w.dy[j][q]) : m.y));
-        ex.map[warp][lane * V + q] = m;
-    }
+    for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q] = make_float2(A.v[q], E.v[q]);
     __syncthreads();
-    link_tiles<V, true>(g, tile, ex, g.dh_last, p.on, p.i);
-    Vec<float, V> e;
+    link_tiles<V, kBackWarps, true>(g, tile, ex, g.dh_last, p.on, p.i);
+    Row<V> e;
 #pragma unroll
     for (int q = 0; q < V; ++q) {
         e.v[q] = ex.state[lane * V + q];
-        for (uint32_t n = kWarps - 1; n > warp; --n) {
+        for (uint32_t n = kBackWarps - 1; n > warp; --n) {
             const float2 m = ex.map[n][lane * V + q];
             e.v[q] = __fmaf_rn(m.x, e.v[q], m.y);
         }
     }
-    float sum[V];
+    Row<V> sum;
     w.emit(g, p, t0, live, e, sum);
-    if (g.dh0 && p.on && tile.k + 1 == g.tiles && warp == 0) *reinterpret_cast<Vec<float, V> *>(g.dh0 + p.i) = e;
+    if (g.dh0 && p.on && tile.k + 1 == g.tiles && warp == 0) store<float, V>(g.dh0 + p.i, e);
     if (std::is_same<G, Fixed>::value && g.partial) {
         __syncthreads();  // ex.map is read above
 #pragma unroll
-        for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q].x = sum[q];
+        for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q].x = sum.v[q];
         __syncthreads();
         if (warp == 0 && p.on) {
 #pragma unroll
             for (int q = 0; q < V; ++q) {
                 double s = 0.0;
-                for (uint32_t n = 0; n < kWarps; ++n) s += (double)ex.map[n][lane * V + q].x;
-                sum[q] = (float)s;
+                for (uint32_t n = 0; n < kBackWarps; ++n) s += (double)ex.map[n][lane * V + q].x;
+                sum.v[q] = (float)s;
             }
-            put_partial(g, p, w.gates, tile.k, sum);
+            put_partial(g, p, w.in.gates, tile.k, sum);
         }
     }
 }
@@ -531,7 +659,7 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
             if (g.gate) z = *reinterpret_cast<const Vec<G, V> *>((const G *)g.gate + r * g.gs + c);
 #pragma unroll
             for (int q = 0; q < V; ++q) {
-                const Leak l = g.gate ? leak_of(to_float(z.v[q]), g.logit) : Leak{g.decay, __fsub_rn(1.0f, g.decay)};
+                const Leak l = g.gate ? leak_from(z.v[q], g.logit) : Leak{g.decay, __fsub_rn(1.0f, g.decay)};
                 float u = __fmul_rn(g.scale, to_float(x.v[q]));
                 if (g.complement) u = __fmul_rn(u, l.rest);
                 h.v[q] = __fmaf_rn(l.a, h.v[q], u);
@@ -563,26 +691,23 @@ cudaError_t step_narrow(cudaStream_t s, const Form &f, const StepArgs &a, dim3 g
 }
 
 template <typename X, typename G, typename Y, int V>
-void launch_forward(cudaStream_t s, const Form &f, const Args &a) {
-    if (f.split) scan_split_kernel<X, G, Y, V><<<a.tiles * a.columns, kWarps * 32, 0, s>>>(a);
-    else scan_whole_kernel<X, G, Y, V><<<(a.columns + 3) / 4, 128, 0, s>>>(a);
+cudaError_t launch_whole(cudaStream_t s, const Args &a, bool back) {
+    const uint32_t grid = (a.columns + 3) / 4;
+    if (back) back_whole_kernel<X, G, Y, V><<<grid, 128, 0, s>>>(a);
+    else scan_whole_kernel<X, G, Y, V><<<grid, 128, 0, s>>>(a);
+    return cudaGetLastError();
 }
 template <typename X, typename G, typename Y, int V>
-void launch_backward(cudaStream_t s, const Form &f, const Args &a) {
-    if (f.split) back_split_kernel<X, G, Y, V><<<a.tiles * a.columns, kWarps * 32, 0, s>>>(a);
-    else back_whole_kernel<X, G, Y, V><<<(a.columns + 3) / 4, 128, 0, s>>>(a);
+cudaError_t launch_split(cudaStream_t s, const Args &a, bool back) {
+    const uint32_t grid = a.tiles * a.columns;
+    if (back) back_split_kernel<X, G, Y, V><<<grid, kBackWarps * 32, 0, s>>>(a);
+    else scan_split_kernel<X, G, Y, V><<<grid, kScanWarps * 32, 0, s>>>(a);
+    return cudaGetLastError();
 }
-
 template <typename X, typename G, typename Y>
 cudaError_t launch(cudaStream_t s, const Form &f, const Args &a, bool back) {
-    if (back) {
-        if (f.width == 2) launch_backward<X, G, Y, 2>(s, f, a);
-        else launch_backward<X, G, Y, 1>(s, f, a);
-    } else {
-        if (f.width == 2) launch_forward<X, G, Y, 2>(s, f, a);
-        else launch_forward<X, G, Y, 1>(s, f, a);
-    }
-    return cudaGetLastError();
+    if (f.split) return f.width == 2 ? launch_split<X, G, Y, 2>(s, a, back) : launch_split<X, G, Y, 1>(s, a, back);
+    return f.width == 2 ? launch_whole<X, G, Y, 2>(s, a, back) : launch_whole<X, G, Y, 1>(s, a, back);
 }
 
 // The combinations of types for 32-bit and spike inputs, and for 16-bit ones.

@@ -8,8 +8,7 @@ namespace b200 {
 namespace leaky {
 
 constexpr uint32_t kSteps = SNN_B200_LEAKY_BLOCK;  // steps a thread holds in registers
-constexpr uint32_t kWarps = 8;
-constexpr uint32_t kTile = kSteps * kWarps;  // steps of a tile (one CTA)
+constexpr uint32_t kScanWarps = 16, kBackWarps = 8;  // warps of a tile (one CTA), kSteps of the steps each
 constexpr uint32_t kSuper = 16;              // tiles between two published states
 
 struct Args {

@@ -17,7 +17,7 @@ import math
 from . import SNN_ERR_INVALID_ARGUMENT, SnnError, _check, lib
 
 F32, F16, BF16, SPIKES = 0, 1, 2, 3
-LEAKY_BLOCK = 16  # SNN_B200_LEAKY_BLOCK
+LEAKY_BLOCK = 8  # SNN_B200_LEAKY_BLOCK
 
 _DTYPES: dict = {}
 

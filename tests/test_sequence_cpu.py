@@ -26,7 +26,7 @@ def test_sizes():
     L = sb.lib()
     assert L.snn_b200_mx4_sizes(1, 1, None, None) == BAD
     assert L.snn_b200_mx4_linear_workspace(2, 784) == sum(sb.mx4_sizes(2, 784))
-    assert L.snn_b200_leaky_saved_floats(3, 33, 5) == 3 * 3 * 5
+    assert L.snn_b200_leaky_saved_floats(3, 33, 5) == 3 * 5 * 5
     assert L.snn_b200_leaky_workspace(None) == 0
 
 

@@ -8,21 +8,55 @@ namespace b200 {
 namespace leaky {
 namespace {
 
+// ---- states between segments ----
+// states[s] = the state before segment s, folded in order from `first` (or
+// zero) and the maps of the segments before it (backward: behind it). A CTA takes
+// 32 channels; each of its warps composes the maps of one run of segments,
+// folds those of the runs before onto the first state, and walks its run again.
+constexpr uint32_t kCarryWarps = 16;
+__global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *maps, uint32_t segments, uint64_t flat,
+                                                                 const float *first, float *states, bool back) {
+    __shared__ float2 s_run[kCarryWarps][32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    const uint64_t i = (uint64_t)blockIdx.x * 32 + lane;
+    const uint32_t run = (segments + kCarryWarps - 1) / kCarryWarps;
+    const uint32_t from = min(segments, warp * run), to = min(segments, from + run);
+    const auto at = [&](uint32_t n) { return (uint64_t)(back ? segments - 1 - n : n) * flat + i; };
+    float2 m = make_float2(1.0f, 0.0f);
+    if (i < flat)
+#pragma unroll 8
+        for (uint32_t n = from; n < to; ++n) {
+            const float2 v = maps[at(n)];
+            m = make_float2(__fmul_rn(v.x, m.x), __fmaf_rn(v.x, m.y, v.y));
+        }
+    s_run[warp][lane] = m;
+    __syncthreads();
+    if (i >= flat) return;
+    float h = first ? first[i] : 0.0f;
+    for (uint32_t w = 0; w < warp; ++w) h = __fmaf_rn(s_run[w][lane].x, h, s_run[w][lane].y);
+#pragma unroll 8
+    for (uint32_t n = from; n < to; ++n) {
+        const float2 v = maps[at(n)];
+        states[at(n)] = h;
+        h = __fmaf_rn(v.x, h, v.y);
+    }
+}
+
 // ---- a shared gate's gradient ----
-// out[r][c] = the sum of partial[t][b][c] over the tiles and, where the gate
+// out[r][c] = the sum of partial[t][b][c] over the segments and, where the gate
 // is shared over the sequences (rows of out: 1), over b. A CTA takes 32
 // channels of a row; its warps share the terms, in an order that depends on
-// the counts only. Terms are few (a tile each), so they are summed in 64 bits.
+// the counts only. Terms are few (one a segment), so they are summed in 64 bits.
 constexpr uint32_t kSumWarps = 16;
-__global__ void __launch_bounds__(kSumWarps * 32) gate_sum_kernel(const float *partial, uint32_t tiles, uint32_t batch,
+__global__ void __launch_bounds__(kSumWarps * 32) gate_sum_kernel(const float *partial, uint32_t segments, uint32_t batch,
                                                                   uint32_t channels, float *out, int64_t row_stride) {
     __shared__ double s_sum[kSumWarps][32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane;
     const uint64_t flat = (uint64_t)batch * channels;
     for (uint32_t r = blockIdx.y; r < (row_stride ? batch : 1u); r += gridDim.y) {
-        const uint64_t terms = row_stride ? tiles : (uint64_t)tiles * batch;
-        // Term n of row r: tile n, sequence r; or n-th of all [tiles][batch].
+        const uint64_t terms = row_stride ? segments : (uint64_t)segments * batch;
+        // Term n of row r: segment n, sequence r; or n-th of all [segments][batch].
         const float *p = partial + (row_stride ? (uint64_t)r * channels : 0) + c;
         const uint64_t step = row_stride ? flat : channels;
         double sum = 0.0;
@@ -71,62 +105,59 @@ snn_status_t check_common(int device, const snn_b200_leaky_t *q, const void *x, 
     return SNN_OK;
 }
 
-// Where the work lies in the workspace, for the split form.
+// How a call is cut and where its parts lie in the workspace.
 struct Plan {
-    uint64_t flat;
-    uint32_t tiles;
-    uint64_t zeroed;  // bytes of ticket and flags, at the start
-    uint64_t aggregates, states, partial, bytes;
+    uint64_t flat, columns;
+    uint32_t segments, segment_steps;
+    uint64_t maps, states, partial, bytes;
 };
-// `width` channels a thread, `warps` in a tile; the workspace is sized for the largest.
-Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, uint32_t warps) {
-    const uint32_t tile = warps * kSteps;
+// Walks of whole sequences, or segments of them (64 steps at least) where
+// those would be too few to keep the loads of 148 SMs under way.
+constexpr uint64_t kFewWalks = 148 * 12, kManyWalks = 148 * 48;
+constexpr uint32_t kLeastSegment = 64;
+Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     Plan p = {};
     p.flat = q.batch * q.channels;
-    p.tiles = (uint32_t)((q.steps + tile - 1) / tile);
-    const uint64_t supers = p.tiles / kSuper, columns = (p.flat + 32 * width - 1) / (32 * width);
+    p.columns = (p.flat + 32 * width - 1) / (32 * width);
+    p.segments = 1, p.segment_steps = (uint32_t)q.steps;
+    if (p.columns && p.columns < kFewWalks && q.steps >= 2 * kLeastSegment) {
+        const uint64_t want = std::max<uint64_t>(kLeastSegment, q.steps * p.columns / kManyWalks);
+        p.segment_steps = (uint32_t)((want + kSteps - 1) / kSteps * kSteps);
+        p.segments = (uint32_t)((q.steps + p.segment_steps - 1) / p.segment_steps);
+    }
     const auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
-    p.zeroed = round((1 + ((uint64_t)p.tiles + supers) * columns) * 4);
-    p.aggregates = p.zeroed;
-    p.states = p.aggregates + round(p.tiles * columns * 32 * width * 8);
-    p.partial = p.states + round(supers * columns * 32 * width * 4);
-    p.bytes = p.partial + round((p.tiles ? p.tiles : 1) * p.flat * 4);
+    const uint64_t cut = p.segments > 1 ? p.segments * p.flat : 0;
+    p.maps = 0;
+    p.states = p.maps + round(cut * 8);
+    p.partial = p.states + round(cut * 4);
+    p.bytes = p.partial + round(p.segments * p.flat * 4);
     return p;
 }
 
-// Split along the steps when whole walks would leave the SMs short of loads
-// in flight, and when there are steps to split.
-bool wants_split(int device, const Plan &p, uint32_t width, snn_size_t steps) {
-    const uint64_t warps = (p.flat + 32 * width - 1) / (32 * width);
-    if (steps <= 2 * kSteps || warps * p.tiles > kMaxCount) return false;
-    return warps < (uint64_t)sm_count(device) * 16;
-}
-
-void fill(Args &g, const snn_b200_leaky_t &q, const Plan &p, uint32_t width, void *workspace) {
+void fill(Args &g, const snn_b200_leaky_t &q, const Plan &p, void *workspace) {
     g.flat = p.flat;
     g.batch = (uint32_t)q.batch, g.steps = (uint32_t)q.steps, g.channels = (uint32_t)q.channels;
     g.xb = q.x_batch_stride, g.xt = q.x_step_stride, g.gb = q.gate_batch_stride, g.gt = q.gate_step_stride;
     g.yb = q.y_batch_stride, g.yt = q.y_step_stride, g.dyb = q.dy_batch_stride, g.dyt = q.dy_step_stride;
     g.dxb = q.dx_batch_stride, g.dxt = q.dx_step_stride, g.dgb = q.dgate_batch_stride, g.dgt = q.dgate_step_stride;
     g.decay = q.decay, g.scale = q.input_scale, g.logit = q.logit, g.complement = q.complement;
-    g.tiles = p.tiles;
-    g.columns = (uint32_t)((p.flat + 32 * width - 1) / (32 * width));
+    g.columns = (uint32_t)p.columns, g.segments = p.segments, g.segment_steps = p.segment_steps;
     char *w = (char *)workspace;
-    g.ticket = (uint32_t *)w;
-    g.tile_flags = g.ticket + 1;
-    g.state_flags = g.tile_flags + (uint64_t)p.tiles * g.columns;
-    g.aggregates = (float2 *)(w + p.aggregates);
+    g.maps = (float2 *)(w + p.maps);
     g.states = (float *)(w + p.states);
 }
 
-// Two channels a thread where every array can be read in pairs.
-bool pairs(const void *p, uint32_t bytes, int64_t sb, int64_t st) {
-    return !p || (aligned_to(p, 2 * bytes) && sb % 2 == 0 && st % 2 == 0);
+// May a thread hold n channels of an array?
+bool pieces(uint32_t n, const void *p, uint32_t bytes, int64_t sb, int64_t st) {
+    return !p || (aligned_to(p, n * bytes) && sb % n == 0 && st % n == 0);
 }
-bool float_pairs(const float *p) { return aligned_to(p, 8); }
+bool float_pieces(uint32_t n, const float *p) { return aligned_to(p, 4 * n); }
 
-cudaError_t run(cudaStream_t s, int x_dtype, const Form &f, const Args &g, bool back) {
-    switch (x_dtype) {
+cudaError_t run(cudaStream_t s, const snn_b200_leaky_t &q, Args &g, const Plan &p, uint32_t width, bool back,
+                void *workspace) {
+    fill(g, q, p, workspace);
+    const Form f = {q.gate_dtype, q.y_dtype, g.gate && q.gate_step_stride, width};
+    switch (q.x_dtype) {
         case SNN_B200_F32: return back ? backward_f32(s, f, g) : forward_f32(s, f, g);
         case SNN_B200_F16: return back ? backward_f16(s, f, g) : forward_f16(s, f, g);
         case SNN_B200_BF16: return back ? backward_bf16(s, f, g) : forward_bf16(s, f, g);
@@ -135,6 +166,13 @@ cudaError_t run(cudaStream_t s, int x_dtype, const Form &f, const Args &g, bool 
 }
 
 }  // namespace
+
+cudaError_t carry(cudaStream_t s, const Args &a, bool back) {
+    carry_kernel<<<(uint32_t)((a.flat + 31) / 32), kCarryWarps * 32, 0, s>>>(
+        a.maps, a.segments, a.flat, back ? a.dh_last : a.h0, a.states, back);
+    return cudaGetLastError();
+}
+
 }  // namespace leaky
 }  // namespace b200
 
@@ -150,10 +188,7 @@ snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_s
 
 snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *q) {
     if (q == nullptr || q->batch > kMaxCount || q->steps > kMaxCount || q->channels > kMaxCount) return 0;
-    uint64_t most = 0;
-    for (uint32_t width = 1; width <= 2; ++width)
-        for (const uint32_t warps : {kScanWarps, kBackWarps}) most = std::max(most, plan_of(*q, width, warps).bytes);
-    return most;
+    return std::max({plan_of(*q, 1).bytes, plan_of(*q, 2).bytes, plan_of(*q, 4).bytes});
 }
 
 snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,
@@ -177,18 +212,17 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
                                  : cudaMemsetAsync(h_last, 0, q.batch * q.channels * 4, s);
         return op_status(e, __func__);
     }
-    const bool even = q.channels % 2 == 0 && pairs(x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
-                      pairs(gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
-                      pairs(y, dtype_bytes(q.y_dtype), q.y_batch_stride, q.y_step_stride) && float_pairs(h0) &&
-                      float_pairs(h_last) && float_pairs(saved);
-    const uint32_t width = even ? 2 : 1;
-    const Plan p = plan_of(q, width, kScanWarps);
-    const Form f = {q.gate_dtype, q.y_dtype, gate && q.gate_step_stride, wants_split(device, p, width, q.steps), width};
+    // Two channels a thread where every array can be read so; four of a raster.
+    const auto holds = [&](uint32_t n) {
+        return q.channels % n == 0 && pieces(n, x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
+               pieces(n, gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
+               pieces(n, y, dtype_bytes(q.y_dtype), q.y_batch_stride, q.y_step_stride) && float_pieces(n, h0) &&
+               float_pieces(n, h_last) && float_pieces(n, saved);
+    };
+    const uint32_t width = q.x_dtype == SNN_B200_SPIKES && holds(4) ? 4 : holds(2) ? 2 : 1;
     Args g = {};
-    fill(g, q, p, width, workspace);
     g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
-    cudaError_t e = f.split ? cudaMemsetAsync(workspace, 0, p.zeroed, s) : cudaSuccess;
-    if (e == cudaSuccess) e = run(s, q.x_dtype, f, g, false);
+    const cudaError_t e = run(s, q, g, plan_of(q, width), width, false, workspace);
     return op_status(e, __func__);
 }
 
@@ -233,26 +267,23 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
                        : cudaMemset2DAsync(dgate, 4 * std::max<size_t>(q.dgate_batch_stride, q.channels), 0, q.channels * 4, q.batch, s);
         return op_status(e, __func__);
     }
-    const bool even = q.channels % 2 == 0 && pairs(x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
-                      pairs(gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
-                      pairs(dy, dtype_bytes(q.y_dtype), q.dy_batch_stride, q.dy_step_stride) &&
-                      pairs(dx, dtype_bytes(dx_type), q.dx_batch_stride, q.dx_step_stride) &&
-                      (!every || pairs(dgate, dtype_bytes(q.gate_dtype), q.dgate_batch_stride, q.dgate_step_stride)) &&
-                      float_pairs(dh_last) && float_pairs(dh0) && float_pairs(saved);
-    const uint32_t width = even ? 2 : 1;
-    const Plan p = plan_of(q, width, kBackWarps);
-    const Form f = {q.gate_dtype, q.y_dtype, every, wants_split(device, p, width, q.steps), width};
+    const bool even = q.channels % 2 == 0 && pieces(2, x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
+                      pieces(2, gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
+                      pieces(2, dy, dtype_bytes(q.y_dtype), q.dy_batch_stride, q.dy_step_stride) &&
+                      pieces(2, dx, dtype_bytes(dx_type), q.dx_batch_stride, q.dx_step_stride) &&
+                      (!every || pieces(2, dgate, dtype_bytes(q.gate_dtype), q.dgate_batch_stride, q.dgate_step_stride)) &&
+                      float_pieces(2, dh_last) && float_pieces(2, dh0) && float_pieces(2, saved);
     Args g = {};
-    fill(g, q, p, width, workspace);
     g.x = x, g.gate = gate, g.lengths = lengths, g.saved = const_cast<float *>(saved), g.dy = dy;
     g.dh_last = dh_last, g.dx = dx, g.dgate = every ? dgate : nullptr, g.dh0 = dh0;
+    const uint32_t width = even ? 2 : 1;
+    const Plan p = plan_of(q, width);
     g.partial = sums ? (float *)((char *)workspace + p.partial) : nullptr;
-    cudaError_t e = f.split ? cudaMemsetAsync(workspace, 0, p.zeroed, s) : cudaSuccess;
-    if (e == cudaSuccess) e = run(s, q.x_dtype, f, g, true);
+    cudaError_t e = run(s, q, g, p, width, true, workspace);
     if (e == cudaSuccess && sums) {
         const uint32_t rows = shared ? 1u : (uint32_t)(q.batch < 65535 ? q.batch : 65535);
         gate_sum_kernel<<<dim3((uint32_t)((q.channels + 31) / 32), rows), kSumWarps * 32, 0, s>>>(
-            g.partial, f.split ? p.tiles : 1u, (uint32_t)q.batch, (uint32_t)q.channels, (float *)dgate,
+            g.partial, p.segments, (uint32_t)q.batch, (uint32_t)q.channels, (float *)dgate,
             shared ? 0 : q.dgate_batch_stride);
         e = cudaGetLastError();
     }
@@ -291,7 +322,7 @@ snn_status_t snn_b200_leaky_step_async(int device, void *stream, snn_size_t batc
     const bool wide = channels % 4 == 0 && fours(x, dtype_bytes(x_dtype), x_row_stride) &&
                       fours(gate, dtype_bytes(gate_dtype), gate_row_stride) && fours(pool, 4, pool_row_stride) &&
                       fours(y, dtype_bytes(y_dtype), y_row_stride);
-    const Form f = {gate ? gate_dtype : SNN_B200_F32, y_dtype, true, false, wide ? 4u : 1u};
+    const Form f = {gate ? gate_dtype : SNN_B200_F32, y_dtype, true, wide ? 4u : 1u};
     const uint32_t pieces = (uint32_t)((channels + f.width - 1) / f.width);  // thread-sized pieces of a row
     // A warp a row, or the whole CTA where that would leave SMs without work.
     const bool many = batch >= (snn_size_t)sm_count(device) * 4;

@@ -1,19 +1,21 @@
 // Kernels of the leaky recurrence h[t] = a[t] h[t-1] + u[t] and of its
 // gradient, instantiated once for each type of x.
 //
-// Two forms. A thread always holds kSteps consecutive steps of `V`
-// neighbouring channels in registers, and the threads of a warp lie side by
-// side across (batch, channel), so every access is one run of 32 V elements.
+// A warp walks along the steps of 32 V neighbouring (batch, channel) numbers, a
+// thread each V of them, with the state in registers, so every access is one
+// run of 32 V elements. What limits it is how much it keeps under way: the next
+// blocks of kSteps steps are copied to shared memory (cp.async) while one is
+// worked on; a thread reads only what it copied itself, so nothing waits for
+// another warp.
 //
-//  * whole: a warp walks through all steps of its channels, kSteps at a time,
-//    with the state in registers.
-//  * split: a CTA takes one tile of steps (its warps one block of kSteps each). Steps compose as affine maps h -> A h + H, so each tile publishes
-//    its (A, H) at once and then folds the maps of the tiles before it onto
-//    the last published state. States are published every kSuper tiles, so a
-//    tile waits for fewer than kSuper neighbours and one state, always in the
-//    same order: the result does not depend on timing.
-//    Tiles are handed out by a ticket, all channels of a tile before the next
-//    tile, so whatever a tile waits for has started already.
+// Few channels leave most of the GPU idle, so their steps are cut into
+// segments. Steps compose as affine maps h -> A h + H: one kernel walks each
+// segment for its (A, H), one folds them in order into the state before each
+// segment, and the walk itself then starts everywhere at once. The inputs are
+// read twice; the second walk goes through the segments in the opposite order
+// and so finds the last ones in L2. (Measured against one pass whose tiles wait
+// for the maps of the tiles before them: 1 x 65536 x 1024 bf16 took 0.37 to 0.45 ms
+// that way, as the tiles under way are too few to cover the waits.)
 #pragma once
 
 #include "b200_leaky.h"
@@ -23,9 +25,6 @@
 namespace b200 {
 namespace leaky {
 namespace {
-
-constexpr unsigned kAll = 0xffffffffu;
-constexpr uint32_t kPollLimit = 1u << 22;  // polls of 32+ ns each before a wait gives up
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
@@ -141,42 +140,41 @@ struct Leak {
 // difference of nearly equal values. A 16-bit logit has a rounding of 2^-9 of
 // itself, so for it the product with log2(e) is rounded once to 32 bits (2^-20
 // of the exponential up to logits of 22).
-template <bool Narrow>
-__device__ __forceinline__ Leak leak_of(float z, int logit) {
-    if (!logit) return {z, __fsub_rn(1.0f, z)};
-    float t;
-    if (Narrow) {
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmul_rn(-fabsf(z), 1.44269504f)));
+template <typename G, bool Logit>
+__device__ __forceinline__ Leak leak_of(G gate) {
+    const float z = to_float(gate);
+    if (!Logit) return {z, __fsub_rn(1.0f, z)};
+    float t, r;
+    if (sizeof(G) == 2) {
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmul_rn(fabsf(z), -1.44269504f)));
     } else {
         t = expf(-fabsf(z));
     }
-    const float r = __fdividef(1.0f, __fadd_rn(1.0f, t)), q = __fmul_rn(t, r);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, t)));
+    const float q = __fmul_rn(t, r);
     return z >= 0.0f ? Leak{r, q} : Leak{q, r};
 }
 template <typename G>
 __device__ __forceinline__ Leak leak_from(G z, int logit) {
-    return leak_of<sizeof(G) == 2>(to_float(z), logit);
+    return logit ? leak_of<G, true>(z) : leak_of<G, false>(z);
 }
 
-__device__ __forceinline__ uint32_t load_acquire(const uint32_t *p) {
-    uint32_t v;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void store_release(uint32_t *p, uint32_t v) {
-    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-// Waits until a flag is set; false when it gave up.
-__device__ __forceinline__ bool wait_flag(const uint32_t *p) {
-    for (uint32_t i = 0; i < kPollLimit; ++i) {
-        if (load_acquire(p)) return true;
-        __nanosleep(32);
+// f(logit, complement) with the call's flags as constants: a test for every
+// step would cost more than the step.
+template <bool B>
+using Flag = std::integral_constant<bool, B>;
+template <typename F>
+__device__ __forceinline__ void with_flags(const Args &g, F f) {
+    if (g.logit) {
+        if (g.complement) f(Flag<true>(), Flag<true>());
+        else f(Flag<true>(), Flag<false>());
+    } else {
+        if (g.complement) f(Flag<false>(), Flag<true>());
+        else f(Flag<false>(), Flag<false>());
     }
-    return false;
 }
 
-// A thread's place: V channels of one sequence. Lanes behind the last
-// channel take part in the shuffles and waits with a length of zero.
+// A thread's place: V channels of one sequence.
 struct Place {
     uint64_t i;  // first of its (batch, channel) numbers
     int64_t b, c;
@@ -193,19 +191,96 @@ __device__ __forceinline__ Place place_of(const Args &g, uint64_t column) {
     p.len = !p.on ? 0u : g.lengths ? min(g.lengths[p.b], g.steps) : g.steps;
     return p;
 }
+// The warp's segment and column; the second walk takes the segments from the other end.
+struct Part {
+    uint64_t column;
+    uint32_t segment, t0, t1;  // steps t0 .. t1-1
+    bool on;
+};
+__device__ __forceinline__ Part part_of(const Args &g, bool ascending) {
+    const uint64_t n = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+    Part w;
+    w.segment = (uint32_t)(n / g.columns);
+    w.column = n - (uint64_t)w.segment * g.columns;
+    w.on = w.segment < g.segments;
+    if (!ascending) w.segment = g.segments - 1 - w.segment;
+    w.t0 = w.segment * g.segment_steps;
+    w.t1 = min(g.steps, w.t0 + g.segment_steps);
+    return w;
+}
+// How many of the steps from t0 on lie within the sequence.
 __device__ __forceinline__ int live_steps(uint32_t len, uint32_t t0) {
     return len <= t0 ? 0 : (int)min(len - t0, kSteps);
 }
 
-// kSteps rows, all of them wanted by most threads.
+// A block's rows of an array: copied ahead to shared memory where a thread's
+// piece of a row has the size of a copy (4 bytes or more), else loaded when the
+// block is worked on.
 template <typename T, int V>
-__device__ __forceinline__ void load_steps(Vec<T, V> (&r)[kSteps], const T *p, int64_t stride, int live) {
-    if (live == (int)kSteps) {
+struct Feed {
+    static constexpr bool kShared = sizeof(T) * V >= 4;
+    static constexpr uint32_t kBytes = kShared ? (uint32_t)sizeof(T) * 32 * V * kSteps : 0;  // a block, a warp
+    const T *p;
+    int64_t stride;
+
+    __device__ __forceinline__ void init(const void *base, const Place &at, int64_t sb, int64_t st) {
+        p = (const T *)base + at.b * sb + at.c;
+        stride = st;
+    }
+    // slot: the warp's memory for the block.
+    __device__ __forceinline__ void fetch(uint8_t *slot, uint32_t t0, int live) const {
+        if constexpr (kShared) {
+            const T *row = p + (int64_t)t0 * stride;
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + (threadIdx.x & 31) * (uint32_t)sizeof(T) * V;
 #pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j) r[j] = load<T, V>(p + j * stride);
-    } else {
+            for (int j = 0; j < (int)kSteps; ++j)
+                if (j < live)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to + j * (uint32_t)sizeof(T) * 32 * V),
+                                 "l"(row + j * stride), "n"(sizeof(T) * V)
+                                 : "memory");
+        }
+    }
+    // The block's rows; those behind the live ones are anything.
+    __device__ __forceinline__ void take(const uint8_t *slot, uint32_t t0, int live, Vec<T, V> (&r)[kSteps]) const {
+        const T *row = p + (int64_t)t0 * stride;
 #pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j) r[j] = j < live ? load<T, V>(p + j * stride) : Vec<T, V>{};
+        for (int j = 0; j < (int)kSteps; ++j)
+            if constexpr (kShared) r[j] = reinterpret_cast<const Vec<T, V> *>(slot)[j * 32 + (threadIdx.x & 31)];
+            else r[j] = j < live ? load<T, V>(row + j * stride) : Vec<T, V>{};
+    }
+};
+template <int V>
+struct Feed<Fixed, V> {
+    static constexpr bool kShared = true;
+    static constexpr uint32_t kBytes = 0;
+    __device__ __forceinline__ void init(const void *, const Place &, int64_t, int64_t) {}
+    __device__ __forceinline__ void fetch(uint8_t *, uint32_t, int) const {}
+};
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void await() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Walks the blocks of [t0, t1) in either direction: fetch(t0, slot) starts a
+// block's copies, work(t0, slot) uses them. Those of kDepth - 1 blocks are under way.
+template <bool Reverse, typename Fetch, typename Work>
+__device__ __forceinline__ void walk_blocks(uint32_t t0, uint32_t t1, Fetch fetch, Work work) {
+    const uint32_t blocks = (t1 - t0 + kSteps - 1) / kSteps;
+    const auto at = [&](uint32_t n) { return t0 + (Reverse ? blocks - 1 - n : n) * kSteps; };
+#pragma unroll
+    for (uint32_t n = 0; n < kDepth - 1; ++n) {
+        if (n < blocks) fetch(at(n), n);
+        fetched();
+    }
+    uint32_t slot = 0;
+    for (uint32_t n = 0; n < blocks; ++n) {
+        const uint32_t to = slot ? slot - 1 : kDepth - 1;
+        if (n + kDepth - 1 < blocks) fetch(at(n + kDepth - 1), to);
+        fetched();
+        await<kDepth - 1>();
+        work(at(n), slot);
+        slot = slot + 1 == kDepth ? 0 : slot + 1;
     }
 }
 
@@ -214,13 +289,14 @@ template <typename G, int V>
 struct Gates {
     Vec<G, V> raw[kSteps];
     __device__ __forceinline__ void init(const Args &, const Place &) {}
-    __device__ __forceinline__ void load(const Args &g, const Place &p, uint32_t t0, int live) {
-        load_steps<G, V>(raw, (const G *)g.gate + p.b * g.gb + (int64_t)t0 * g.gt + p.c, g.gt, live);
+    __device__ __forceinline__ void take(const Feed<G, V> &feed, const uint8_t *slot, uint32_t t0, int live) {
+        feed.take(slot, t0, live, raw);
     }
-    __device__ __forceinline__ void at(const Args &g, int j, Row<V> &a, Row<V> &rest) const {
+    template <bool Logit>
+    __device__ __forceinline__ void at(int j, Row<V> &a, Row<V> &rest) const {
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-            const Leak l = leak_from(raw[j].v[q], g.logit);
+            const Leak l = leak_of<G, Logit>(raw[j].v[q]);
             a.v[q] = l.a, rest.v[q] = l.rest;
         }
     }
@@ -232,210 +308,114 @@ struct Gates<Fixed, V> {
 #pragma unroll
         for (int q = 0; q < V; ++q) {
             const Leak l = !g.gate ? Leak{g.decay, __fsub_rn(1.0f, g.decay)}
-                           : p.on  ? leak_from(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit)
-                                   : Leak{1.0f, 0.0f};
+                                   : leak_from(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit);
             a_.v[q] = l.a, rest_.v[q] = l.rest;
         }
     }
-    __device__ __forceinline__ void load(const Args &, const Place &, uint32_t, int) {}
-    __device__ __forceinline__ void at(const Args &, int, Row<V> &a, Row<V> &rest) const { a = a_, rest = rest_; }
+    __device__ __forceinline__ void take(const Feed<Fixed, V> &, const uint8_t *, uint32_t, int) {}
+    template <bool Logit>
+    __device__ __forceinline__ void at(int, Row<V> &a, Row<V> &rest) const {
+        a = a_, rest = rest_;
+    }
 };
 
 template <int V>
-__device__ __forceinline__ Row<V> load_state(const float *p, uint64_t i, bool on) {
-    return on && p ? load<float, V>(p + i) : Row<V>{};
+__device__ __forceinline__ Row<V> load_state(const float *p, uint64_t i) {
+    return p ? load<float, V>(p + i) : all<V>(0.0f);
+}
+template <int V>
+__device__ __forceinline__ void store_map(float2 *p, const Row<V> &A, const Row<V> &H) {
+#pragma unroll
+    for (int q = 0; q < V; q += 2) {
+        if constexpr (V == 1) *p = make_float2(A.v[0], H.v[0]);
+        else *reinterpret_cast<float4 *>(p + q) = make_float4(A.v[q], H.v[q], A.v[q + 1], H.v[q + 1]);
+    }
 }
 
-// The state before a block of steps, kept for the backward pass.
+// The state before a block of kSteps steps, kept for the backward pass.
 __device__ __forceinline__ float *saved_at(const Args &g, const Place &p, uint32_t t0) {
     const uint32_t blocks = (g.steps + kSteps - 1) / kSteps;
     return g.saved + ((uint64_t)p.b * blocks + t0 / kSteps) * g.channels + p.c;
 }
 
-// Walks a thread's steps from state h on, writing y.
-template <typename Y, int V>
-__device__ __forceinline__ void emit(const Args &g, const Place &p, uint32_t t0, int live, const Row<V> (&a)[kSteps],
-                                     const Row<V> (&u)[kSteps], Row<V> &h) {
-    if (!p.on) return;
-    if (g.saved) store<float, V>(saved_at(g, p, t0), h);
-    Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
-    if (live == (int)kSteps) {
+// A block's steps from its gates and inputs: step(j, a, u) for each of the
+// `live` ones, with the call's flags as constants.
+template <typename X, typename G, int V, typename Step>
+__device__ __forceinline__ void each_step(const Args &g, const Gates<G, V> &gates, const Vec<X, V> (&x)[kSteps], int live,
+                                          Step step) {
+    with_flags(g, [&](auto logit, auto complement) {
+        const auto one = [&](int j) {
+            Row<V> a, rest;
+            gates.template at<logit.value>(j, a, rest);
+            Row<V> u = mul(all<V>(g.scale), widen(x[j]));
+            if (complement.value) u = mul(u, rest);
+            step(j, a, u);
+        };
+        if (live == (int)kSteps) {
 #pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j) {
-            h = fma(a[j], h, u[j]);
-            store<Y, V>(y + j * g.yt, narrow<Y, V>(h));
-        }
-    } else {
-        const int rows = (int)min(g.steps - t0, kSteps);
-#pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j) {
-            h = fma(a[j], h, u[j]);
-            if (j < rows) store<Y, V>(y + j * g.yt, j < live ? narrow<Y, V>(h) : Vec<Y, V>{});
-        }
-    }
-}
-
-// What a block reads, before it is worked on.
-template <typename X, typename G, int V>
-struct Inputs {
-    Gates<G, V> gates;
-    Vec<X, V> x[kSteps];
-    __device__ __forceinline__ void load(const Args &g, const Place &p, uint32_t t0, int live) {
-        gates.load(g, p, t0, live);
-        load_steps<X, V>(x, (const X *)g.x + p.b * g.xb + (int64_t)t0 * g.xt + p.c, g.xt, live);
-    }
-    // Gates and inputs of the steps; rows behind the sequence keep the state (a = 1, u = 0).
-    __device__ __forceinline__ void maps(const Args &g, int live, Row<V> (&a)[kSteps], Row<V> (&u)[kSteps]) const {
-        const Row<V> scale = all<V>(g.scale);
-#pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j) {
-            Row<V> rest;
-            gates.at(g, j, a[j], rest);
-            u[j] = mul(scale, widen(x[j]));
-            if (g.complement) u[j] = mul(u[j], rest);
-        }
-        if (live < (int)kSteps) {
+            for (int j = 0; j < (int)kSteps; ++j) one(j);
+        } else {
 #pragma unroll
             for (int j = 0; j < (int)kSteps; ++j)
-                if (j >= live) a[j] = all<V>(1.0f), u[j] = all<V>(0.0f);
+                if (j < live) one(j);
         }
-    }
-};
+    });
+}
 
-template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(128) scan_whole_kernel(Args g) {
-    const Place p = place_of<V>(g, (uint64_t)blockIdx.x * 4 + threadIdx.x / 32);
+// Maps: only each segment's map is wanted; else y, from h0 or the segments' states.
+template <typename X, typename G, typename Y, int V, bool Maps>
+__global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_constant__ Args g) {
+    extern __shared__ __align__(16) uint8_t s_feed[];
+    const Part w = part_of(g, Maps);
+    if (!w.on) return;
+    const Place p = place_of<V>(g, w.column);
     if (!p.on) return;
-    Inputs<X, G, V> in;
-    in.gates.init(g, p);
-    Row<V> h = load_state<V>(g.h0, p.i, true);
-    in.load(g, p, 0, live_steps(p.len, 0));
-    for (uint32_t t0 = 0; t0 < g.steps; t0 += kSteps) {
-        Row<V> a[kSteps], u[kSteps];
-        const int live = live_steps(p.len, t0);
-        in.maps(g, live, a, u);
-        if (t0 + kSteps < g.steps) in.load(g, p, t0 + kSteps, live_steps(p.len, t0 + kSteps));  // on the way while this block is written
-        emit<Y, V>(g, p, t0, live, a, u, h);
-    }
-    if (g.h_last) store<float, V>(g.h_last + p.i, h);
-}
-
-// ---- split form ----
-struct Tile {
-    uint32_t k;       // along the steps (in the direction of the walk)
-    uint64_t column;  // across the channels
-};
-__device__ __forceinline__ Tile take_tile(const Args &g) {
-    __shared__ uint32_t s_ticket;
-    if (threadIdx.x == 0) s_ticket = atomicAdd(g.ticket, 1u);
-    __syncthreads();
-    return {s_ticket / g.columns, s_ticket % g.columns};
-}
-
-template <int V, uint32_t W>
-struct Exchange {
-    float2 map[W][32 * V];  // each warp's (A, H)
-    float state[32 * V];         // the state that enters the tile
-};
-
-// Publishes the tile's map and finds the state that enters it; `first` is
-// the state that enters tile 0. Warp w's own map is in ex.map[w]; `order`
-// gives the warps in the direction of the walk. On return (after a barrier)
-// ex.state is set.
-template <int V, uint32_t W, bool Reverse>
-__device__ __forceinline__ void link_tiles(const Args &g, const Tile &tile, Exchange<V, W> &ex, const float *first,
-                                           bool on, uint64_t i) {
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const uint64_t width = (uint64_t)g.columns * 32 * V, at = tile.column * 32 * V + lane * V;
-    const bool last = tile.k + 1 == g.tiles;
-    const bool keeps = !last && (tile.k + 1) % kSuper == 0;  // publishes a state
-    if (warp < 2 && (warp == 1 || !last)) {
-        // Both warps need the tile's map (warp 1 only to publish a state).
-        float2 m[V];
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            m[q] = make_float2(1.0f, 0.0f);
-#pragma unroll
-            for (uint32_t w = 0; w < W; ++w) {
-                const float2 n = ex.map[Reverse ? W - 1 - w : w][lane * V + q];
-                m[q] = make_float2(__fmul_rn(n.x, m[q].x), __fmaf_rn(n.x, m[q].y, n.y));
+    constexpr uint32_t kX = Feed<X, V>::kBytes, kSlot = kX + Feed<G, V>::kBytes;
+    uint8_t *mine = s_feed + threadIdx.x / 32 * (kDepth * kSlot);
+    Feed<X, V> fx;
+    Feed<G, V> fz;
+    Gates<G, V> gates;
+    gates.init(g, p);
+    fx.init(g.x, p, g.xb, g.xt);
+    fz.init(g.gate, p, g.gb, g.gt);
+    Row<V> h = Maps ? all<V>(0.0f) : g.segments > 1 ? load<float, V>(g.states + w.segment * g.flat + p.i)
+                                                    : load_state<V>(g.h0, p.i);
+    Row<V> A = all<V>(1.0f);
+    // Behind the sequence nothing happens to the map.
+    const uint32_t end = Maps ? max(w.t0, min(w.t1, p.len)) : w.t1;
+    walk_blocks<false>(
+        w.t0, end,
+        [&](uint32_t t0, uint32_t slot) {
+            const int live = live_steps(p.len, t0);
+            fz.fetch(mine + slot * kSlot + kX, t0, live);
+            fx.fetch(mine + slot * kSlot, t0, live);
+        },
+        [&](uint32_t t0, uint32_t slot) {
+            const int live = live_steps(p.len, t0);
+            Vec<X, V> x[kSteps];
+            gates.take(fz, mine + slot * kSlot + kX, t0, live);
+            fx.take(mine + slot * kSlot, t0, live, x);
+            if constexpr (Maps) {
+                each_step<X, G, V>(g, gates, x, live, [&](int, const Row<V> &a, const Row<V> &u) {
+                    A = mul(a, A);
+                    h = fma(a, h, u);
+                });
+            } else {
+                if (g.saved) store<float, V>(saved_at(g, p, t0), h);
+                Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
+                each_step<X, G, V>(g, gates, x, live, [&](int j, const Row<V> &a, const Row<V> &u) {
+                    h = fma(a, h, u);
+                    store<Y, V>(y + j * g.yt, narrow<Y, V>(h));
+                });
+                if (live < (int)kSteps)
+                    for (int j = live; j < (int)min(w.t1 - t0, kSteps); ++j) store<Y, V>(y + j * g.yt, Vec<Y, V>{});
             }
-        }
-        if (warp == 0) {
-#pragma unroll
-            for (int q = 0; q < V; ++q) g.aggregates[tile.k * width + at + q] = m[q];
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) store_release(g.tile_flags + (uint64_t)tile.k * g.columns + tile.column, 1u);
-        } else {
-            const uint32_t super = tile.k / kSuper, before = tile.k % kSuper;
-            bool ok = true;
-            if (lane < before)
-                ok = wait_flag(g.tile_flags + (uint64_t)(super * kSuper + lane) * g.columns + tile.column);
-            else if (lane == 31 && super)
-                ok = wait_flag(g.state_flags + (uint64_t)(super - 1) * g.columns + tile.column);
-            ok = __all_sync(kAll, ok);
-            float h[V];
-#pragma unroll
-            for (int q = 0; q < V; ++q)
-                h[q] = super ? __ldcg(g.states + (super - 1) * width + at + q) : on && first ? first[i + q] : 0.0f;
-            const float2 *maps = g.aggregates + (uint64_t)super * kSuper * width + at;
-#pragma unroll 4
-            for (uint32_t k = 0; k < before; ++k)
-#pragma unroll
-                for (int q = 0; q < V; ++q) {
-                    const float2 n = __ldcg(maps + k * width + q);
-                    h[q] = __fmaf_rn(n.x, h[q], n.y);
-                }
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                if (!ok) h[q] = __uint_as_float(0x7fffffffu);  // a wait gave up: let the result say so
-                ex.state[lane * V + q] = h[q];
-                if (keeps) g.states[super * width + at + q] = __fmaf_rn(m[q].x, h[q], m[q].y);
-            }
-            if (keeps) {
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) store_release(g.state_flags + (uint64_t)super * g.columns + tile.column, 1u);
-            }
-        }
+        });
+    if constexpr (Maps) {
+        store_map<V>(g.maps + w.segment * g.flat + p.i, A, h);
+    } else {
+        if (g.h_last && w.segment + 1 == g.segments) store<float, V>(g.h_last + p.i, h);
     }
-    __syncthreads();
-}
-
-template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_split_kernel(Args g) {
-    __shared__ Exchange<V, kScanWarps> ex;
-    const Tile tile = take_tile(g);
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const Place p = place_of<V>(g, tile.column);
-    const uint32_t t0 = (tile.k * kScanWarps + warp) * kSteps;
-    Row<V> a[kSteps], u[kSteps];
-    const int live = live_steps(p.len, t0);
-    {
-        Inputs<X, G, V> in;
-        in.gates.init(g, p);
-        in.load(g, p, t0, live);
-        in.maps(g, live, a, u);
-    }
-    Row<V> A = all<V>(1.0f), H = all<V>(0.0f);
-#pragma unroll
-    for (int j = 0; j < (int)kSteps; ++j) A = mul(a[j], A), H = fma(a[j], H, u[j]);
-#pragma unroll
-    for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q] = make_float2(A.v[q], H.v[q]);
-    __syncthreads();
-    link_tiles<V, kScanWarps, false>(g, tile, ex, g.h0, p.on, p.i);
-    Row<V> h;
-#pragma unroll
-    for (int q = 0; q < V; ++q) {
-        h.v[q] = ex.state[lane * V + q];
-        for (uint32_t w = 0; w < warp; ++w) {
-            const float2 n = ex.map[w][lane * V + q];
-            h.v[q] = __fmaf_rn(n.x, h.v[q], n.y);
-        }
-    }
-    if (t0 < g.steps) emit<Y, V>(g, p, t0, live, a, u, h);
-    if (g.h_last && p.on && tile.k + 1 == g.tiles && warp + 1 == kScanWarps) store<float, V>(g.h_last + p.i, h);
 }
 
 // ---- gradient ----
@@ -454,157 +434,145 @@ struct GradientOf<Spike> {
 
 template <typename X, typename G, typename Y, int V>
 struct Back {
-    Inputs<X, G, V> in;
+    static constexpr bool kEvery = !std::is_same<G, Fixed>::value;
+    Gates<G, V> gates;
     Vec<Y, V> dy[kSteps];
-    Row<V> h;
-    Row<V> a[kSteps], rest[kSteps], k[kSteps];  // k: what d is multiplied with
+    // Of each step: the gate, and what d is multiplied with for dx and for
+    // the gate's gradient (where it is shared, without its common factor).
+    Row<V> a[kSteps], fx[kSteps], fz[kSteps];
 
-    __device__ __forceinline__ void load(const Args &g, const Place &p, uint32_t t0, int live) {
-        in.load(g, p, t0, live);
-        load_steps<Y, V>(dy, (const Y *)g.dy + p.b * g.dyb + (int64_t)t0 * g.dyt + p.c, g.dyt, live);
-        h = live ? leaky::load<float, V>(saved_at(g, p, t0)) : Row<V>{};
-    }
-    __device__ __forceinline__ void maps(const Args &g, int live) {
-        const Row<V> scale = all<V>(g.scale);
+    __device__ __forceinline__ void maps(const Args &g, const Vec<X, V> (&x)[kSteps], Row<V> h, int live) {
+        with_flags(g, [&](auto logit, auto complement) {
+            const Row<V> scale = all<V>(g.scale);
 #pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j) {
-            in.gates.at(g, j, a[j], rest[j]);
-            const Row<V> v = mul(scale, widen(in.x[j]));
-            if (g.complement) {
-                k[j] = add(h, mul(all<V>(-1.0f), v));
-                h = fma(a[j], h, mul(v, rest[j]));
-            } else {
-                k[j] = h;
+            for (int j = 0; j < (int)kSteps; ++j) {
+                Row<V> rest, v = mul(scale, widen(x[j]));
+                gates.template at<logit.value>(j, a[j], rest);
+                if (complement.value) {
+                    fz[j] = fma(all<V>(-1.0f), v, h);
+                    fx[j] = mul(scale, rest);
+                    v = mul(v, rest);
+                } else {
+                    fz[j] = h;
+                    fx[j] = scale;
+                }
                 h = fma(a[j], h, v);
+                if (kEvery && logit.value) fz[j] = mul(fz[j], mul(a[j], rest));
             }
-        }
+        });
         if (live < (int)kSteps) {
 #pragma unroll
             for (int j = 0; j < (int)kSteps; ++j)
                 if (j >= live) a[j] = all<V>(1.0f);
         }
     }
-    // One step back: d and e before it.
+    // One step back: d, and e before it.
     __device__ __forceinline__ Row<V> step(int j, int live, Row<V> &e) const {
         const Row<V> d = add(widen(dy[j]), e);
         if (j < live) e = mul(a[j], d);
         return d;
     }
     // Walks back from e, writes dx and the gradient of a gate with a value
-    // for every step, and returns the block's sum of da in sum.
-    __device__ __forceinline__ void emit(const Args &g, const Place &p, uint32_t t0, int live, Row<V> &e,
-                                         Row<V> &sum) {
+    // for every step, and returns the block's sum for a shared one.
+    template <bool Whole>
+    __device__ __forceinline__ Row<V> walk(const Args &g, const Place &p, uint32_t t0, int live, Row<V> &e) {
         using D = typename GradientOf<X>::type;
-        constexpr bool every = !std::is_same<G, Fixed>::value;
         D *dx = (D *)g.dx + p.b * g.dxb + (int64_t)t0 * g.dxt + p.c;
-        const int rows = !p.on || t0 >= g.steps ? 0 : (int)min(g.steps - t0, kSteps);
-        const Row<V> scale = all<V>(g.scale);
-        sum = all<V>(0.0f);
+        G *dz = (G *)g.dgate + p.b * g.dgb + (int64_t)t0 * g.dgt + p.c;
+        const int rows = t0 >= g.steps ? 0 : (int)min(g.steps - t0, kSteps);
+        Row<V> sum = all<V>(0.0f);
 #pragma unroll
         for (int j = (int)kSteps - 1; j >= 0; --j) {
-            const bool on = j < live;
-            const Row<V> d = step(j, live, e);
-            Row<V> z = mul(d, k[j]);
-            if (!every && on) sum = add(sum, z);
-            if (j >= rows) continue;
-            if (g.dx) {
-                Row<V> f = mul(scale, d);
-                if (g.complement) f = mul(f, rest[j]);
-                store<D, V>(dx + j * g.dxt, on ? narrow<D, V>(f) : Vec<D, V>{});
-            }
-            if constexpr (every) {
-                if (g.dgate) {
-                    if (g.logit) z = mul(z, mul(a[j], rest[j]));
-                    store<G, V>((G *)g.dgate + p.b * g.dgb + (int64_t)(t0 + j) * g.dgt + p.c,
-                                on ? narrow<G, V>(z) : Vec<G, V>{});
-                }
-            }
+            const bool on = Whole || j < live;
+            const Row<V> d = step(j, Whole ? (int)kSteps : live, e);
+            if (!kEvery && on) sum = fma(d, fz[j], sum);
+            if (!Whole && j >= rows) continue;
+            if (g.dx) store<D, V>(dx + j * g.dxt, on ? narrow<D, V>(mul(fx[j], d)) : Vec<D, V>{});
+            if constexpr (kEvery)
+                if (g.dgate) store<G, V>(dz + j * g.dgt, on ? narrow<G, V>(mul(d, fz[j])) : Vec<G, V>{});
         }
+        return sum;
+    }
+    __device__ __forceinline__ Row<V> emit(const Args &g, const Place &p, uint32_t t0, int live, Row<V> &e) {
+        if (!p.on) return all<V>(0.0f);
+        return live == (int)kSteps ? walk<true>(g, p, t0, live, e) : walk<false>(g, p, t0, live, e);
     }
 };
-
 // A shared gate's sum for one thread: of logits, the gate's own slope is a common factor.
 template <int V>
-__device__ __forceinline__ void put_partial(const Args &g, const Place &p, const Gates<Fixed, V> &gates, uint32_t tile,
+__device__ __forceinline__ void put_partial(const Args &g, const Place &p, const Gates<Fixed, V> &gates, uint32_t segment,
                                             const Row<V> &sum) {
-    store<float, V>(g.partial + tile * g.flat + p.i, g.logit ? mul(sum, mul(gates.a_, gates.rest_)) : sum);
+    store<float, V>(g.partial + segment * g.flat + p.i, g.logit ? mul(sum, mul(gates.a_, gates.rest_)) : sum);
 }
 template <typename G, int V>
 __device__ __forceinline__ void put_partial(const Args &, const Place &, const Gates<G, V> &, uint32_t,
                                             const Row<V> &) {}
 
-template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(128) back_whole_kernel(Args g) {
-    const Place p = place_of<V>(g, (uint64_t)blockIdx.x * 4 + threadIdx.x / 32);
+// Maps: only each segment's map of e is wanted, for which x does not count.
+template <typename X, typename G, typename Y, int V, bool Maps>
+__global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const __grid_constant__ Args g) {
+    extern __shared__ __align__(16) uint8_t s_feed[];
+    const Part w = part_of(g, Maps);
+    if (!w.on) return;
+    const Place p = place_of<V>(g, w.column);
     if (!p.on) return;
-    Back<X, G, Y, V> w;
-    w.in.gates.init(g, p);
-    Row<V> e = load_state<V>(g.dh_last, p.i, true);
+    constexpr uint32_t kY = Feed<Y, V>::kBytes, kZ = kY + Feed<G, V>::kBytes, kSlot = kZ + (Maps ? 0 : Feed<X, V>::kBytes);
+    uint8_t *mine = s_feed + threadIdx.x / 32 * (kDepth * kSlot);
+    Feed<X, V> fx;
+    Feed<G, V> fz;
+    Feed<Y, V> fy;
+    fx.init(g.x, p, g.xb, g.xt);
+    fz.init(g.gate, p, g.gb, g.gt);
+    fy.init(g.dy, p, g.dyb, g.dyt);
+    Back<X, G, Y, V> b;
+    b.gates.init(g, p);
+    Row<V> e = Maps ? all<V>(0.0f) : g.segments > 1 ? load<float, V>(g.states + w.segment * g.flat + p.i)
+                                                    : load_state<V>(g.dh_last, p.i);
+    Row<V> A = all<V>(1.0f);
     double total[V] = {};
-    for (uint32_t n = (g.steps + kSteps - 1) / kSteps; n-- > 0;) {
-        const uint32_t t0 = n * kSteps;
-        const int live = live_steps(p.len, t0);
-        Row<V> sum;
-        w.load(g, p, t0, live);
-        w.maps(g, live);
-        w.emit(g, p, t0, live, e, sum);
-        if (std::is_same<G, Fixed>::value)
+    walk_blocks<true>(
+        w.t0, Maps ? max(w.t0, min(w.t1, p.len)) : w.t1,
+        [&](uint32_t t0, uint32_t slot) {
+            const int live = live_steps(p.len, t0);
+            fy.fetch(mine + slot * kSlot, t0, live);
+            fz.fetch(mine + slot * kSlot + kY, t0, live);
+            if (!Maps) fx.fetch(mine + slot * kSlot + kZ, t0, live);
+        },
+        [&](uint32_t t0, uint32_t slot) {
+            const int live = live_steps(p.len, t0);
+            b.gates.take(fz, mine + slot * kSlot + kY, t0, live);
+            fy.take(mine + slot * kSlot, t0, live, b.dy);
+            if constexpr (Maps) {
+                with_flags(g, [&](auto logit, auto) {
 #pragma unroll
-            for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
-    }
-    if (g.dh0) store<float, V>(g.dh0 + p.i, e);
-    if (g.partial) {
-        Row<V> sum;
+                    for (int j = (int)kSteps - 1; j >= 0; --j)
+                        if (j < live) {
+                            Row<V> a, rest;
+                            b.gates.template at<logit.value>(j, a, rest);
+                            A = mul(a, A);
+                            e = mul(a, add(widen(b.dy[j]), e));
+                        }
+                });
+            } else {
+                const Row<V> h = live ? load<float, V>(saved_at(g, p, t0)) : all<V>(0.0f);
+                Vec<X, V> x[kSteps];
+                fx.take(mine + slot * kSlot + kZ, t0, live, x);
+                b.maps(g, x, h, live);
+                const Row<V> sum = b.emit(g, p, t0, live, e);
+                if (!b.kEvery)
 #pragma unroll
-        for (int q = 0; q < V; ++q) sum.v[q] = (float)total[q];
-        put_partial(g, p, w.in.gates, 0, sum);
-    }
-}
-
-template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(kBackWarps * 32) back_split_kernel(Args g) {
-    __shared__ Exchange<V, kBackWarps> ex;
-    const Tile tile = take_tile(g);
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const Place p = place_of<V>(g, tile.column);
-    const uint32_t t0 = ((g.tiles - 1 - tile.k) * kBackWarps + warp) * kSteps;
-    Back<X, G, Y, V> w;
-    w.in.gates.init(g, p);
-    const int live = live_steps(p.len, t0);
-    w.load(g, p, t0, live);
-    w.maps(g, live);
-    Row<V> A = all<V>(1.0f), E = all<V>(0.0f);
-#pragma unroll
-    for (int j = (int)kSteps - 1; j >= 0; --j) A = mul(w.a[j], A), w.step(j, live, E);
-#pragma unroll
-    for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q] = make_float2(A.v[q], E.v[q]);
-    __syncthreads();
-    link_tiles<V, kBackWarps, true>(g, tile, ex, g.dh_last, p.on, p.i);
-    Row<V> e;
-#pragma unroll
-    for (int q = 0; q < V; ++q) {
-        e.v[q] = ex.state[lane * V + q];
-        for (uint32_t n = kBackWarps - 1; n > warp; --n) {
-            const float2 m = ex.map[n][lane * V + q];
-            e.v[q] = __fmaf_rn(m.x, e.v[q], m.y);
-        }
-    }
-    Row<V> sum;
-    w.emit(g, p, t0, live, e, sum);
-    if (g.dh0 && p.on && tile.k + 1 == g.tiles && warp == 0) store<float, V>(g.dh0 + p.i, e);
-    if (std::is_same<G, Fixed>::value && g.partial) {
-        __syncthreads();  // ex.map is read above
-#pragma unroll
-        for (int q = 0; q < V; ++q) ex.map[warp][lane * V + q].x = sum.v[q];
-        __syncthreads();
-        if (warp == 0 && p.on) {
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                double s = 0.0;
-                for (uint32_t n = 0; n < kBackWarps; ++n) s += (double)ex.map[n][lane * V + q].x;
-                sum.v[q] = (float)s;
+                    for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
             }
-            put_partial(g, p, w.in.gates, tile.k, sum);
+        });
+    if constexpr (Maps) {
+        store_map<V>(g.maps + w.segment * g.flat + p.i, A, e);
+    } else {
+        if (g.dh0 && w.segment == 0) store<float, V>(g.dh0 + p.i, e);
+        if (g.partial) {
+            Row<V> sum;
+#pragma unroll
+            for (int q = 0; q < V; ++q) sum.v[q] = (float)total[q];
+            put_partial(g, p, b.gates, w.segment, sum);
         }
     }
 }
@@ -690,24 +658,42 @@ cudaError_t step_narrow(cudaStream_t s, const Form &f, const StepArgs &a, dim3 g
     return wide ? launch_step<X, X, float>(s, f, a, grid) : launch_step<X, X, X>(s, f, a, grid);
 }
 
-template <typename X, typename G, typename Y, int V>
-cudaError_t launch_whole(cudaStream_t s, const Args &a, bool back) {
-    const uint32_t grid = (a.columns + 3) / 4;
-    if (back) back_whole_kernel<X, G, Y, V><<<grid, 128, 0, s>>>(a);
-    else scan_whole_kernel<X, G, Y, V><<<grid, 128, 0, s>>>(a);
+template <typename K>
+cudaError_t start(K kernel, cudaStream_t s, const Args &a, uint32_t slot) {
+    const uint32_t smem = kWarps * kDepth * slot;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    kernel<<<(uint32_t)(((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps), kWarps * 32, smem, s>>>(a);
     return cudaGetLastError();
 }
 template <typename X, typename G, typename Y, int V>
-cudaError_t launch_split(cudaStream_t s, const Args &a, bool back) {
-    const uint32_t grid = a.tiles * a.columns;
-    if (back) back_split_kernel<X, G, Y, V><<<grid, kBackWarps * 32, 0, s>>>(a);
-    else scan_split_kernel<X, G, Y, V><<<grid, kScanWarps * 32, 0, s>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_scan(cudaStream_t s, const Args &a) {
+    constexpr uint32_t slot = Feed<X, V>::kBytes + Feed<G, V>::kBytes;
+    if (a.segments > 1) {
+        cudaError_t e = start(scan_kernel<X, G, Y, V, true>, s, a, slot);
+        if (e == cudaSuccess) e = carry(s, a, false);
+        if (e != cudaSuccess) return e;
+    }
+    return start(scan_kernel<X, G, Y, V, false>, s, a, slot);
+}
+template <typename X, typename G, typename Y, int V>
+cudaError_t launch_back(cudaStream_t s, const Args &a) {
+    constexpr uint32_t slot = Feed<G, V>::kBytes + Feed<Y, V>::kBytes;
+    if (a.segments > 1) {
+        cudaError_t e = start(back_kernel<X, G, Y, V, true>, s, a, slot);
+        if (e == cudaSuccess) e = carry(s, a, true);
+        if (e != cudaSuccess) return e;
+    }
+    return start(back_kernel<X, G, Y, V, false>, s, a, slot + Feed<X, V>::kBytes);
 }
 template <typename X, typename G, typename Y>
 cudaError_t launch(cudaStream_t s, const Form &f, const Args &a, bool back) {
-    if (f.split) return f.width == 2 ? launch_split<X, G, Y, 2>(s, a, back) : launch_split<X, G, Y, 1>(s, a, back);
-    return f.width == 2 ? launch_whole<X, G, Y, 2>(s, a, back) : launch_whole<X, G, Y, 1>(s, a, back);
+    if constexpr (std::is_same<X, Spike>::value)
+        if (f.width == 4) return launch_scan<X, G, Y, 4>(s, a);
+    if (back) return f.width == 2 ? launch_back<X, G, Y, 2>(s, a) : launch_back<X, G, Y, 1>(s, a);
+    return f.width == 2 ? launch_scan<X, G, Y, 2>(s, a) : launch_scan<X, G, Y, 1>(s, a);
 }
 
 // The combinations of types for 32-bit and spike inputs, and for 16-bit ones.

@@ -7,9 +7,9 @@
 namespace b200 {
 namespace leaky {
 
-constexpr uint32_t kSteps = SNN_B200_LEAKY_BLOCK;  // steps a thread holds in registers
-constexpr uint32_t kScanWarps = 16, kBackWarps = 8;  // warps of a tile (one CTA), kSteps of the steps each
-constexpr uint32_t kSuper = 16;              // tiles between two published states
+constexpr uint32_t kSteps = SNN_B200_LEAKY_BLOCK;  // steps worked on at a time, and of a saved state
+constexpr uint32_t kWarps = 4;                     // of a CTA
+constexpr uint32_t kDepth = 4;                     // blocks of steps under way or at hand
 
 struct Args {
     uint64_t flat;  // batch * channels
@@ -22,22 +22,24 @@ struct Args {
     int64_t xb, xt, gb, gt, yb, yt, dyb, dyt, dxb, dxt, dgb, dgt;
     float decay, scale;
     int logit, complement;
-    // Work split along the steps: a ticket, flags and what tiles publish.
-    uint32_t tiles, columns;  // tiles along the steps, warps' widths across the channels
-    uint32_t *ticket, *tile_flags, *state_flags;
-    float2 *aggregates;  // [tiles][columns * width]
-    float *states;       // [tiles / kSuper][columns * width]
-    float *partial;      // backward: sums of a shared gate's gradient, [tiles (1 unsplit)][flat]
+    uint32_t columns;                  // warps' widths across the channels
+    uint32_t segments, segment_steps;  // along the steps
+    float2 *maps;                      // [segments][flat], (A, H) of h -> A h + H
+    float *states;                     // [segments][flat], before each (backward: behind each)
+    float *partial;                    // backward: sums of a shared gate's gradient, [segments][flat]
 };
 
 // x's type is the translation unit's; g and y are snn_b200_dtype_t, `every`
 // says that the gate has a value for every step. width: channels a thread
-// holds. split: tiles along the steps.
+// holds.
 struct Form {
     int gate_dtype, y_dtype;
-    bool every, split;
+    bool every;
     uint32_t width;
 };
+
+// The states between segments from their maps.
+cudaError_t carry(cudaStream_t s, const Args &a, bool back);
 
 cudaError_t forward_f32(cudaStream_t s, const Form &f, const Args &a);
 cudaError_t forward_f16(cudaStream_t s, const Form &f, const Args &a);

@@ -24,8 +24,7 @@
 //    order of their ranks.
 // Every wait is bounded; one that gives up makes its tile NaN.
 #include "b200_mx4.h"
-
-#include <cuda.h>
+#include "b200_tma.h"
 
 #include <algorithm>
 
@@ -37,46 +36,14 @@ constexpr uint32_t kRows = 128;        // weight rows of a tile
 constexpr uint32_t kStageK = 256;      // k of a stage
 constexpr uint32_t kStageBytes = 128;  // of a row
 constexpr uint32_t kScaleTile = 512;
-constexpr uint32_t kPolls = 1u << 24;
 
-__device__ __forceinline__ uint32_t smem_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// ---- barriers ----
-__device__ __forceinline__ void bar_init(uint64_t *b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_of(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_of(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t *b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(b)) : "memory");
-}
-__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
-    const uint32_t at = smem_of(b);
-    for (uint32_t i = 0; i < kPolls; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(done)
-            : "r"(at), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
-
-// ---- copies ----
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_of(bar))
-        : "memory");
-}
-__device__ __forceinline__ void load_run(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(smem_of(bar))
-                 : "memory");
-}
+using tma::bar_arrive;
+using tma::bar_expect;
+using tma::bar_init;
+using tma::bar_wait;
+using tma::load_box;
+using tma::load_run;
+using tma::smem_of;
 
 // ---- tensor memory and instructions ----
 __device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t columns) {
@@ -218,7 +185,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         for (uint32_t s = 0; s < kWideStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
         bar_init(&s_ready, 1);
         bar_init(&s_free, 256);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma::bar_init_done();
     }
     if (warp == 0) tmem_alloc(&s_tmem, 512);
     fence_before();
@@ -345,7 +312,7 @@ __global__ void __launch_bounds__(128)
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < K::kStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
         bar_init(&s_ready, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tma::bar_init_done();
     }
     if (warp == 0) tmem_alloc(&s_tmem, K::kColumns);
     fence_before();
@@ -417,33 +384,11 @@ __global__ void __launch_bounds__(128)
 }
 
 // ---- host side ----
-using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                            const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                            CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-Encode encoder() {
-    static Encode f = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
-            r != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return (Encode)p;
-    }();
-    return f;
-}
-
 // Boxes of `box` rows and 128 bytes of a packed matrix.
 cudaError_t map_of(CUtensorMap *map, const Packed &q, uint64_t k, uint32_t box) {
-    const Encode f = encoder();
-    if (f == nullptr) return cudaErrorNotSupported;
     const cuuint64_t dims[2] = {blocks_of(k) * 16, q.rows}, strides[1] = {blocks_of(k) * 16};
-    const cuuint32_t boxes[2] = {kStageBytes, box}, steps[2] = {1, 1};
-    return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(q.codes), dims, strides, boxes, steps,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? cudaSuccess
-               : cudaErrorInvalidValue;
+    const cuuint32_t boxes[2] = {kStageBytes, box};
+    return tma::encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q.codes, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <typename T>

@@ -183,6 +183,9 @@ def test_long_sequences_keep_their_accuracy():
     p = Problem(1, 70001, 5, "f32", "channel", seed=10)
     p.verify()
     Problem(1, 33000, 3, "bf16", "step", "bf16", None, True, True, seed=11).verify()
+    Problem(1, 40000, 64, "bf16", "step", "bf16", None, True, True, seed=15).verify()
+    Problem(2, 17000, 48, "f32", "step", "f32", None, False, True, lengths=[17000, 9000], seed=16).verify()
+    Problem(1, 35000, 80, "u8", "channel", "f32", None, False, False, seed=17).verify()
 
 
 def test_gradient_against_differences():

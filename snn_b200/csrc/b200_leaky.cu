@@ -153,10 +153,20 @@ bool pieces(uint32_t n, const void *p, uint32_t bytes, int64_t sb, int64_t st) {
 }
 bool float_pieces(uint32_t n, const float *p) { return aligned_to(p, 4 * n); }
 
+// 16 bytes of a row at a time, from one sequence each.
+bool wide_rows(const void *p, int dtype, uint64_t channels, int64_t sb, int64_t st) {
+    const uint32_t n = 16 / dtype_bytes(dtype);
+    return channels % n == 0 && pieces(n, p, dtype_bytes(dtype), sb, st);
+}
+
 cudaError_t run(cudaStream_t s, const snn_b200_leaky_t &q, Args &g, const Plan &p, uint32_t width, bool back,
                 void *workspace) {
     fill(g, q, p, workspace);
-    const Form f = {q.gate_dtype, q.y_dtype, g.gate && q.gate_step_stride, width};
+    const bool every = g.gate && q.gate_step_stride;
+    g.wide = wide_rows(g.x, q.x_dtype, q.channels, q.x_batch_stride, q.x_step_stride) &&
+             (!every || wide_rows(g.gate, q.gate_dtype, q.channels, q.gate_batch_stride, q.gate_step_stride)) &&
+             (!back || wide_rows(g.dy, q.y_dtype, q.channels, q.dy_batch_stride, q.dy_step_stride));
+    const Form f = {q.gate_dtype, q.y_dtype, every, width};
     switch (q.x_dtype) {
         case SNN_B200_F32: return back ? backward_f32(s, f, g) : forward_f32(s, f, g);
         case SNN_B200_F16: return back ? backward_f16(s, f, g) : forward_f16(s, f, g);

@@ -213,48 +213,76 @@ __device__ __forceinline__ int live_steps(uint32_t len, uint32_t t0) {
     return len <= t0 ? 0 : (int)min(len - t0, kSteps);
 }
 
-// A block's rows of an array: copied ahead to shared memory where a thread's
-// piece of a row has the size of a copy (4 bytes or more), else loaded when the
-// block is worked on.
+// A block's rows of an array: copied ahead to the warp's shared memory, in
+// pieces of 16 bytes that the lanes share where every row allows it (g.wide),
+// in the thread's own pieces where those are 4 bytes or more, else loaded when
+// the block is worked on.
 template <typename T, int V>
 struct Feed {
-    static constexpr bool kShared = sizeof(T) * V >= 4;
-    static constexpr uint32_t kBytes = kShared ? (uint32_t)sizeof(T) * 32 * V * kSteps : 0;  // a block, a warp
-    const T *p;
+    static constexpr uint32_t kOwn = (uint32_t)sizeof(T) * V;           // bytes of a thread's piece of a row
+    static constexpr uint32_t kRow = 32 * kOwn, kBytes = kRow * kSteps;  // of a row, of a block
+    static constexpr uint32_t kAcross = kRow / 16, kAtOnce = 32 / kAcross;  // lanes on a row, rows of a copy
+    const T *p, *q;  // the thread's piece, the one it copies
     int64_t stride;
+    uint32_t len;  // of the sequence it copies from
+    bool wide;
 
-    __device__ __forceinline__ void init(const void *base, const Place &at, int64_t sb, int64_t st) {
+    __device__ __forceinline__ void init(const Args &g, const void *base, const Place &at, uint64_t column, int64_t sb,
+                                         int64_t st) {
         p = (const T *)base + at.b * sb + at.c;
         stride = st;
+        wide = g.wide;
+        if (wide) {
+            const uint64_t i = column * 32 * V + (threadIdx.x & 31) % kAcross * (16 / sizeof(T));
+            const int64_t b = i < g.flat ? (int64_t)(i / g.channels) : 0;
+            q = (const T *)base + b * sb + (int64_t)(i - (uint64_t)b * g.channels);
+            len = i >= g.flat ? 0u : g.lengths ? min(g.lengths[b], g.steps) : g.steps;
+        } else {
+            q = p;
+            len = at.len;
+        }
+    }
+    template <uint32_t N>
+    static __device__ __forceinline__ void copy(uint32_t to, const void *from) {
+        if constexpr (N == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(N) : "memory");
     }
     // slot: the warp's memory for the block.
-    __device__ __forceinline__ void fetch(uint8_t *slot, uint32_t t0, int live) const {
-        if constexpr (kShared) {
-            const T *row = p + (int64_t)t0 * stride;
-            const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + (threadIdx.x & 31) * (uint32_t)sizeof(T) * V;
+    __device__ __forceinline__ void fetch(uint8_t *slot, uint32_t t0) const {
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(slot), lane = threadIdx.x & 31;
+        const int live = live_steps(len, t0);
+        const T *row = q + (int64_t)t0 * stride;
+        if (wide) {
+#pragma unroll
+            for (uint32_t j = 0; j < kSteps; j += kAtOnce) {
+                const uint32_t r = j + lane / kAcross;
+                if ((int)r < live) copy<16>(at + (j * kAcross + lane) * 16, row + r * stride);
+            }
+        } else if constexpr (kOwn >= 4) {
 #pragma unroll
             for (int j = 0; j < (int)kSteps; ++j)
-                if (j < live)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to + j * (uint32_t)sizeof(T) * 32 * V),
-                                 "l"(row + j * stride), "n"(sizeof(T) * V)
-                                 : "memory");
+                if (j < live) copy<kOwn>(at + j * kRow + lane * kOwn, row + j * stride);
         }
     }
     // The block's rows; those behind the live ones are anything.
     __device__ __forceinline__ void take(const uint8_t *slot, uint32_t t0, int live, Vec<T, V> (&r)[kSteps]) const {
-        const T *row = p + (int64_t)t0 * stride;
+        if (kOwn >= 4 || wide) {
 #pragma unroll
-        for (int j = 0; j < (int)kSteps; ++j)
-            if constexpr (kShared) r[j] = reinterpret_cast<const Vec<T, V> *>(slot)[j * 32 + (threadIdx.x & 31)];
-            else r[j] = j < live ? load<T, V>(row + j * stride) : Vec<T, V>{};
+            for (int j = 0; j < (int)kSteps; ++j)
+                r[j] = *reinterpret_cast<const Vec<T, V> *>(slot + j * kRow + (threadIdx.x & 31) * kOwn);
+        } else {
+            const T *row = p + (int64_t)t0 * stride;
+#pragma unroll
+            for (int j = 0; j < (int)kSteps; ++j) r[j] = j < live ? load<T, V>(row + j * stride) : Vec<T, V>{};
+        }
     }
 };
 template <int V>
 struct Feed<Fixed, V> {
-    static constexpr bool kShared = true;
     static constexpr uint32_t kBytes = 0;
-    __device__ __forceinline__ void init(const void *, const Place &, int64_t, int64_t) {}
-    __device__ __forceinline__ void fetch(uint8_t *, uint32_t, int) const {}
+    __device__ __forceinline__ void init(const Args &, const void *, const Place &, uint64_t, int64_t, int64_t) {}
+    __device__ __forceinline__ void fetch(uint8_t *, uint32_t) const {}
 };
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -279,7 +307,9 @@ __device__ __forceinline__ void walk_blocks(uint32_t t0, uint32_t t1, Fetch fetc
         if (n + kDepth - 1 < blocks) fetch(at(n + kDepth - 1), to);
         fetched();
         await<kDepth - 1>();
+        __syncwarp();
         work(at(n), slot);
+        __syncwarp();  // the slot may be copied to again
         slot = slot + 1 == kDepth ? 0 : slot + 1;
     }
 }
@@ -308,7 +338,8 @@ struct Gates<Fixed, V> {
 #pragma unroll
         for (int q = 0; q < V; ++q) {
             const Leak l = !g.gate ? Leak{g.decay, __fsub_rn(1.0f, g.decay)}
-                                   : leak_from(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit);
+                           : p.on  ? leak_from(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit)
+                                   : Leak{1.0f, 0.0f};
             a_.v[q] = l.a, rest_.v[q] = l.rest;
         }
     }
@@ -368,27 +399,22 @@ __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_const
     extern __shared__ __align__(16) uint8_t s_feed[];
     const Part w = part_of(g, Maps);
     if (!w.on) return;
-    const Place p = place_of<V>(g, w.column);
-    if (!p.on) return;
+    const Place p = place_of<V>(g, w.column);  // lanes behind the last channel only help to copy
     constexpr uint32_t kX = Feed<X, V>::kBytes, kSlot = kX + Feed<G, V>::kBytes;
     uint8_t *mine = s_feed + threadIdx.x / 32 * (kDepth * kSlot);
     Feed<X, V> fx;
     Feed<G, V> fz;
     Gates<G, V> gates;
     gates.init(g, p);
-    fx.init(g.x, p, g.xb, g.xt);
-    fz.init(g.gate, p, g.gb, g.gt);
-    Row<V> h = Maps ? all<V>(0.0f) : g.segments > 1 ? load<float, V>(g.states + w.segment * g.flat + p.i)
-                                                    : load_state<V>(g.h0, p.i);
-    Row<V> A = all<V>(1.0f);
-    // Behind the sequence nothing happens to the map.
-    const uint32_t end = Maps ? max(w.t0, min(w.t1, p.len)) : w.t1;
+    fx.init(g, g.x, p, w.column, g.xb, g.xt);
+    fz.init(g, g.gate, p, w.column, g.gb, g.gt);
+    Row<V> h = all<V>(0.0f), A = all<V>(1.0f);
+    if (!Maps && p.on) h = load_state<V>(g.segments > 1 ? g.states + w.segment * g.flat : g.h0, p.i);
     walk_blocks<false>(
-        w.t0, end,
+        w.t0, w.t1,
         [&](uint32_t t0, uint32_t slot) {
-            const int live = live_steps(p.len, t0);
-            fz.fetch(mine + slot * kSlot + kX, t0, live);
-            fx.fetch(mine + slot * kSlot, t0, live);
+            fz.fetch(mine + slot * kSlot + kX, t0);
+            fx.fetch(mine + slot * kSlot, t0);
         },
         [&](uint32_t t0, uint32_t slot) {
             const int live = live_steps(p.len, t0);
@@ -400,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_const
                     A = mul(a, A);
                     h = fma(a, h, u);
                 });
-            } else {
+            } else if (p.on) {
                 if (g.saved) store<float, V>(saved_at(g, p, t0), h);
                 Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
                 each_step<X, G, V>(g, gates, x, live, [&](int j, const Row<V> &a, const Row<V> &u) {
@@ -411,6 +437,7 @@ __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_const
                     for (int j = live; j < (int)min(w.t1 - t0, kSteps); ++j) store<Y, V>(y + j * g.yt, Vec<Y, V>{});
             }
         });
+    if (!p.on) return;
     if constexpr (Maps) {
         store_map<V>(g.maps + w.segment * g.flat + p.i, A, h);
     } else {
@@ -508,35 +535,41 @@ template <typename G, int V>
 __device__ __forceinline__ void put_partial(const Args &, const Place &, const Gates<G, V> &, uint32_t,
                                             const Row<V> &) {}
 
+template <int V>
+constexpr uint32_t kSavedBytes = 32 * V * 4;  // the states before a block
+
 // Maps: only each segment's map of e is wanted, for which x does not count.
 template <typename X, typename G, typename Y, int V, bool Maps>
 __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
     const Part w = part_of(g, Maps);
     if (!w.on) return;
-    const Place p = place_of<V>(g, w.column);
-    if (!p.on) return;
-    constexpr uint32_t kY = Feed<Y, V>::kBytes, kZ = kY + Feed<G, V>::kBytes, kSlot = kZ + (Maps ? 0 : Feed<X, V>::kBytes);
+    const Place p = place_of<V>(g, w.column);  // lanes behind the last channel only help to copy
+    constexpr uint32_t kY = Feed<Y, V>::kBytes, kZ = kY + Feed<G, V>::kBytes, kS = kZ + (Maps ? 0 : Feed<X, V>::kBytes),
+                       kSlot = kS + (Maps ? 0 : kSavedBytes<V>);
     uint8_t *mine = s_feed + threadIdx.x / 32 * (kDepth * kSlot);
     Feed<X, V> fx;
     Feed<G, V> fz;
     Feed<Y, V> fy;
-    fx.init(g.x, p, g.xb, g.xt);
-    fz.init(g.gate, p, g.gb, g.gt);
-    fy.init(g.dy, p, g.dyb, g.dyt);
+    if (!Maps) fx.init(g, g.x, p, w.column, g.xb, g.xt);
+    fz.init(g, g.gate, p, w.column, g.gb, g.gt);
+    fy.init(g, g.dy, p, w.column, g.dyb, g.dyt);
     Back<X, G, Y, V> b;
     b.gates.init(g, p);
-    Row<V> e = Maps ? all<V>(0.0f) : g.segments > 1 ? load<float, V>(g.states + w.segment * g.flat + p.i)
-                                                    : load_state<V>(g.dh_last, p.i);
-    Row<V> A = all<V>(1.0f);
+    Row<V> e = all<V>(0.0f), A = all<V>(1.0f);
+    if (!Maps && p.on) e = load_state<V>(g.segments > 1 ? g.states + w.segment * g.flat : g.dh_last, p.i);
     double total[V] = {};
     walk_blocks<true>(
-        w.t0, Maps ? max(w.t0, min(w.t1, p.len)) : w.t1,
+        w.t0, w.t1,
         [&](uint32_t t0, uint32_t slot) {
-            const int live = live_steps(p.len, t0);
-            fy.fetch(mine + slot * kSlot, t0, live);
-            fz.fetch(mine + slot * kSlot + kY, t0, live);
-            if (!Maps) fx.fetch(mine + slot * kSlot + kZ, t0, live);
+            fy.fetch(mine + slot * kSlot, t0);
+            fz.fetch(mine + slot * kSlot + kY, t0);
+            if (Maps) return;
+            fx.fetch(mine + slot * kSlot + kZ, t0);
+            if (p.on && t0 < p.len)
+                Feed<float, V>::template copy<4 * V>(
+                    (uint32_t)__cvta_generic_to_shared(mine + slot * kSlot + kS) + (threadIdx.x & 31) * 4 * V,
+                    saved_at(g, p, t0));
         },
         [&](uint32_t t0, uint32_t slot) {
             const int live = live_steps(p.len, t0);
@@ -554,7 +587,7 @@ __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const _
                         }
                 });
             } else {
-                const Row<V> h = live ? load<float, V>(saved_at(g, p, t0)) : all<V>(0.0f);
+                const Row<V> h = reinterpret_cast<const Row<V> *>(mine + slot * kSlot + kS)[threadIdx.x & 31];
                 Vec<X, V> x[kSteps];
                 fx.take(mine + slot * kSlot + kZ, t0, live, x);
                 b.maps(g, x, h, live);
@@ -564,6 +597,7 @@ __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const _
                     for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
             }
         });
+    if (!p.on) return;
     if constexpr (Maps) {
         store_map<V>(g.maps + w.segment * g.flat + p.i, A, e);
     } else {
@@ -686,7 +720,7 @@ cudaError_t launch_back(cudaStream_t s, const Args &a) {
         if (e == cudaSuccess) e = carry(s, a, true);
         if (e != cudaSuccess) return e;
     }
-    return start(back_kernel<X, G, Y, V, false>, s, a, slot + Feed<X, V>::kBytes);
+    return start(back_kernel<X, G, Y, V, false>, s, a, slot + Feed<X, V>::kBytes + kSavedBytes<V>);
 }
 template <typename X, typename G, typename Y>
 cudaError_t launch(cudaStream_t s, const Form &f, const Args &a, bool back) {

@@ -22,6 +22,7 @@ struct Args {
     int64_t xb, xt, gb, gt, yb, yt, dyb, dyt, dxb, dxt, dgb, dgt;
     float decay, scale;
     int logit, complement;
+    int wide;                          // rows of x, gate and dy can be read in pieces of 16 bytes
     uint32_t columns;                  // warps' widths across the channels
     uint32_t segments, segment_steps;  // along the steps
     float2 *maps;                      // [segments][flat], (A, H) of h -> A h + H

@@ -113,7 +113,7 @@ struct Plan {
 };
 // Walks of whole sequences, or segments of them (64 steps at least) where
 // those would be too few to keep the loads of 148 SMs under way.
-constexpr uint64_t kFewWalks = 148 * 12, kManyWalks = 148 * 48;
+constexpr uint64_t kFewWalks = 148 * 5, kManyWalks = 148 * 48;
 constexpr uint32_t kLeastSegment = 64;
 Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     Plan p = {};

@@ -1,22 +1,10 @@
 // Packed 4-bit matrices (MXFP4): packing, reading back and the product.
-#include "b200_mx4.h"
+#include "b200_mx4.cuh"
 
 namespace b200 {
 namespace mx4 {
 namespace {
 
-__host__ __device__ inline uint64_t scale_offset(uint64_t r, uint64_t b, uint64_t tiles) {
-    return 512 * ((r / 128) * tiles + b / 4) + 16 * (r % 32) + 4 * (r % 128 / 32) + b % 4;
-}
-
-__device__ __forceinline__ float load_any(const void *p, int dtype, int64_t i) {
-    switch (dtype) {
-        case SNN_B200_F32: return ((const float *)p)[i];
-        case SNN_B200_F16: return to_float(((const __half *)p)[i]);
-        case SNN_B200_BF16: return to_float(((const __nv_bfloat16 *)p)[i]);
-        default: return to_float(((const Spike *)p)[i]);
-    }
-}
 __device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v) {
     switch (dtype) {
         case SNN_B200_F32: ((float *)p)[i] = v; break;
@@ -25,70 +13,122 @@ __device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v
     }
 }
 
-// The scale byte of a block from its largest magnitude (bits of a
-// non-negative float): exponent - 2, at least 2^-127, 255 when not finite.
-// Scale byte s stands for 2^(s - 127) and the float's exponent field f for
-// 2^(f - 127), so the byte is f - 2.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
-    const uint32_t f = amax_bits >> 23;
-    return f == 255u ? 255u : f > 2u ? f - 2u : 0u;
-}
-// 2^(127 - s) for s of 0..252.
-__device__ __forceinline__ float inverse_scale(uint32_t s) { return __uint_as_float((254u - s) << 23); }
-// 2^(s - 127), the smallest one subnormal.
-__device__ __forceinline__ float scale_value(uint32_t s) {
-    return s == 255u ? __uint_as_float(0x7fffffffu) : s ? __uint_as_float(s << 23) : __uint_as_float(0x00400000u);
-}
-// e2m1 code of v, ties to the even code, saturating.
-__device__ __forceinline__ uint32_t encode(float v) {
-    const float m = fabsf(v);
-    uint32_t c = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.0f);
-    return c | (__float_as_uint(v) >> 31 << 3);
-}
-__device__ __forceinline__ float decode(uint32_t c) {
-    const uint32_t m = c & 7u;
-    const float v = m < 4u ? 0.5f * (float)m : m < 6u ? (float)(m - 2u) : (m == 6u ? 4.0f : 6.0f);
-    return c & 8u ? -v : v;
-}
+// 128 rows x 4 blocks: the unit of the packers' CTAs, and one tile of scales.
+constexpr uint32_t kTileRows = 128, kTileCols = 128;
 
-// One thread a (padded) block.
-__global__ void mx4_quantize_kernel(const void *src, int dtype, uint64_t rows, uint64_t cols, int64_t rs, int64_t cs,
-                                    uint4 *codes, uint8_t *scales) {
-    const uint64_t nb = blocks_of(cols), tiles = scale_tiles(cols);
-    const uint64_t padded_rows = (rows + 127) / 128 * 128, padded_blocks = tiles * 4;
-    const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < padded_rows * padded_blocks; i += step) {
-        const uint64_t r = i / padded_blocks, b = i % padded_blocks;
-        uint32_t s = 0;
-        if (r < rows && b < nb) {
-            float v[kBlock];
-            uint32_t top = 0;
-            for (uint32_t k = 0; k < kBlock; ++k) {
-                const uint64_t c = b * kBlock + k;
-                v[k] = c < cols ? load_any(src, dtype, (int64_t)r * rs + (int64_t)c * cs) : 0.0f;
-                top = max(top, __float_as_uint(fabsf(v[k])));
-            }
-            s = scale_byte(top);
-            uint32_t w[4] = {};
-            if (s != 255u) {
-                const float inv = inverse_scale(s);
-                for (uint32_t k = 0; k < kBlock; ++k) w[k / 8] |= encode(__fmul_rn(v[k], inv)) << (4 * (k % 8));
-            }
-            codes[r * nb + b] = make_uint4(w[0], w[1], w[2], w[3]);
+// Rows of neighbouring elements that can be read 16 bytes at a time. Lanes lie
+// across a row, each with the elements of one 16-byte load, and find their
+// block's largest magnitude by shuffles, so loads and stores are whole runs.
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, uint32_t rows, uint32_t cols, int64_t rs,
+                                                                uint8_t *codes, uint8_t *scales, uint32_t tiles) {
+    constexpr uint32_t kOwn = 16 / sizeof(T), kAcross = kTileCols / kOwn;  // elements of a lane, lanes on a row
+    constexpr uint32_t kRowsAtOnce = 256 / kAcross, kPasses = kTileRows / kRowsAtOnce, kLanes = kBlock / kOwn;
+    constexpr uint32_t kHeld = kPasses < 8 ? kPasses : 8;  // loads under way
+    __shared__ __align__(16) uint8_t s_scales[512];
+    const uint32_t tile = blockIdx.x, r0 = blockIdx.y * kTileRows;
+    const uint32_t part = threadIdx.x % kAcross, first = threadIdx.x / kAcross, c = tile * kTileCols + part * kOwn;
+    const uint64_t pitch = blocks_of(cols) * 16;
+#pragma unroll 1
+    for (uint32_t pass = 0; pass < kPasses; pass += kHeld) {
+        Piece<T> v[kHeld];
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) {
+            const uint32_t r = r0 + (pass + i) * kRowsAtOnce + first;
+            if (r < rows && c < cols) v[i] = load_piece(src + (int64_t)r * rs + c, cols - c);
+            else v[i] = Piece<T>{};
         }
-        scales[scale_offset(r, b, tiles)] = (uint8_t)s;
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) {
+            const uint32_t at = (pass + i) * kRowsAtOnce + first, r = r0 + at;
+            uint32_t top = v[i].largest();
+#pragma unroll
+            for (uint32_t d = 1; d < kLanes; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const uint32_t s = scale_byte(top);
+            v[i].store(codes + r * pitch + c / 2, s, r < rows && c / kBlock < (cols + kBlock - 1) / kBlock);
+            if (part % kLanes == 0) s_scales[scale_slot(at, part / kLanes)] = (uint8_t)s;
+        }
     }
+    __syncthreads();
+    if (threadIdx.x < 32)
+        reinterpret_cast<uint4 *>(scales + ((uint64_t)blockIdx.y * tiles + tile) * 512)[threadIdx.x] =
+            reinterpret_cast<const uint4 *>(s_scales)[threadIdx.x];
 }
 
-__global__ void mx4_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, uint64_t rows, uint64_t cols,
-                                      void *dst, int dtype, int64_t rs) {
-    const uint64_t nb = blocks_of(cols), tiles = scale_tiles(cols);
-    const uint64_t step = (uint64_t)gridDim.x * blockDim.x;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * cols; i += step) {
-        const uint64_t r = i / cols, c = i % cols;
-        const uint32_t code = codes[r * nb * 16 + c / 2] >> (4 * (c & 1)) & 15u;
-        store_any(dst, dtype, (int64_t)r * rs + (int64_t)c,
-                  __fmul_rn(decode(code), scale_value(scales[scale_offset(r, c / kBlock, tiles)])));
+// Any strides: a thread a block, lanes along the rows, so a transposed source
+// is read in whole runs too.
+template <typename T>
+__global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uint32_t rows, uint32_t cols, int64_t rs,
+                                                               int64_t cs, uint8_t *codes, uint8_t *scales,
+                                                               uint32_t tiles) {
+    __shared__ __align__(16) uint8_t s_scales[512];
+    const uint32_t tile = blockIdx.x, at = threadIdx.x % kTileRows, b = threadIdx.x / kTileRows;
+    const uint64_t r = (uint64_t)blockIdx.y * kTileRows + at, c = (uint64_t)tile * kTileCols + b * kBlock;
+    uint32_t s = 0;
+    if (r < rows && c < cols) {
+        const T *p = src + (int64_t)r * rs + (int64_t)c * cs;
+        const uint32_t n = min(kBlock, (uint32_t)(cols - c));
+        float v[kBlock];
+        uint32_t top = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kBlock; ++k) v[k] = k < n ? to_float(p[(int64_t)k * cs]) : 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < kBlock; ++k) top = max(top, __float_as_uint(fabsf(v[k])));
+        s = scale_byte(top);
+        const float inv = inverse_scale(s);
+        uint32_t w[4];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) w[q] = s == 255u ? 0u : encode8(v + 8 * q, inv);
+        reinterpret_cast<uint4 *>(codes)[r * blocks_of(cols) + c / kBlock] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    s_scales[scale_slot(at, b)] = (uint8_t)s;
+    __syncthreads();
+    if (threadIdx.x < 32)
+        reinterpret_cast<uint4 *>(scales + ((uint64_t)blockIdx.y * tiles + tile) * 512)[threadIdx.x] =
+            reinterpret_cast<const uint4 *>(s_scales)[threadIdx.x];
+}
+
+// A thread 8 elements: 4 bytes of codes, written as whole 16-byte pieces where
+// the rows allow it.
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t rows,
+                                                             uint32_t cols, uint32_t tiles, T *dst, int64_t rs,
+                                                             bool pieces) {
+    const uint64_t pitch = blocks_of(cols) * 16;
+    const uint32_t c = (blockIdx.x * 64 + threadIdx.x % 64) * 8;
+    if (c >= cols) return;
+    const uint32_t b = c / kBlock;
+    for (uint64_t r0 = (uint64_t)blockIdx.y * 16 + threadIdx.x / 64; r0 < rows; r0 += (uint64_t)gridDim.y * 16) {
+        uint32_t w[4], s[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint64_t r = r0 + 4 * i;
+            w[i] = s[i] = 0;
+            if (r < rows) {
+                w[i] = *reinterpret_cast<const uint32_t *>(codes + r * pitch + c / 2);
+                s[i] = scales[512 * ((r / kTileRows) * tiles + b / 4) + scale_slot((uint32_t)(r % kTileRows), b % 4)];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint64_t r = r0 + 4 * i;
+            if (r >= rows) continue;
+            float v[8];
+            decode8(w[i], scale_value(s[i]), v);
+            T *to = dst + (int64_t)r * rs + c;
+            if (pieces && c + 8 <= cols) {
+                Eight<T> o;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) o.v[q] = from_float<T>(v[q]);
+#pragma unroll
+                for (uint32_t q = 0; q < sizeof(T) / 2; ++q)
+                    reinterpret_cast<uint4 *>(to)[q] = reinterpret_cast<const uint4 *>(&o)[q];
+            } else {
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q)
+                    if (c + q < cols) to[q] = from_float<T>(v[q]);
+            }
+        }
     }
 }
 
@@ -122,11 +162,39 @@ snn_status_t check_rows(const void *out, int dtype, snn_size_t rows, snn_size_t 
     return SNN_OK;
 }
 
-void enqueue_quantize(int device, cudaStream_t s, const void *src, int dtype, uint64_t rows, uint64_t cols, int64_t rs,
-                      int64_t cs, void *codes, void *scales) {
-    const uint64_t padded = (rows + 127) / 128 * 128 * scale_tiles(cols) * 4;
-    mx4_quantize_kernel<<<grid_for(device, padded, 128), 128, 0, s>>>(src, dtype, rows, cols, rs, cs, (uint4 *)codes,
-                                                                      (uint8_t *)scales);
+template <typename T>
+void quantize_as(cudaStream_t s, const void *src, uint64_t rows, uint64_t cols, int64_t rs, int64_t cs, uint8_t *codes,
+                 uint8_t *scales) {
+    const uint32_t tiles = (uint32_t)scale_tiles(cols);
+    // Tiles of rows beyond a grid's height go in several launches.
+    for (uint64_t r0 = 0; r0 < rows; r0 += 65535ull * kTileRows) {
+        const uint64_t n = rows - r0 < 65535ull * kTileRows ? rows - r0 : 65535ull * kTileRows;
+        const dim3 grid(tiles, (uint32_t)((n + kTileRows - 1) / kTileRows));
+        const T *from = (const T *)src + (int64_t)r0 * rs;
+        uint8_t *c = codes + code_bytes(r0, cols), *x = scales + scale_bytes(r0, cols);
+        if (cs == 1 && aligned_to(src, 16) && rs * (int64_t)sizeof(T) % 16 == 0)
+            mx4_quantize_rows_kernel<T><<<grid, 256, 0, s>>>(from, (uint32_t)n, (uint32_t)cols, rs, c, x, tiles);
+        else
+            mx4_quantize_any_kernel<T><<<grid, 512, 0, s>>>(from, (uint32_t)n, (uint32_t)cols, rs, cs, c, x, tiles);
+    }
+}
+void enqueue_quantize(cudaStream_t s, const void *src, int dtype, uint64_t rows, uint64_t cols, int64_t rs, int64_t cs,
+                      void *codes, void *scales) {
+    uint8_t *c = (uint8_t *)codes, *x = (uint8_t *)scales;
+    switch (dtype) {
+        case SNN_B200_F32: return quantize_as<float>(s, src, rows, cols, rs, cs, c, x);
+        case SNN_B200_F16: return quantize_as<__half>(s, src, rows, cols, rs, cs, c, x);
+        case SNN_B200_BF16: return quantize_as<__nv_bfloat16>(s, src, rows, cols, rs, cs, c, x);
+        default: return quantize_as<Spike>(s, src, rows, cols, rs, cs, c, x);
+    }
+}
+template <typename T>
+void dequantize_as(cudaStream_t s, const void *codes, const void *scales, uint64_t rows, uint64_t cols, void *dst,
+                   int64_t rs) {
+    const uint64_t high = (rows + 15) / 16;
+    mx4_dequantize_kernel<T><<<dim3((uint32_t)((cols + 511) / 512), (uint32_t)(high < 65535 ? high : 65535)), 256, 0, s>>>(
+        (const uint8_t *)codes, (const uint8_t *)scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)scale_tiles(cols),
+        (T *)dst, rs, aligned_to(dst, 16) && rs * (int64_t)sizeof(T) % 16 == 0);
 }
 
 cudaError_t enqueue_matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,
@@ -165,7 +233,7 @@ snn_status_t snn_b200_mx4_quantize_async(int device, void *stream, const void *s
     if (rows == 0 || cols == 0) return SNN_OK;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
-    enqueue_quantize(device, (cudaStream_t)stream, src, src_dtype, rows, cols, row_stride, col_stride, codes, scales);
+    enqueue_quantize((cudaStream_t)stream, src, src_dtype, rows, cols, row_stride, col_stride, codes, scales);
     return op_status(cudaGetLastError(), __func__);
 }
 
@@ -179,8 +247,10 @@ snn_status_t snn_b200_mx4_dequantize_async(int device, void *stream, const void 
     if (rows == 0 || cols == 0) return SNN_OK;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
-    mx4_dequantize_kernel<<<grid_for(device, rows * cols, 256), 256, 0, (cudaStream_t)stream>>>(
-        (const uint8_t *)codes, (const uint8_t *)scales, rows, cols, dst, dst_dtype, row_stride);
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (dst_dtype == SNN_B200_F32) dequantize_as<float>(s, codes, scales, rows, cols, dst, row_stride);
+    else if (dst_dtype == SNN_B200_F16) dequantize_as<__half>(s, codes, scales, rows, cols, dst, row_stride);
+    else dequantize_as<__nv_bfloat16>(s, codes, scales, rows, cols, dst, row_stride);
     return op_status(cudaGetLastError(), __func__);
 }
 
@@ -224,7 +294,7 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
     uint8_t *codes = (uint8_t *)workspace, *scales = codes + code_bytes(m, k);
-    if (k) enqueue_quantize(device, (cudaStream_t)stream, x, x_dtype, m, k, x_row_stride, x_col_stride, codes, scales);
+    if (k) enqueue_quantize((cudaStream_t)stream, x, x_dtype, m, k, x_row_stride, x_col_stride, codes, scales);
     cudaError_t e = cudaGetLastError();
     const Packed xq = {codes, scales, m}, w = {(const uint8_t *)w_codes, (const uint8_t *)w_scales, n};
     if (e == cudaSuccess)

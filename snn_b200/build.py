@@ -7,6 +7,8 @@ cudart is linked statically (nvcc's default), so the library does not depend
 on which libcudart the host process (e.g. PyTorch) already loaded. NCCL is the
 one the installed PyTorch uses (the nvidia-nccl wheel), found through an
 rpath, so a process that also runs torch.distributed loads a single NCCL.
+snn_b200/_lib/sequence_ops.so, the sequence operators for torch tensors, is
+built beside it with g++ against the installed PyTorch.
 """
 from __future__ import annotations
 
@@ -17,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -24,6 +27,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(OUT_DIR, "libsnn_b200.so")
+TORCH_OPS = os.path.join(OUT_DIR, "sequence_ops.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 # --fmad=false: no FMA contraction anywhere (the reference's bit-parity rule,
@@ -60,6 +64,30 @@ def _newer(src_files, target) -> bool:
     return any(os.path.getmtime(f) > t for f in src_files)
 
 
+def torch_dir() -> str:
+    for p in sys.path:
+        d = os.path.join(p, "torch")
+        if os.path.exists(os.path.join(d, "include", "ATen", "ATen.h")):
+            return d
+    raise RuntimeError("PyTorch's headers not found")
+
+
+def build_torch_ops(headers, force: bool, verbose: bool) -> None:
+    src = os.path.join(CSRC, "torch", "sequence_ops.cpp")
+    if not (force or _newer([src] + headers, TORCH_OPS)):
+        return
+    t = torch_dir()
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(t, "include"), "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"], src, "-o", TORCH_OPS,
+           "-L", os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-L", OUT_DIR, "-lsnn_b200", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + os.path.join(t, "lib")]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -88,6 +116,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)
+    build_torch_ops([h for h in headers if h.startswith(os.path.join(ROOT, "include"))], force, verbose)
     return LIB
 
 

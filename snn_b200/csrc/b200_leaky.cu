@@ -22,6 +22,8 @@ __global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *m
     const uint32_t run = (segments + kCarryWarps - 1) / kCarryWarps;
     const uint32_t from = min(segments, warp * run), to = min(segments, from + run);
     const auto at = [&](uint32_t n) { return (uint64_t)(back ? segments - 1 - n : n) * flat + i; };
+    allow_next();
+    after_previous();
     float2 m = make_float2(1.0f, 0.0f);
     if (i < flat)
 #pragma unroll 8
@@ -54,6 +56,8 @@ __global__ void __launch_bounds__(kSumWarps * 32) gate_sum_kernel(const float *p
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane;
     const uint64_t flat = (uint64_t)batch * channels;
+    allow_next();
+    after_previous();
     for (uint32_t r = blockIdx.y; r < (row_stride ? batch : 1u); r += gridDim.y) {
         const uint64_t terms = row_stride ? segments : (uint64_t)segments * batch;
         // Term n of row r: segment n, sequence r; or n-th of all [segments][batch].
@@ -178,9 +182,8 @@ cudaError_t run(cudaStream_t s, const snn_b200_leaky_t &q, Args &g, const Plan &
 }  // namespace
 
 cudaError_t carry(cudaStream_t s, const Args &a, bool back) {
-    carry_kernel<<<(uint32_t)((a.flat + 31) / 32), kCarryWarps * 32, 0, s>>>(
-        a.maps, a.segments, a.flat, back ? a.dh_last : a.h0, a.states, back);
-    return cudaGetLastError();
+    return launch_early(carry_kernel, (uint32_t)((a.flat + 31) / 32), kCarryWarps * 32, 0, s, 1, a.maps, a.segments, a.flat,
+                        back ? a.dh_last : a.h0, a.states, back);
 }
 
 }  // namespace leaky
@@ -292,10 +295,8 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
     cudaError_t e = run(s, q, g, p, width, true, workspace);
     if (e == cudaSuccess && sums) {
         const uint32_t rows = shared ? 1u : (uint32_t)(q.batch < 65535 ? q.batch : 65535);
-        gate_sum_kernel<<<dim3((uint32_t)((q.channels + 31) / 32), rows), kSumWarps * 32, 0, s>>>(
-            g.partial, p.segments, (uint32_t)q.batch, (uint32_t)q.channels, (float *)dgate,
-            shared ? 0 : q.dgate_batch_stride);
-        e = cudaGetLastError();
+        e = launch_early(gate_sum_kernel, dim3((uint32_t)((q.channels + 31) / 32), rows), kSumWarps * 32, 0, s, 1, g.partial,
+                         p.segments, q.batch, q.channels, (float *)dgate, shared ? 0 : q.dgate_batch_stride);
     }
     return op_status(e, __func__);
 }

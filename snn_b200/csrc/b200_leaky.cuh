@@ -398,6 +398,8 @@ template <typename X, typename G, typename Y, int V, bool Maps>
 __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
     const Part w = part_of(g, Maps);
+    allow_next();
+    after_previous();
     if (!w.on) return;
     const Place p = place_of<V>(g, w.column);  // lanes behind the last channel only help to copy
     constexpr uint32_t kX = Feed<X, V>::kBytes, kSlot = kX + Feed<G, V>::kBytes;
@@ -543,6 +545,8 @@ template <typename X, typename G, typename Y, int V, bool Maps>
 __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
     const Part w = part_of(g, Maps);
+    allow_next();
+    after_previous();
     if (!w.on) return;
     const Place p = place_of<V>(g, w.column);  // lanes behind the last channel only help to copy
     constexpr uint32_t kY = Feed<Y, V>::kBytes, kZ = kY + Feed<G, V>::kBytes, kS = kZ + (Maps ? 0 : Feed<X, V>::kBytes),
@@ -620,6 +624,8 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
     __shared__ uint32_t s_before[8], s_after[8];  // rows named before, rows named again
     const uint32_t across = 256 / g.rows, mine = threadIdx.x / across;
     const uint32_t row = blockIdx.x * g.rows + mine;
+    allow_next();
+    after_previous();
     if (g.slots && g.batch > 1) {
         if (threadIdx.x < 8) s_before[threadIdx.x] = s_after[threadIdx.x] = 0u;
         __syncthreads();
@@ -676,9 +682,7 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
 
 template <typename X, typename G, typename Y>
 cudaError_t launch_step(cudaStream_t s, const Form &f, const StepArgs &a, dim3 grid) {
-    if (f.width == 4) step_kernel<X, G, Y, 4><<<grid, 256, 0, s>>>(a);
-    else step_kernel<X, G, Y, 1><<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(f.width == 4 ? step_kernel<X, G, Y, 4> : step_kernel<X, G, Y, 1>, grid, 256, 0, s, 1, a);
 }
 template <typename X>
 cudaError_t step_wide(cudaStream_t s, const Form &f, const StepArgs &a, dim3 grid) {
@@ -699,8 +703,8 @@ cudaError_t start(K kernel, cudaStream_t s, const Args &a, uint32_t slot) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    kernel<<<(uint32_t)(((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps), kWarps * 32, smem, s>>>(a);
-    return cudaGetLastError();
+    const uint32_t grid = (uint32_t)(((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps);
+    return launch_early(kernel, grid, kWarps * 32, smem, s, 1, a);
 }
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_scan(cudaStream_t s, const Args &a) {

@@ -29,6 +29,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, ui
     const uint32_t tile = blockIdx.x, r0 = blockIdx.y * kTileRows;
     const uint32_t part = threadIdx.x % kAcross, first = threadIdx.x / kAcross, c = tile * kTileCols + part * kOwn;
     const uint64_t pitch = blocks_of(cols) * 16;
+    allow_next();
+    after_previous();
 #pragma unroll 1
     for (uint32_t pass = 0; pass < kPasses; pass += kHeld) {
         Piece<T> v[kHeld];
@@ -65,6 +67,8 @@ __global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uin
     const uint32_t tile = blockIdx.x, at = threadIdx.x % kTileRows, b = threadIdx.x / kTileRows;
     const uint64_t r = (uint64_t)blockIdx.y * kTileRows + at, c = (uint64_t)tile * kTileCols + b * kBlock;
     uint32_t s = 0;
+    allow_next();
+    after_previous();
     if (r < rows && c < cols) {
         const T *p = src + (int64_t)r * rs + (int64_t)c * cs;
         const uint32_t n = min(kBlock, (uint32_t)(cols - c));
@@ -96,6 +100,8 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t *code
                                                              bool pieces) {
     const uint64_t pitch = blocks_of(cols) * 16;
     const uint32_t c = (blockIdx.x * 64 + threadIdx.x % 64) * 8;
+    allow_next();
+    after_previous();
     if (c >= cols) return;
     const uint32_t b = c / kBlock;
     for (uint64_t r0 = (uint64_t)blockIdx.y * 16 + threadIdx.x / 64; r0 < rows; r0 += (uint64_t)gridDim.y * 16) {
@@ -173,9 +179,9 @@ void quantize_as(cudaStream_t s, const void *src, uint64_t rows, uint64_t cols, 
         const T *from = (const T *)src + (int64_t)r0 * rs;
         uint8_t *c = codes + code_bytes(r0, cols), *x = scales + scale_bytes(r0, cols);
         if (cs == 1 && aligned_to(src, 16) && rs * (int64_t)sizeof(T) % 16 == 0)
-            mx4_quantize_rows_kernel<T><<<grid, 256, 0, s>>>(from, (uint32_t)n, (uint32_t)cols, rs, c, x, tiles);
+            launch_early(mx4_quantize_rows_kernel<T>, grid, 256, 0, s, 1, from, n, cols, rs, c, x, tiles);
         else
-            mx4_quantize_any_kernel<T><<<grid, 512, 0, s>>>(from, (uint32_t)n, (uint32_t)cols, rs, cs, c, x, tiles);
+            launch_early(mx4_quantize_any_kernel<T>, grid, 512, 0, s, 1, from, n, cols, rs, cs, c, x, tiles);
     }
 }
 void enqueue_quantize(cudaStream_t s, const void *src, int dtype, uint64_t rows, uint64_t cols, int64_t rs, int64_t cs,
@@ -192,9 +198,9 @@ template <typename T>
 void dequantize_as(cudaStream_t s, const void *codes, const void *scales, uint64_t rows, uint64_t cols, void *dst,
                    int64_t rs) {
     const uint64_t high = (rows + 15) / 16;
-    mx4_dequantize_kernel<T><<<dim3((uint32_t)((cols + 511) / 512), (uint32_t)(high < 65535 ? high : 65535)), 256, 0, s>>>(
-        (const uint8_t *)codes, (const uint8_t *)scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)scale_tiles(cols),
-        (T *)dst, rs, aligned_to(dst, 16) && rs * (int64_t)sizeof(T) % 16 == 0);
+    const dim3 grid((uint32_t)((cols + 511) / 512), (uint32_t)(high < 65535 ? high : 65535));
+    launch_early(mx4_dequantize_kernel<T>, grid, 256, 0, s, 1, (const uint8_t *)codes, (const uint8_t *)scales, rows, cols,
+                 scale_tiles(cols), (T *)dst, rs, aligned_to(dst, 16) && rs * (int64_t)sizeof(T) % 16 == 0);
 }
 
 cudaError_t enqueue_matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,
@@ -293,12 +299,16 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
     if (m == 0 || n == 0) return SNN_OK;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
+    const cudaStream_t s = (cudaStream_t)stream;
+    const Packed w = {(const uint8_t *)w_codes, (const uint8_t *)w_scales, n};
+    if (k && packs_on_the_way(x, x_dtype, m, x_row_stride, x_col_stride))
+        return op_status(linear(device, s, x, x_dtype, m, x_row_stride, w, k, bias, out, out_dtype, out_row_stride),
+                         __func__);
     uint8_t *codes = (uint8_t *)workspace, *scales = codes + code_bytes(m, k);
-    if (k) enqueue_quantize((cudaStream_t)stream, x, x_dtype, m, k, x_row_stride, x_col_stride, codes, scales);
+    if (k) enqueue_quantize(s, x, x_dtype, m, k, x_row_stride, x_col_stride, codes, scales);
     cudaError_t e = cudaGetLastError();
-    const Packed xq = {codes, scales, m}, w = {(const uint8_t *)w_codes, (const uint8_t *)w_scales, n};
-    if (e == cudaSuccess)
-        e = enqueue_matmul(device, (cudaStream_t)stream, xq, w, k, bias, out, out_dtype, out_row_stride);
+    const Packed xq = {codes, scales, m};
+    if (e == cudaSuccess) e = enqueue_matmul(device, s, xq, w, k, bias, out, out_dtype, out_row_stride);
     return op_status(e, __func__);
 }
 

@@ -99,12 +99,12 @@ struct Piece<Spike> {
         if (on) *reinterpret_cast<uint2 *>(to) = make_uint2(four(raw.x) | four(raw.y) << 16, four(raw.z) | four(raw.w) << 16);
     }
 };
-// The piece at p, of which n elements are left in the row.
-template <typename T>
+// The piece at p, of which n elements are left in the row; Again: others read it too.
+template <bool Again = false, typename T>
 __device__ __forceinline__ Piece<T> load_piece(const T *p, uint32_t n) {
     Piece<T> v;
     if (n >= Piece<T>::kOwn) {
-        v.raw = __ldcs(reinterpret_cast<const uint4 *>(p));
+        v.raw = Again ? *reinterpret_cast<const uint4 *>(p) : __ldcs(reinterpret_cast<const uint4 *>(p));
     } else {
         __align__(16) T e[Piece<T>::kOwn];
 #pragma unroll
@@ -112,6 +112,26 @@ __device__ __forceinline__ Piece<T> load_piece(const T *p, uint32_t n) {
         v.raw = *reinterpret_cast<const uint4 *>(e);
     }
     return v;
+}
+
+// The four words of a block's codes from its pieces.
+template <typename T, uint32_t N>
+__device__ __forceinline__ void pack_block(const Piece<T> (&v)[N], uint32_t s, uint32_t (&w)[4]) {
+    const float inv = inverse_scale(s);
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) {
+        float e[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) e[i] = v[(8 * q + i) / Piece<T>::kOwn].at((8 * q + i) % Piece<T>::kOwn);
+        w[q] = s == 255u ? 0u : encode8(e, inv);
+    }
+}
+__device__ __forceinline__ void pack_block(const Piece<Spike> (&v)[2], uint32_t, uint32_t (&w)[4]) {
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q) {
+        w[2 * q] = Piece<Spike>::four(v[q].raw.x) | Piece<Spike>::four(v[q].raw.y) << 16;
+        w[2 * q + 1] = Piece<Spike>::four(v[q].raw.z) | Piece<Spike>::four(v[q].raw.w) << 16;
+    }
 }
 
 }  // namespace mx4

@@ -23,5 +23,11 @@ struct Packed {
 cudaError_t matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,
                    void *out, int dtype, int64_t row_stride);
 
+// The same with up to 16 rows of plain x, packed by the product's own kernel,
+// where packs_on_the_way.
+bool packs_on_the_way(const void *x, int x_dtype, uint64_t m, int64_t row_stride, int64_t col_stride);
+cudaError_t linear(int device, cudaStream_t s, const void *x, int x_dtype, uint64_t m, int64_t x_stride, const Packed &w,
+                   uint64_t k, const float *bias, void *out, int dtype, int64_t row_stride);
+
 }  // namespace mx4
 }  // namespace b200

@@ -21,12 +21,14 @@
 //    a tile overlap the next one's instructions.
 //  * skinny: one tile a CTA and BN down to 16, the k of a tile split over the
 //    CTAs of a cluster, which add their parts through shared memory in the
-//    order of their ranks.
+//    order of their ranks. Up to 16 rows of x are packed on the way: four more
+//    warps write their codes and scales where the copies would have put them.
 // Every wait is bounded; one that gives up makes its tile NaN.
-#include "b200_mx4.h"
+#include "b200_mx4.cuh"
 #include "b200_tma.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200 {
 namespace mx4 {
@@ -116,6 +118,8 @@ struct Shape {
 };
 
 struct Problem {
+    const void *x;  // plain x, rows of x_stride elements
+    int64_t x_stride;
     const uint8_t *x_scales, *w_scales;
     uint32_t m, n, k, scale_tiles;  // scale tiles along k
     const float *bias;
@@ -124,17 +128,18 @@ struct Problem {
     uint32_t tiles_n, tiles_m, splits, stages;  // stages along k
 };
 
-// Loads stage `at` (of k) of a tile into slot memory.
-template <uint32_t BN>
+// Loads stage `at` (of k) of a tile into slot memory; Plain x is packed there by others.
+template <uint32_t BN, bool Plain = false>
 __device__ __forceinline__ void load_stage(const Problem &p, const CUtensorMap *wm, const CUtensorMap *xm,
                                            uint32_t slot, uint64_t *full, uint32_t at, uint32_t j0, uint32_t i0) {
     using S = Shape<BN>;
     const uint32_t tile = at * 2, bytes = kScaleTile * min(2u, p.scale_tiles - tile);
     const uint32_t row_tiles = min(S::kScaleRows, (p.m + 127) / 128 - i0 / 128);
-    bar_expect(full, S::kW + S::kX + bytes * (1 + row_tiles));
+    bar_expect(full, S::kW + bytes + (Plain ? 0 : S::kX + bytes * row_tiles));
     load_box(slot, wm, (int32_t)(at * kStageBytes), (int32_t)j0, full);
-    load_box(slot + S::kAtX, xm, (int32_t)(at * kStageBytes), (int32_t)i0, full);
     load_run(slot + S::kAtWScales, p.w_scales + ((uint64_t)(j0 / 128) * p.scale_tiles + tile) * kScaleTile, bytes, full);
+    if (Plain) return;
+    load_box(slot + S::kAtX, xm, (int32_t)(at * kStageBytes), (int32_t)i0, full);
     for (uint32_t r = 0; r < row_tiles; ++r)
         load_run(slot + S::kAtXScales + r * 2 * kScaleTile,
                  p.x_scales + ((uint64_t)(i0 / 128 + r) * p.scale_tiles + tile) * kScaleTile, bytes, full);
@@ -187,10 +192,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         bar_init(&s_free, 256);
         tma::bar_init_done();
     }
+    allow_next();
     if (warp == 0) tmem_alloc(&s_tmem, 512);
     fence_before();
     __syncthreads();
     fence_after();
+    after_previous();
     const uint32_t tmem = s_tmem, tiles = p.tiles_n * p.tiles_m;
     bool ok = true;
     if (warp == 0) {
@@ -268,6 +275,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 }
 
 // ---- skinny form ----
+constexpr uint32_t kMostSplits = 8;
 template <uint32_t BN>
 struct Skinny {
     static constexpr uint32_t kStages = BN >= 128 ? 3 : BN >= 64 ? 4 : 5;  // two CTAs an SM
@@ -285,17 +293,63 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float read_remote(uint32_t smem, uint32_t rank) {
+__device__ __forceinline__ float4 read_remote(uint32_t smem, uint32_t rank) {
     uint32_t at;
-    float v;
+    float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at)
+                 : "memory");
     return v;
 }
 
-template <typename T, uint32_t BN>
-__global__ void __launch_bounds__(128)
+// Packs a stage of plain x (rows of 16-byte pieces) into a slot: a lane a block of 32.
+template <typename X, uint32_t BN>
+__device__ __forceinline__ void pack_stage(const Problem &p, uint32_t slot, uint32_t at) {
+    using S = Shape<BN>;
+    constexpr uint32_t kPieces = kBlock / Piece<X>::kOwn, kRounds = BN * 8 / 32;
+    constexpr uint32_t kHeld = kPieces * kRounds <= 16 ? kRounds : 16 / kPieces;  // rounds whose loads are under way
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (uint32_t round = 0; round < kRounds; round += kHeld) {
+        Piece<X> v[kHeld][kPieces];
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h) {
+            const uint32_t n = (round + h) * 32 + lane, r = n / 8, c = at * kStageK + n % 8 * kBlock;
+#pragma unroll
+            for (uint32_t q = 0; q < kPieces; ++q) {
+                const uint32_t e = c + q * Piece<X>::kOwn;
+                v[h][q] = r < p.m && e < p.k ? load_piece<true>((const X *)p.x + r * p.x_stride + e, p.k - e) : Piece<X>{};
+            }
+        }
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h) {
+            const uint32_t n = (round + h) * 32 + lane, r = n / 8, b = n % 8;
+            if (r >= p.m) continue;
+            uint32_t top = 0, w[4];
+#pragma unroll
+            for (uint32_t q = 0; q < kPieces; ++q) top = max(top, v[h][q].largest());
+            const uint32_t s = scale_byte(top);
+            pack_block(v[h], s, w);
+            // Chunk b of the row, where the 128-byte swizzle puts it.
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot + S::kAtX + r * kStageBytes + ((b ^ r % 8) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+            asm volatile("st.shared.u8 [%0], %1;" ::"r"(slot + S::kAtXScales + b / 4 * kScaleTile + scale_slot(r, b % 4)),
+                         "r"(s)
+                         : "memory");
+        }
+    }
+}
+
+struct None {};  // x is packed already
+
+template <typename T, uint32_t BN, typename X>
+__global__ void __launch_bounds__(std::is_same<X, None>::value ? 128 : 256)
     skinny_kernel(const __grid_constant__ CUtensorMap wm, const __grid_constant__ CUtensorMap xm, Problem p) {
+    constexpr bool kPlain = !std::is_same<X, None>::value;
+    constexpr uint32_t kSkinnyWarps = kPlain ? 8 : 4;
     using S = Shape<BN>;
     using K = Skinny<BN>;
     extern __shared__ uint8_t s_raw[];
@@ -310,14 +364,16 @@ __global__ void __launch_bounds__(128)
     const uint32_t first = (uint32_t)((uint64_t)p.stages * rank / p.splits);
     const uint32_t count = (uint32_t)((uint64_t)p.stages * (rank + 1) / p.splits) - first;
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < K::kStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
+        for (uint32_t s = 0; s < K::kStages; ++s) bar_init(&s_full[s], kPlain ? 33 : 1), bar_init(&s_empty[s], 1);
         bar_init(&s_ready, 1);
         tma::bar_init_done();
     }
+    allow_next();
     if (warp == 0) tmem_alloc(&s_tmem, K::kColumns);
     fence_before();
     __syncthreads();
     fence_after();
+    after_previous();
     const uint32_t tmem = s_tmem;
     bool ok = true;
     if (warp == 0 && lane == 0) {
@@ -326,7 +382,7 @@ __global__ void __launch_bounds__(128)
             const uint32_t s = n % K::kStages, turn = n / K::kStages;
             ok = turn == 0 || bar_wait(&s_empty[s], (turn - 1) & 1);
             if (!ok) break;
-            load_stage<BN>(p, &wm, &xm, base + s * S::kStage, &s_full[s], first + n, j0, i0);
+            load_stage<BN, kPlain>(p, &wm, &xm, base + s * S::kStage, &s_full[s], first + n, j0, i0);
         }
         for (uint32_t d = 1; d <= K::kStages && d <= n; ++d)
             bar_wait(&s_full[(n - d) % K::kStages], ((n - d) / K::kStages) & 1);
@@ -341,16 +397,27 @@ __global__ void __launch_bounds__(128)
             commit(&s_empty[s]);
         }
         if (ok) commit(&s_ready);
+    } else if (kPlain && warp >= 4) {
+        // A stage a warp: the loads of four stages are under way at a time.
+        if constexpr (kPlain)
+            for (uint32_t n = warp - 4; ok && n < count; n += 4) {
+                const uint32_t s = n % K::kStages, turn = n / K::kStages;
+                ok = turn == 0 || bar_wait(&s_empty[s], (turn - 1) & 1);
+                if (!ok) break;
+                pack_stage<X, BN>(p, base + s * S::kStage, first + n);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(&s_full[s]);
+            }
     }
     __syncwarp();
     const uint32_t feature = warp * 32 + lane, j = j0 + feature;
-    const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
+    const float bias = warp < 4 && p.bias && j < p.n ? p.bias[j] : 0.0f;
     ok = bar_wait(&s_ready, 0);
     ok = __all_sync(0xffffffffu, ok);
     fence_after();
     // All instructions are done, so the stages' memory is free.
 #pragma unroll 1
-    for (uint32_t c = 0; c < BN; c += 16) {
+    for (uint32_t c = 0; warp < 4 && c < BN; c += 16) {
         float v[16];
         read_columns(tmem + (warp * 32 << 16) + c, v);
         read_done();
@@ -365,13 +432,25 @@ __global__ void __launch_bounds__(128)
         }
     }
     if (p.splits > 1) {
-        // Rank r adds up rows r, r + splits, ... of x.
+        // The ranks share the rows of x; a warp takes one at a time, a lane four features of it.
         cluster_sync();
-        for (uint32_t c = rank; c < BN && i0 + c < p.m; c += p.splits) {
-            float sum = 0.0f;
-            for (uint32_t r = 0; r < p.splits; ++r)
-                sum = __fadd_rn(sum, read_remote(base + (c * kRows + feature) * 4, r));
-            if (j < p.n) put<T>(p, i0 + c, j, __fadd_rn(sum, bias));
+        const uint32_t f = lane * 4;
+        for (uint32_t c = rank * kSkinnyWarps + warp; c < BN && i0 + c < p.m; c += p.splits * kSkinnyWarps) {
+            float4 part[kMostSplits];
+#pragma unroll
+            for (uint32_t r = 0; r < kMostSplits; ++r)
+                if (r < p.splits) part[r] = read_remote(base + (c * kRows + f) * 4, r);
+            float sum[4] = {};
+#pragma unroll
+            for (uint32_t r = 0; r < kMostSplits; ++r)
+                if (r < p.splits) {
+                    sum[0] = __fadd_rn(sum[0], part[r].x), sum[1] = __fadd_rn(sum[1], part[r].y);
+                    sum[2] = __fadd_rn(sum[2], part[r].z), sum[3] = __fadd_rn(sum[3], part[r].w);
+                }
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q)
+                if (j0 + f + q < p.n)
+                    put<T>(p, i0 + c, j0 + f + q, p.bias ? __fadd_rn(sum[q], p.bias[j0 + f + q]) : sum[q]);
         }
         cluster_sync();
     }
@@ -396,71 +475,102 @@ cudaError_t launch_wide(int device, cudaStream_t s, const CUtensorMap &wm, const
     const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
     if (e != cudaSuccess) return e;
     const uint32_t grid = std::min<uint64_t>((uint64_t)p.tiles_n * p.tiles_m, (uint64_t)sm_count(device));
-    wide_kernel<T><<<grid, kWideThreads, kWideSmem, s>>>(wm, xm, p);
-    return cudaGetLastError();
+    return launch_early(wide_kernel<T>, grid, kWideThreads, kWideSmem, s, 1, wm, xm, p);
 }
 
-template <typename T, uint32_t BN>
+template <typename T, uint32_t BN, typename X>
 cudaError_t launch_skinny(cudaStream_t s, const CUtensorMap &wm, const CUtensorMap &xm, const Problem &p) {
     using K = Skinny<BN>;
-    const cudaError_t e =
-        cudaFuncSetAttribute(skinny_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kSmem);
+    const auto kernel = skinny_kernel<T, BN, X>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kSmem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(p.tiles_n * p.tiles_m * p.splits);
-    c.blockDim = dim3(128);
-    c.dynamicSmemBytes = K::kSmem;
-    c.stream = s;
-    cudaLaunchAttribute cluster = {};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = p.splits;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    c.attrs = &cluster;
-    c.numAttrs = p.splits > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&c, skinny_kernel<T, BN>, wm, xm, p);
+    const uint32_t threads = std::is_same<X, None>::value ? 128 : 256;
+    return launch_early(kernel, p.tiles_n * p.tiles_m * p.splits, threads, K::kSmem, s, p.splits, wm, xm, p);
+}
+
+Problem problem_of(uint64_t m, const Packed &w, uint64_t k, const float *bias, void *out, int64_t row_stride) {
+    Problem p = {};
+    p.w_scales = w.scales;
+    p.m = (uint32_t)m, p.n = (uint32_t)w.rows, p.k = (uint32_t)k;
+    p.scale_tiles = (uint32_t)scale_tiles(k);
+    p.bias = bias, p.out = out, p.row_stride = row_stride;
+    p.stages = (uint32_t)((k + kStageK - 1) / kStageK);
+    p.tiles_n = (uint32_t)((w.rows + kRows - 1) / kRows);
+    return p;
+}
+// As many parts of k (of two stages at least) as two CTAs an SM hold at once.
+void split_k(int device, Problem &p) {
+    const uint64_t tiles = (uint64_t)p.tiles_n * p.tiles_m, most = (uint64_t)sm_count(device) * 2;
+    p.splits = 1;
+    while (p.splits < kMostSplits && tiles * p.splits * 2 <= most && p.stages >= p.splits * 4) p.splits *= 2;
 }
 
 template <typename T>
 cudaError_t run(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, Problem &p) {
     const uint64_t sms = (uint64_t)sm_count(device);
-    p.tiles_n = (uint32_t)((w.rows + kRows - 1) / kRows);
     const uint64_t wide_tiles = p.tiles_n * ((x.rows + kWideN - 1) / kWideN);
+    p.x_scales = x.scales;
     CUtensorMap wm, xm;
     cudaError_t e = map_of(&wm, w, k, kRows);
     if (e != cudaSuccess) return e;
     // Wide tiles where they fill the SMs, else narrower ones with k split.
     if (x.rows > 128 && wide_tiles * 4 >= sms * 3) {
         p.tiles_m = (uint32_t)((x.rows + kWideN - 1) / kWideN);
-        p.splits = 1;
         e = map_of(&xm, x, k, kWideN);
         return e != cudaSuccess ? e : launch_wide<T>(device, s, wm, xm, p);
     }
     const uint32_t bn = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : x.rows <= 64 ? 64 : 128;
     p.tiles_m = (uint32_t)((x.rows + bn - 1) / bn);
-    // As many parts of k (of two stages at least) as two CTAs an SM hold at once.
-    uint32_t splits = 1;
-    while (splits < 8 && (uint64_t)p.tiles_n * p.tiles_m * splits * 2 <= sms * 2 && p.stages >= splits * 4) splits *= 2;
-    p.splits = splits;
+    split_k(device, p);
     e = map_of(&xm, x, k, bn);
     if (e != cudaSuccess) return e;
     switch (bn) {
-        case 16: return launch_skinny<T, 16>(s, wm, xm, p);
-        case 32: return launch_skinny<T, 32>(s, wm, xm, p);
-        case 64: return launch_skinny<T, 64>(s, wm, xm, p);
-        default: return launch_skinny<T, 128>(s, wm, xm, p);
+        case 16: return launch_skinny<T, 16, None>(s, wm, xm, p);
+        case 32: return launch_skinny<T, 32, None>(s, wm, xm, p);
+        case 64: return launch_skinny<T, 64, None>(s, wm, xm, p);
+        default: return launch_skinny<T, 128, None>(s, wm, xm, p);
+    }
+}
+
+template <typename T, typename X>
+cudaError_t run_plain(int device, cudaStream_t s, const Packed &w, uint64_t k, Problem &p) {
+    CUtensorMap wm;
+    const cudaError_t e = map_of(&wm, w, k, kRows);
+    if (e != cudaSuccess) return e;
+    p.tiles_m = 1;
+    split_k(device, p);
+    return launch_skinny<T, 16, X>(s, wm, wm, p);
+}
+template <typename T>
+cudaError_t run_plain_as(int device, cudaStream_t s, int x_dtype, const Packed &w, uint64_t k, Problem &p) {
+    switch (x_dtype) {
+        case SNN_B200_F32: return run_plain<T, float>(device, s, w, k, p);
+        case SNN_B200_F16: return run_plain<T, __half>(device, s, w, k, p);
+        case SNN_B200_BF16: return run_plain<T, __nv_bfloat16>(device, s, w, k, p);
+        default: return run_plain<T, Spike>(device, s, w, k, p);
     }
 }
 
 }  // namespace
 
+bool packs_on_the_way(const void *x, int x_dtype, uint64_t m, int64_t row_stride, int64_t col_stride) {
+    return m <= 16 && col_stride == 1 && aligned_to(x, 16) && row_stride * dtype_bytes(x_dtype) % 16 == 0;
+}
+
+cudaError_t linear(int device, cudaStream_t s, const void *x, int x_dtype, uint64_t m, int64_t x_stride, const Packed &w,
+                   uint64_t k, const float *bias, void *out, int dtype, int64_t row_stride) {
+    Problem p = problem_of(m, w, k, bias, out, row_stride);
+    p.x = x, p.x_stride = x_stride;
+    switch (dtype) {
+        case SNN_B200_F32: return run_plain_as<float>(device, s, x_dtype, w, k, p);
+        case SNN_B200_F16: return run_plain_as<__half>(device, s, x_dtype, w, k, p);
+        default: return run_plain_as<__nv_bfloat16>(device, s, x_dtype, w, k, p);
+    }
+}
+
 cudaError_t matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,
                    void *out, int dtype, int64_t row_stride) {
-    Problem p = {};
-    p.x_scales = x.scales, p.w_scales = w.scales;
-    p.m = (uint32_t)x.rows, p.n = (uint32_t)w.rows, p.k = (uint32_t)k;
-    p.scale_tiles = (uint32_t)scale_tiles(k);
-    p.bias = bias, p.out = out, p.row_stride = row_stride;
-    p.stages = (uint32_t)((k + kStageK - 1) / kStageK);
+    Problem p = problem_of(x.rows, w, k, bias, out, row_stride);
     switch (dtype) {
         case SNN_B200_F32: return run<float>(device, s, x, w, k, p);
         case SNN_B200_F16: return run<__half>(device, s, x, w, k, p);

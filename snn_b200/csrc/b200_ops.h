@@ -62,6 +62,27 @@ inline bool disjoint_runs(snn_size_t na, int64_t sa, snn_size_t nb, int64_t sb, 
     return inner >= run && (unsigned __int128)(n - 1) * inner + run <= outer;
 }
 
+// Launches that may start while the kernel before them in the stream ends: their
+// set-up overlaps its last CTAs. Every kernel launched so calls after_previous()
+// before it reads or writes global memory, which waits for all of that kernel,
+// and allow_next() early, so that its own successor may do the same.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, uint32_t cluster,
+                         A &&...args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = smem, c.stream = stream;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 // Element types: a spike byte counts as one when it is not zero.
 struct Spike {
     uint8_t byte;

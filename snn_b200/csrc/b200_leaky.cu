@@ -22,7 +22,6 @@ __global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *m
     const uint32_t run = (segments + kCarryWarps - 1) / kCarryWarps;
     const uint32_t from = min(segments, warp * run), to = min(segments, from + run);
     const auto at = [&](uint32_t n) { return (uint64_t)(back ? segments - 1 - n : n) * flat + i; };
-    allow_next();
     after_previous();
     float2 m = make_float2(1.0f, 0.0f);
     if (i < flat)
@@ -56,7 +55,6 @@ __global__ void __launch_bounds__(kSumWarps * 32) gate_sum_kernel(const float *p
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint32_t c = blockIdx.x * 32 + lane;
     const uint64_t flat = (uint64_t)batch * channels;
-    allow_next();
     after_previous();
     for (uint32_t r = blockIdx.y; r < (row_stride ? batch : 1u); r += gridDim.y) {
         const uint64_t terms = row_stride ? segments : (uint64_t)segments * batch;

@@ -398,7 +398,6 @@ template <typename X, typename G, typename Y, int V, bool Maps>
 __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
     const Part w = part_of(g, Maps);
-    allow_next();
     after_previous();
     if (!w.on) return;
     const Place p = place_of<V>(g, w.column);  // lanes behind the last channel only help to copy
@@ -545,7 +544,6 @@ template <typename X, typename G, typename Y, int V, bool Maps>
 __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
     const Part w = part_of(g, Maps);
-    allow_next();
     after_previous();
     if (!w.on) return;
     const Place p = place_of<V>(g, w.column);  // lanes behind the last channel only help to copy
@@ -624,7 +622,6 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
     __shared__ uint32_t s_before[8], s_after[8];  // rows named before, rows named again
     const uint32_t across = 256 / g.rows, mine = threadIdx.x / across;
     const uint32_t row = blockIdx.x * g.rows + mine;
-    allow_next();
     after_previous();
     if (g.slots && g.batch > 1) {
         if (threadIdx.x < 8) s_before[threadIdx.x] = s_after[threadIdx.x] = 0u;

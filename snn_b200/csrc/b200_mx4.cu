@@ -29,7 +29,6 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, ui
     const uint32_t tile = blockIdx.x, r0 = blockIdx.y * kTileRows;
     const uint32_t part = threadIdx.x % kAcross, first = threadIdx.x / kAcross, c = tile * kTileCols + part * kOwn;
     const uint64_t pitch = blocks_of(cols) * 16;
-    allow_next();
     after_previous();
 #pragma unroll 1
     for (uint32_t pass = 0; pass < kPasses; pass += kHeld) {
@@ -67,7 +66,6 @@ __global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uin
     const uint32_t tile = blockIdx.x, at = threadIdx.x % kTileRows, b = threadIdx.x / kTileRows;
     const uint64_t r = (uint64_t)blockIdx.y * kTileRows + at, c = (uint64_t)tile * kTileCols + b * kBlock;
     uint32_t s = 0;
-    allow_next();
     after_previous();
     if (r < rows && c < cols) {
         const T *p = src + (int64_t)r * rs + (int64_t)c * cs;
@@ -100,7 +98,6 @@ __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t *code
                                                              bool pieces) {
     const uint64_t pitch = blocks_of(cols) * 16;
     const uint32_t c = (blockIdx.x * 64 + threadIdx.x % 64) * 8;
-    allow_next();
     after_previous();
     if (c >= cols) return;
     const uint32_t b = c / kBlock;

@@ -16,9 +16,9 @@
 //
 // One warp issues the loads, one the instructions; the others read the
 // accumulators and write. Two forms share this:
-//  * wide: BN = 256, a CTA an SM, tiles in turn; the accumulators are moved to
-//    registers and given back before they are written, so that the writes of
-//    a tile overlap the next one's instructions.
+//  * pairs: two CTAs on two SMs share 256 x 256 tiles, one after another; the
+//    accumulators are moved to registers and given back before they are
+//    written, so that the writes of a tile overlap the next one's instructions.
 //  * skinny: one tile a CTA and BN down to 16, the k of a tile split over the
 //    CTAs of a cluster, which add their parts through shared memory in the
 //    order of their ranks. Up to 16 rows of x are packed on the way: four more
@@ -62,30 +62,78 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_of(bar))
                  : "memory");
 }
-// Rows of 128 bytes in 8-row groups of 1024, swizzled by 128 bytes.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t smem) {
-    return (uint64_t)((smem & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
-           (uint64_t)2 << 61;
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t on;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(on));
+    return on != 0;
 }
+// Descriptors of shared memory, of which only the low word changes: operands
+// are rows of 128 bytes in 8-row groups of 1024, swizzled by 128 bytes; scales
 // 32 rows of 16 bytes, one behind the other.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
-    return (uint64_t)((smem & 0x3ffffu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29, kScaleHigh = 128 >> 4 | 1u << 14;
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem) { return (smem & 0x3ffffu) >> 4 | 1u << 16; }
+
+template <bool Pair>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t low) {
+    if constexpr (Pair)
+        asm volatile("{\n .reg .b64 d;\n mov.b64 d, {%1, %2};\n tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n}" ::"r"(tmem),
+                     "r"(low), "n"(kScaleHigh)
+                     : "memory");
+    else
+        asm volatile("{\n .reg .b64 d;\n mov.b64 d, {%1, %2};\n tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n}" ::"r"(tmem),
+                     "r"(low), "n"(kScaleHigh)
+                     : "memory");
 }
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t smem) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_desc(smem)) : "memory");
-}
-// Both operands e2m1, K-major; scales ue8m0; 128 x n. The scale bytes of 64 of
+// Both operands e2m1, K-major; scales ue8m0; m x n. The scale bytes of 64 of
 // k are the low or the high half of a scale column's word.
-__device__ __forceinline__ uint32_t instruction(uint32_t n, uint32_t half) {
-    return (half * 2u) << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (kRows >> 7) << 27 | (half * 2u) << 29;
+constexpr uint32_t instruction(uint32_t m, uint32_t n, uint32_t half) {
+    return (half * 2u) << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (m >> 7) << 27 | (half * 2u) << 29;
 }
-__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
-                                         bool add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"((uint32_t)add)
-        : "memory");
+template <bool Pair>
+__device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                         uint32_t add) {
+    if constexpr (Pair)
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %6, 0;\n mov.b64 a, {%1, %7};\n mov.b64 b, {%2, %7};\n"
+            " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(add), "n"(kOperandHigh)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %6, 0;\n mov.b64 a, {%1, %7};\n mov.b64 b, {%2, %7};\n"
+            " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], a, b, %3, [%4], [%5], p;\n}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(add), "n"(kOperandHigh)
+            : "memory");
+}
+// A loaded stage's instructions, by one thread: weights at w, BN rows of x at x
+// (of which this CTA may hold half), their scales at ws and xs; d the accumulators,
+// sf the stage's tensor memory columns for scales; pieces of 64 of k. What changes
+// from stage to stage is few additions, as the issuing thread has to keep ahead.
+template <bool Pair, uint32_t BN>
+__device__ __forceinline__ void issue_stage(uint32_t w, uint32_t x, uint32_t ws, uint32_t xs, uint32_t d, uint32_t sf,
+                                            uint32_t pieces, uint32_t add) {
+    constexpr uint32_t kM = Pair ? 256 : 128, kR = (BN + 127) / 128;
+    const uint32_t a = desc_low(w), b = desc_low(x), cs = desc_low(ws), cx = desc_low(xs);
+#pragma unroll
+    for (uint32_t t = 0; t < 2; ++t) {
+        copy_scales<Pair>(sf + 4 * t, cs + t * (512 >> 4));
+#pragma unroll
+        for (uint32_t r = 0; r < kR; ++r)
+            copy_scales<Pair>(sf + 8 + 4 * (t * kR + r), cx + (r * 2 + t) * (512 >> 4));
+    }
+    if (pieces == 4) {
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q)
+            multiply<Pair>(d, a + q * 2, b + q * 2, instruction(kM, BN, q & 1), sf + 4 * (q / 2), sf + 8 + 4 * kR * (q / 2),
+                           q ? 1u : add);
+    } else {
+#pragma unroll
+        for (uint32_t q = 0; q < 3; ++q)
+            if (q < pieces)
+                multiply<Pair>(d, a + q * 2, b + q * 2, instruction(kM, BN, q & 1), sf + 4 * (q / 2),
+                               sf + 8 + 4 * kR * (q / 2), q ? 1u : add);
+    }
 }
 // 16 accumulator columns of the warp's 32 lanes.
 __device__ __forceinline__ void read_columns(uint32_t at, float (&v)[16]) {
@@ -105,6 +153,14 @@ __device__ __forceinline__ void settle(float (&v)[16]) {
     for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[i]));
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
 // ---- a tile's k loop ----
 template <uint32_t BN>
 struct Shape {
@@ -145,27 +201,6 @@ __device__ __forceinline__ void load_stage(const Problem &p, const CUtensorMap *
                  p.x_scales + ((uint64_t)(i0 / 128 + r) * p.scale_tiles + tile) * kScaleTile, bytes, full);
 }
 
-// Issues a loaded stage's instructions. sf: tensor memory columns of its scales.
-template <uint32_t BN>
-__device__ __forceinline__ void multiply_stage(const Problem &p, uint32_t slot, uint32_t at, uint32_t d, uint32_t sf,
-                                               bool &add) {
-    using S = Shape<BN>;
-    const uint32_t pieces = min(kStageK / 64, (p.k - at * kStageK + 63) / 64);
-#pragma unroll
-    for (uint32_t t = 0; t < 2; ++t) {
-        copy_scales(sf + 4 * t, slot + S::kAtWScales + t * kScaleTile);
-#pragma unroll
-        for (uint32_t r = 0; r < S::kScaleRows; ++r)
-            copy_scales(sf + 8 + 4 * (t * S::kScaleRows + r), slot + S::kAtXScales + (r * 2 + t) * kScaleTile);
-    }
-    const uint64_t a = operand_desc(slot), b = operand_desc(slot + S::kAtX);
-    for (uint32_t q = 0; q < pieces; ++q) {
-        multiply(d, a + q * 2, b + q * 2, instruction(BN, q & 1), sf + 4 * (q / 2), sf + 8 + 4 * S::kScaleRows * (q / 2),
-                 add);
-        add = true;
-    }
-}
-
 template <typename T>
 __device__ __forceinline__ void put(const Problem &p, uint32_t i, uint32_t j, float v) {
     ((T *)p.out)[(int64_t)i * p.row_stride + j] = from_float<T>(v);
@@ -174,93 +209,151 @@ __device__ __forceinline__ void put(const Problem &p, uint32_t i, uint32_t j, fl
 constexpr uint32_t kNoValue = 0x7fffffffu;
 
 // ---- wide form ----
-constexpr uint32_t kWideN = 256, kWideStages = 4, kWideThreads = 384;
-constexpr uint32_t kWideSmem = 1024 + kWideStages * Shape<kWideN>::kStage;
+// A pair of CTAs (cta_group::2) works on 256 weight rows and 256 rows of x: each
+// CTA holds 128 of both in shared memory and the accumulators of its weight
+// rows, and the instructions read x from both. What a CTA loads for a tile is
+// the bound (about 11 TB/s come out of L2 for all SMs; 256 rows of x a CTA took
+// 309 us at 8192x8192x8192), and this halves x's part of it.
+constexpr uint32_t kPairN = 256, kPairStages = 6, kPairThreads = 384;
+constexpr uint32_t kPairX = 128 * kStageBytes, kPairW = kRows * kStageBytes;
+// A stage: weights, x, the scales of the CTA's weights, of all of x's rows.
+constexpr uint32_t kPairAtX = kPairW, kPairAtWScales = kPairW + kPairX, kPairAtXScales = kPairAtWScales + 2 * kScaleTile;
+constexpr uint32_t kPairStage = kPairAtXScales + 4 * kScaleTile;
+constexpr uint32_t kPairSmem = 1024 + kPairStages * kPairStage;
+constexpr uint32_t kPairColumns = 24;  // tensor memory columns of a stage's scales
+static_assert(kPairN + kPairStages * kPairColumns <= 512, "tensor memory");
 
+struct PairMaps {
+    CUtensorMap w, x, w_scales, x_scales;
+};
+
+// An address of this CTA's shared memory, in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
+    return at;
+}
+// Into this CTA's memory, counted by a barrier of either CTA of the pair.
+__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_of(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
 template <typename T>
-__global__ void __launch_bounds__(kWideThreads, 1)
-    wide_kernel(const __grid_constant__ CUtensorMap wm, const __grid_constant__ CUtensorMap xm, Problem p) {
-    using S = Shape<kWideN>;
+__global__ void __launch_bounds__(kPairThreads, 1)
+    pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ Problem p) {
     extern __shared__ uint8_t s_raw[];
-    __shared__ uint64_t s_full[kWideStages], s_empty[kWideStages], s_ready, s_free;
+    __shared__ uint64_t s_full[kPairStages], s_empty[kPairStages], s_ready, s_free;
     __shared__ uint32_t s_tmem;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_of(s_raw) + 1023) & ~1023u;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x & 31, rank = cluster_rank();
+    const uint32_t base = (smem_of(s_raw) + 1023) & ~1023u;  // the same in both CTAs
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < kWideStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
+        for (uint32_t s = 0; s < kPairStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
         bar_init(&s_ready, 1);
-        bar_init(&s_free, 256);
+        bar_init(&s_free, 16);  // the warps that read accumulators, of both CTAs
         tma::bar_init_done();
     }
-    allow_next();
-    if (warp == 0) tmem_alloc(&s_tmem, 512);
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
     fence_before();
     __syncthreads();
+    cluster_sync();
     fence_after();
     after_previous();
-    const uint32_t tmem = s_tmem, tiles = p.tiles_n * p.tiles_m;
+    const uint32_t tmem = s_tmem, tiles = p.tiles_n * p.tiles_m, pairs = gridDim.x / 2, pair = blockIdx.x / 2;
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
             uint32_t n = 0;  // stages so far
-            for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-                const uint32_t j0 = tile % p.tiles_n * kRows, i0 = tile / p.tiles_n * kWideN;
-                for (uint32_t at = 0; ok && at < p.stages; ++at, ++n) {
-                    const uint32_t s = n % kWideStages, turn = n / kWideStages;
+            for (uint32_t tile = pair; ok && tile < tiles; tile += pairs) {
+                const uint32_t j0 = tile % p.tiles_n * 256 + rank * 128, i0 = tile / p.tiles_n * kPairN;
+                for (uint32_t at = 0; at < p.stages; ++at, ++n) {
+                    const uint32_t s = n % kPairStages, turn = n / kPairStages, slot = base + s * kPairStage;
                     ok = turn == 0 || bar_wait(&s_empty[s], (turn - 1) & 1);
-                    if (ok) load_stage<kWideN>(p, &wm, &xm, base + s * S::kStage, &s_full[s], at, j0, i0);
-                    else --n;
+                    if (!ok) break;
+                    // Both CTAs' bytes are counted by the first one's barrier.
+                    if (rank == 0) bar_expect(&s_full[s], 2 * kPairStage);
+                    const uint32_t full = in_cta(smem_of(&s_full[s]), 0);
+                    load_pair(slot, &maps.w, at * kStageBytes, j0, full);
+                    load_pair(slot + kPairAtX, &maps.x, at * kStageBytes, i0 + rank * 128, full);
+                    load_pair(slot + kPairAtWScales, &maps.w_scales, at * 256, j0 / 128, full);
+                    load_pair(slot + kPairAtXScales, &maps.x_scales, at * 256, i0 / 128, full);
                 }
             }
-            // Let the last copies land before the CTA may end.
-            for (uint32_t d = 1; d <= kWideStages && d <= n; ++d)
-                bar_wait(&s_full[(n - d) % kWideStages], ((n - d) / kWideStages) & 1);
+            // Let the last copies land before the CTAs may end.
+            if (rank == 0)
+                for (uint32_t d = 1; d <= kPairStages && d <= n; ++d)
+                    bar_wait(&s_full[(n - d) % kPairStages], ((n - d) / kPairStages) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t n = 0, count = 0;
-            for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++count) {
+        // The whole warp keeps the count, so that what it issues lies in uniform registers.
+        if (rank == 0) {
+            const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
+            uint32_t n = 0, count = 0, s = 0, parity = 0;
+            for (uint32_t tile = pair; ok && tile < tiles; tile += pairs, ++count) {
                 ok = count == 0 || bar_wait(&s_free, (count - 1) & 1);
                 fence_after();
-                bool add = false;
                 for (uint32_t at = 0; ok && at < p.stages; ++at, ++n) {
-                    const uint32_t s = n % kWideStages;
-                    ok = bar_wait(&s_full[s], (n / kWideStages) & 1);
+                    ok = __all_sync(0xffffffffu, bar_wait(&s_full[s], parity));
                     fence_after();
                     if (!ok) break;
-                    multiply_stage<kWideN>(p, base + s * S::kStage, at, tmem, tmem + kWideN + s * S::kScaleColumns, add);
-                    commit(&s_empty[s]);
+                    const uint32_t slot = base + s * kPairStage;
+                    if (elect()) {
+                        issue_stage<true, kPairN>(slot, slot + kPairAtX, slot + kPairAtWScales, slot + kPairAtXScales, acc,
+                                                  acc + kPairN + s * kPairColumns,
+                                                  min(kStageK / 64, (p.k - at * kStageK + 63) / 64), at);
+                        commit_pair(&s_empty[s]);
+                    }
+                    __syncwarp();
+                    if (++s == kPairStages) s = 0, parity ^= 1;
                 }
-                if (ok) commit(&s_ready);
+                if (ok && elect()) commit_pair(&s_ready);
+                __syncwarp();
             }
         }
     } else if (warp >= 4) {
         // Four warps share the lanes, two share the columns.
         const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+        const uint32_t free = in_cta(smem_of(&s_free), 0);
         uint32_t count = 0;
-        for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++count) {
-            const uint32_t j0 = tile % p.tiles_n * kRows, i0 = tile / p.tiles_n * kWideN;
-            const uint32_t j = j0 + quarter * 32 + lane;
+        for (uint32_t tile = pair; tile < tiles; tile += pairs, ++count) {
+            const uint32_t j = tile % p.tiles_n * 256 + rank * 128 + quarter * 32 + lane;
+            const uint32_t i0 = tile / p.tiles_n * kPairN + half * (kPairN / 2);
             const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
             ok = ok && bar_wait(&s_ready, count & 1);
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            float v[kWideN / 2 / 16][16];
+            float v[kPairN / 2 / 16][16];
 #pragma unroll
-            for (uint32_t c = 0; c < kWideN / 2 / 16; ++c)
-                read_columns(tmem + (quarter * 32 << 16) + half * (kWideN / 2) + c * 16, v[c]);
+            for (uint32_t c = 0; c < kPairN / 2 / 16; ++c)
+                read_columns(tmem + (quarter * 32 << 16) + half * (kPairN / 2) + c * 16, v[c]);
             read_done();
 #pragma unroll
-            for (uint32_t c = 0; c < kWideN / 2 / 16; ++c) settle(v[c]);
+            for (uint32_t c = 0; c < kPairN / 2 / 16; ++c) settle(v[c]);
             fence_before();
-            bar_arrive(&s_free);
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free) : "memory");
             if (j < p.n) {
+                T *to = (T *)p.out + (int64_t)i0 * p.row_stride + j;
+                const uint32_t rows = i0 < p.m ? min(p.m - i0, kPairN / 2) : 0;
 #pragma unroll
-                for (uint32_t c = 0; c < kWideN / 2 / 16; ++c)
+                for (uint32_t c = 0; c < kPairN / 2 / 16; ++c)
 #pragma unroll
                     for (uint32_t q = 0; q < 16; ++q) {
-                        const uint32_t i = i0 + half * (kWideN / 2) + c * 16 + q;
-                        if (i < p.m) put<T>(p, i, j, ok ? __fadd_rn(v[c][q], bias) : __uint_as_float(kNoValue));
+                        if (c * 16 + q < rows)
+                            *to = from_float<T>(ok ? __fadd_rn(v[c][q], bias) : __uint_as_float(kNoValue));
+                        to += p.row_stride;
                     }
             }
         }
@@ -268,9 +361,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     __syncwarp();
     fence_before();
     __syncthreads();
+    cluster_sync();  // neither CTA's memory is used any more
     if (warp == 0) {
         fence_after();
-        tmem_free(tmem, 512);
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
 }
 
@@ -285,18 +379,9 @@ struct Skinny {
     static_assert(BN * kRows * 4 <= kStages * Shape<BN>::kStage, "the parts lie where the stages were");
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float4 read_remote(uint32_t smem, uint32_t rank) {
-    uint32_t at;
+    const uint32_t at = in_cta(smem, rank);
     float4 v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem), "r"(rank));
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                  : "r"(at)
@@ -355,7 +440,7 @@ __global__ void __launch_bounds__(std::is_same<X, None>::value ? 128 : 256)
     extern __shared__ uint8_t s_raw[];
     __shared__ uint64_t s_full[K::kStages], s_empty[K::kStages], s_ready;
     __shared__ uint32_t s_tmem;
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
     const uint32_t base = (smem_of(s_raw) + 1023) & ~1023u;
     const uint32_t rank = p.splits > 1 ? cluster_rank() : 0;
     const uint32_t tile = blockIdx.x / p.splits;
@@ -368,11 +453,13 @@ __global__ void __launch_bounds__(std::is_same<X, None>::value ? 128 : 256)
         bar_init(&s_ready, 1);
         tma::bar_init_done();
     }
-    allow_next();
     if (warp == 0) tmem_alloc(&s_tmem, K::kColumns);
     fence_before();
     __syncthreads();
     fence_after();
+    // Only now that this CTA has its tensor memory: one of the next kernel's, which
+    // ends after it, could hold what it waits for.
+    allow_next();
     after_previous();
     const uint32_t tmem = s_tmem;
     bool ok = true;
@@ -386,17 +473,23 @@ __global__ void __launch_bounds__(std::is_same<X, None>::value ? 128 : 256)
         }
         for (uint32_t d = 1; d <= K::kStages && d <= n; ++d)
             bar_wait(&s_full[(n - d) % K::kStages], ((n - d) / K::kStages) & 1);
-    } else if (warp == 1 && lane == 0) {
-        bool add = false;
+    } else if (warp == 1) {
+        const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
         for (uint32_t n = 0; ok && n < count; ++n) {
             const uint32_t s = n % K::kStages;
-            ok = bar_wait(&s_full[s], (n / K::kStages) & 1);
+            ok = __all_sync(0xffffffffu, bar_wait(&s_full[s], (n / K::kStages) & 1));
             fence_after();
             if (!ok) break;
-            multiply_stage<BN>(p, base + s * S::kStage, first + n, tmem, tmem + BN + s * S::kScaleColumns, add);
-            commit(&s_empty[s]);
+            const uint32_t slot = base + s * S::kStage;
+            if (elect()) {
+                issue_stage<false, BN>(slot, slot + S::kAtX, slot + S::kAtWScales, slot + S::kAtXScales, acc,
+                                       acc + BN + s * S::kScaleColumns,
+                                       min(kStageK / 64, (p.k - (first + n) * kStageK + 63) / 64), n);
+                commit(&s_empty[s]);
+            }
+            __syncwarp();
         }
-        if (ok) commit(&s_ready);
+        if (ok && elect()) commit(&s_ready);
     } else if (kPlain && warp >= 4) {
         // A stage a warp: the loads of four stages are under way at a time.
         if constexpr (kPlain)
@@ -470,12 +563,24 @@ cudaError_t map_of(CUtensorMap *map, const Packed &q, uint64_t k, uint32_t box) 
     return tma::encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, q.codes, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// The scales of a packed matrix as rows of 512-byte tiles, two of them wide and `high` rows high.
+cudaError_t scale_map_of(CUtensorMap *map, const Packed &q, uint64_t k, uint32_t high) {
+    const cuuint64_t dims[2] = {scale_tiles(k) * 128, (q.rows + 127) / 128}, strides[1] = {scale_tiles(k) * 512};
+    const cuuint32_t boxes[2] = {256, high};
+    return tma::encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, q.scales, dims, strides, boxes, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <typename T>
-cudaError_t launch_wide(int device, cudaStream_t s, const CUtensorMap &wm, const CUtensorMap &xm, const Problem &p) {
-    const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+cudaError_t launch_pairs(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const Problem &p) {
+    PairMaps m;
+    cudaError_t e = map_of(&m.w, w, k, 128);
+    if (e == cudaSuccess) e = map_of(&m.x, x, k, 128);
+    if (e == cudaSuccess) e = scale_map_of(&m.w_scales, w, k, 1);
+    if (e == cudaSuccess) e = scale_map_of(&m.x_scales, x, k, 2);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
     if (e != cudaSuccess) return e;
-    const uint32_t grid = std::min<uint64_t>((uint64_t)p.tiles_n * p.tiles_m, (uint64_t)sm_count(device));
-    return launch_early(wide_kernel<T>, grid, kWideThreads, kWideSmem, s, 1, wm, xm, p);
+    const uint64_t tiles = (uint64_t)p.tiles_n * p.tiles_m, most = (uint64_t)sm_count(device) / 2;
+    return launch_early(pair_kernel<T>, 2 * (uint32_t)std::min(tiles, most), kPairThreads, kPairSmem, s, 2, m, p);
 }
 
 template <typename T, uint32_t BN, typename X>
@@ -507,18 +612,16 @@ void split_k(int device, Problem &p) {
 
 template <typename T>
 cudaError_t run(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, Problem &p) {
-    const uint64_t sms = (uint64_t)sm_count(device);
-    const uint64_t wide_tiles = p.tiles_n * ((x.rows + kWideN - 1) / kWideN);
     p.x_scales = x.scales;
+    // Pairs of CTAs where their tiles fill the SMs, else narrower tiles with k split.
+    const uint64_t across = (w.rows + 255) / 256, high = (x.rows + kPairN - 1) / kPairN;
+    if (x.rows > 128 && w.rows > 128 && across * high * 8 >= (uint64_t)sm_count(device) * 3) {
+        p.tiles_n = (uint32_t)across, p.tiles_m = (uint32_t)high, p.splits = 1;
+        return launch_pairs<T>(device, s, x, w, k, p);
+    }
     CUtensorMap wm, xm;
     cudaError_t e = map_of(&wm, w, k, kRows);
     if (e != cudaSuccess) return e;
-    // Wide tiles where they fill the SMs, else narrower ones with k split.
-    if (x.rows > 128 && wide_tiles * 4 >= sms * 3) {
-        p.tiles_m = (uint32_t)((x.rows + kWideN - 1) / kWideN);
-        e = map_of(&xm, x, k, kWideN);
-        return e != cudaSuccess ? e : launch_wide<T>(device, s, wm, xm, p);
-    }
     const uint32_t bn = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : x.rows <= 64 ? 64 : 128;
     p.tiles_m = (uint32_t)((x.rows + bn - 1) / bn);
     split_k(device, p);

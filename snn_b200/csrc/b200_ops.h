@@ -64,8 +64,10 @@ inline bool disjoint_runs(snn_size_t na, int64_t sa, snn_size_t nb, int64_t sb, 
 
 // Launches that may start while the kernel before them in the stream ends: their
 // set-up overlaps its last CTAs. Every kernel launched so calls after_previous()
-// before it reads or writes global memory, which waits for all of that kernel,
-// and allow_next() early, so that its own successor may do the same.
+// before it reads or writes global memory, which waits for all of that kernel.
+// allow_next() lets its own successor start before its CTAs have ended; only the
+// skinny product, a single wave of CTAs, gains by it (4x8192x8192: 10.4 against
+// 11.2 us; a step of 2000 rows lost by it: 11.6 against 8.1 us).
 template <typename... P, typename... A>
 cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, uint32_t cluster,
                          A &&...args) {

@@ -29,11 +29,13 @@ __device__ __forceinline__ void bar_expect(uint64_t *b, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint64_t *b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_of(b)) : "memory");
 }
-// Waits for the phase of that parity to end; false when it gave up.
+// Waits for the phase of that parity to end; false when it gave up, after about
+// two seconds of the SM's clock.
 __device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
-    constexpr uint32_t kPolls = 1u << 24;
+    constexpr long long kMostCycles = 1ll << 32;
     const uint32_t at = smem_of(b);
-    for (uint32_t i = 0; i < kPolls; ++i) {
+    const long long start = clock64();
+    do {
         uint32_t done;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
@@ -41,7 +43,7 @@ __device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
             : "r"(at), "r"(parity)
             : "memory");
         if (done) return true;
-    }
+    } while (clock64() - start < kMostCycles);
     return false;
 }
 
@@ -49,14 +51,6 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, i
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
             "r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_of(bar))
-        : "memory");
-}
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
-                                         uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_of(bar))
         : "memory");
 }
 // Both addresses and the size are multiples of 16.

@@ -110,12 +110,14 @@ snn_status_t check_common(int device, const snn_b200_leaky_t *q, const void *x, 
 // How a call is cut and where its parts lie in the workspace.
 struct Plan {
     uint64_t flat, columns;
-    uint32_t segments, segment_steps;
+    uint32_t segments, segment_steps, partials;  // partials: sums of a shared gate's gradient a channel
+    bool crew;
     uint64_t maps, states, partial, bytes;
 };
-// Walks of whole sequences, or segments of them (64 steps at least) where
-// those would be too few to keep the loads of 148 SMs under way.
-constexpr uint64_t kFewWalks = 148 * 5, kManyWalks = 148 * 48;
+// Warps that walk whole sequences, or where those would be too few to keep the
+// loads of 148 SMs under way, crews, or where even those are too few, segments
+// (64 steps at least).
+constexpr uint64_t kFewWalks = 148 * 5, kFewCrews = 64, kManyWalks = 148 * 48;
 constexpr uint32_t kLeastSegment = 64;
 Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     Plan p = {};
@@ -123,16 +125,20 @@ Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     p.columns = (p.flat + 32 * width - 1) / (32 * width);
     p.segments = 1, p.segment_steps = (uint32_t)q.steps;
     if (p.columns && p.columns < kFewWalks && q.steps >= 2 * kLeastSegment) {
-        const uint64_t want = std::max<uint64_t>(kLeastSegment, q.steps * p.columns / kManyWalks);
-        p.segment_steps = (uint32_t)((want + kSteps - 1) / kSteps * kSteps);
-        p.segments = (uint32_t)((q.steps + p.segment_steps - 1) / p.segment_steps);
+        p.crew = width <= 2 && p.columns >= kFewCrews;
+        if (!p.crew) {
+            const uint64_t want = std::max<uint64_t>(kLeastSegment, q.steps * p.columns / kManyWalks);
+            p.segment_steps = (uint32_t)((want + kSteps - 1) / kSteps * kSteps);
+            p.segments = (uint32_t)((q.steps + p.segment_steps - 1) / p.segment_steps);
+        }
     }
+    p.partials = p.crew ? kCrew : p.segments;
     const auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
     const uint64_t cut = p.segments > 1 ? p.segments * p.flat : 0;
     p.maps = 0;
     p.states = p.maps + round(cut * 8);
     p.partial = p.states + round(cut * 4);
-    p.bytes = p.partial + round(p.segments * p.flat * 4);
+    p.bytes = p.partial + round(p.partials * p.flat * 4);
     return p;
 }
 
@@ -143,7 +149,7 @@ void fill(Args &g, const snn_b200_leaky_t &q, const Plan &p, void *workspace) {
     g.yb = q.y_batch_stride, g.yt = q.y_step_stride, g.dyb = q.dy_batch_stride, g.dyt = q.dy_step_stride;
     g.dxb = q.dx_batch_stride, g.dxt = q.dx_step_stride, g.dgb = q.dgate_batch_stride, g.dgt = q.dgate_step_stride;
     g.decay = q.decay, g.scale = q.input_scale, g.logit = q.logit, g.complement = q.complement;
-    g.columns = (uint32_t)p.columns, g.segments = p.segments, g.segment_steps = p.segment_steps;
+    g.columns = (uint32_t)p.columns, g.segments = p.segments, g.segment_steps = p.segment_steps, g.crew = p.crew;
     char *w = (char *)workspace;
     g.maps = (float2 *)(w + p.maps);
     g.states = (float *)(w + p.states);
@@ -294,7 +300,7 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
     if (e == cudaSuccess && sums) {
         const uint32_t rows = shared ? 1u : (uint32_t)(q.batch < 65535 ? q.batch : 65535);
         e = launch_early(gate_sum_kernel, dim3((uint32_t)((q.channels + 31) / 32), rows), kSumWarps * 32, 0, s, 1, g.partial,
-                         p.segments, q.batch, q.channels, (float *)dgate, shared ? 0 : q.dgate_batch_stride);
+                         p.partials, q.batch, q.channels, (float *)dgate, shared ? 0 : q.dgate_batch_stride);
     }
     return op_status(e, __func__);
 }

@@ -8,10 +8,15 @@
 // worked on; a thread reads only what it copied itself, so nothing waits for
 // another warp.
 //
-// Few channels leave most of the GPU idle, so their steps are cut into
-// segments. Steps compose as affine maps h -> A h + H: one kernel walks each
-// segment for its (A, H), one folds them in order into the state before each
-// segment, and the walk itself then starts everywhere at once. The inputs are
+// Fewer channels than keep the GPU busy that way are walked by crews: the warps
+// of a CTA take the next blocks of one column side by side. Steps compose as
+// affine maps h -> A h + H; each warp shares its block's map, folds those before
+// its own onto the state, and then walks its block.
+//
+// Where even crews are too few, the steps are cut into
+// segments: one kernel walks each segment for its map, one folds them in order
+// into the state before each segment, and the walk itself then starts
+// everywhere at once. The inputs are
 // read twice; the second walk goes through the segments in the opposite order
 // and so finds the last ones in L2. (Measured against one pass whose tiles wait
 // for the maps of the tiles before them: 1 x 65536 x 1024 bf16 took 0.37 to 0.45 ms
@@ -355,6 +360,18 @@ __device__ __forceinline__ Row<V> load_state(const float *p, uint64_t i) {
     return p ? load<float, V>(p + i) : all<V>(0.0f);
 }
 template <int V>
+__device__ __forceinline__ void load_map(const float2 *p, Row<V> &A, Row<V> &H) {
+#pragma unroll
+    for (int q = 0; q < V; q += 2) {
+        if constexpr (V == 1) {
+            A.v[0] = p->x, H.v[0] = p->y;
+        } else {
+            const float4 m = *reinterpret_cast<const float4 *>(p + q);
+            A.v[q] = m.x, H.v[q] = m.y, A.v[q + 1] = m.z, H.v[q + 1] = m.w;
+        }
+    }
+}
+template <int V>
 __device__ __forceinline__ void store_map(float2 *p, const Row<V> &A, const Row<V> &H) {
 #pragma unroll
     for (int q = 0; q < V; q += 2) {
@@ -444,6 +461,125 @@ __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_const
     } else {
         if (g.h_last && w.segment + 1 == g.segments) store<float, V>(g.h_last + p.i, h);
     }
+}
+
+// ---- crews ----
+template <int V>
+struct Crew {
+    float2 map[2][kCrew][32 * V];  // of this round and the one before
+    float state[2][32 * V];        // behind a round
+};
+// Blocks under way or at hand for each warp, as shared memory allows.
+template <int V>
+constexpr uint32_t crew_depth(uint32_t slot) {
+    return 3 * kCrew * slot + (uint32_t)sizeof(Crew<V>) <= 227 * 1024 ? 3 : 2;
+}
+// The next rounds of a crew's warp: fetch(t0, slot) and work(n, t0, slot) of
+// its block in each; a block behind the last one is only worked on (on = false).
+template <bool Reverse, uint32_t Depth, typename Fetch, typename Work>
+__device__ __forceinline__ void walk_rounds(uint32_t steps, Fetch fetch, Work work) {
+    const uint32_t warp = threadIdx.x / 32, blocks = (steps + kSteps - 1) / kSteps;
+    const uint32_t rounds = (blocks + kCrew - 1) / kCrew;
+    const auto at = [&](uint32_t n) { return (Reverse ? blocks - 1 - (n * kCrew + warp) : n * kCrew + warp) * kSteps; };
+    const auto on = [&](uint32_t n) { return n * kCrew + warp < blocks; };
+#pragma unroll
+    for (uint32_t n = 0; n < Depth - 1; ++n) {
+        if (on(n)) fetch(at(n), n);
+        fetched();
+    }
+    uint32_t slot = 0;
+    for (uint32_t n = 0; n < rounds; ++n) {
+        const uint32_t next = n + Depth - 1;
+        if (on(next)) fetch(at(next), slot ? slot - 1 : Depth - 1);
+        fetched();
+        await<Depth - 1>();
+        __syncwarp();
+        work(n, on(n), at(n), slot);
+        slot = slot + 1 == Depth ? 0 : slot + 1;
+    }
+}
+// Shares a block's map and folds the state before it. The last warp's walk of the
+// round before has left the state there.
+template <int V>
+__device__ __forceinline__ Row<V> crew_state(Crew<V> &c, uint32_t n, const Row<V> &A, const Row<V> &H, const Row<V> &first) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, turn = n & 1;
+    store_map<V>(&c.map[turn][warp][lane * V], A, H);
+    __syncthreads();
+    Row<V> h = n ? load<float, V>(&c.state[turn ^ 1][lane * V]) : first;
+#pragma unroll
+    for (uint32_t w = 0; w + 1 < kCrew; ++w) {
+        if (w >= warp) break;
+        Row<V> a, b;
+        load_map<V>(&c.map[turn][w][lane * V], a, b);
+        h = fma(a, h, b);
+    }
+    return h;
+}
+template <int V>
+__device__ __forceinline__ void crew_done(Crew<V> &c, uint32_t n, const Row<V> &h) {
+    if (threadIdx.x / 32 + 1 == kCrew) store<float, V>(&c.state[n & 1][(threadIdx.x & 31) * V], h);
+}
+
+template <typename X, typename G, typename Y, int V>
+__global__ void __launch_bounds__(kCrew * 32) scan_crew_kernel(const __grid_constant__ Args g) {
+    extern __shared__ __align__(16) uint8_t s_feed[];
+    __shared__ Crew<V> s_crew;
+    after_previous();
+    const uint32_t warp = threadIdx.x / 32;
+    const Place p = place_of<V>(g, blockIdx.x);
+    constexpr uint32_t kX = Feed<X, V>::kBytes, kSlot = kX + Feed<G, V>::kBytes;
+    constexpr uint32_t kDeep = crew_depth<V>(kSlot);
+    uint8_t *mine = s_feed + warp * (kDeep * kSlot);
+    Feed<X, V> fx;
+    Feed<G, V> fz;
+    Gates<G, V> gates;
+    gates.init(g, p);
+    fx.init(g, g.x, p, blockIdx.x, g.xb, g.xt);
+    fz.init(g, g.gate, p, blockIdx.x, g.gb, g.gt);
+    const Row<V> first = p.on ? load_state<V>(g.h0, p.i) : all<V>(0.0f);
+    Row<V> h = first;
+    walk_rounds<false, kDeep>(
+        g.steps,
+        [&](uint32_t t0, uint32_t slot) {
+            fz.fetch(mine + slot * kSlot + kX, t0);
+            fx.fetch(mine + slot * kSlot, t0);
+        },
+        [&](uint32_t n, bool on, uint32_t t0, uint32_t slot) {
+            const int live = on ? live_steps(p.len, t0) : 0;
+            Row<V> a[kSteps], u[kSteps], A = all<V>(1.0f), H = all<V>(0.0f);
+            {
+                Vec<X, V> x[kSteps];
+                if (on) {
+                    gates.take(fz, mine + slot * kSlot + kX, t0, live);
+                    fx.take(mine + slot * kSlot, t0, live, x);
+                }
+                each_step<X, G, V>(g, gates, x, live, [&](int j, const Row<V> &aj, const Row<V> &uj) {
+                    a[j] = aj, u[j] = uj;
+                    A = mul(aj, A);
+                    H = fma(aj, H, uj);
+                });
+            }
+            h = crew_state<V>(s_crew, n, A, H, first);
+            if (on && p.on) {
+                if (g.saved) store<float, V>(saved_at(g, p, t0), h);
+                Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
+                if (live == (int)kSteps) {
+#pragma unroll
+                    for (int j = 0; j < (int)kSteps; ++j) {
+                        h = fma(a[j], h, u[j]);
+                        store<Y, V>(y + j * g.yt, narrow<Y, V>(h));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < (int)kSteps; ++j) {
+                        if (j < live) h = fma(a[j], h, u[j]);
+                        if (t0 + j < g.steps) store<Y, V>(y + j * g.yt, j < live ? narrow<Y, V>(h) : Vec<Y, V>{});
+                    }
+                }
+            }
+            crew_done<V>(s_crew, n, h);
+        });
+    if (g.h_last && p.on && warp + 1 == kCrew) store<float, V>(g.h_last + p.i, h);
 }
 
 // ---- gradient ----
@@ -613,6 +749,70 @@ __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const _
     }
 }
 
+template <typename X, typename G, typename Y, int V>
+__global__ void __launch_bounds__(kCrew * 32) back_crew_kernel(const __grid_constant__ Args g) {
+    extern __shared__ __align__(16) uint8_t s_feed[];
+    __shared__ Crew<V> s_crew;
+    after_previous();
+    const uint32_t warp = threadIdx.x / 32;
+    const Place p = place_of<V>(g, blockIdx.x);
+    constexpr uint32_t kY = Feed<Y, V>::kBytes, kZ = kY + Feed<G, V>::kBytes, kS = kZ + Feed<X, V>::kBytes,
+                       kSlot = kS + kSavedBytes<V>;
+    constexpr uint32_t kDeep = crew_depth<V>(kSlot);
+    uint8_t *mine = s_feed + warp * (kDeep * kSlot);
+    Feed<X, V> fx;
+    Feed<G, V> fz;
+    Feed<Y, V> fy;
+    fx.init(g, g.x, p, blockIdx.x, g.xb, g.xt);
+    fz.init(g, g.gate, p, blockIdx.x, g.gb, g.gt);
+    fy.init(g, g.dy, p, blockIdx.x, g.dyb, g.dyt);
+    Back<X, G, Y, V> b;
+    b.gates.init(g, p);
+    const Row<V> first = p.on ? load_state<V>(g.dh_last, p.i) : all<V>(0.0f);
+    Row<V> e = first;
+    double total[V] = {};
+    walk_rounds<true, kDeep>(
+        g.steps,
+        [&](uint32_t t0, uint32_t slot) {
+            fy.fetch(mine + slot * kSlot, t0);
+            fz.fetch(mine + slot * kSlot + kY, t0);
+            fx.fetch(mine + slot * kSlot + kZ, t0);
+            if (p.on && t0 < p.len)
+                Feed<float, V>::template copy<4 * V>(
+                    (uint32_t)__cvta_generic_to_shared(mine + slot * kSlot + kS) + (threadIdx.x & 31) * 4 * V,
+                    saved_at(g, p, t0));
+        },
+        [&](uint32_t n, bool on, uint32_t t0, uint32_t slot) {
+            const int live = on ? live_steps(p.len, t0) : 0;
+            Row<V> A = all<V>(1.0f), E = all<V>(0.0f);
+            if (on) {
+                Vec<X, V> x[kSteps];
+                b.gates.take(fz, mine + slot * kSlot + kY, t0, live);
+                fy.take(mine + slot * kSlot, t0, live, b.dy);
+                fx.take(mine + slot * kSlot + kZ, t0, live, x);
+                b.maps(g, x, reinterpret_cast<const Row<V> *>(mine + slot * kSlot + kS)[threadIdx.x & 31], live);
+#pragma unroll
+                for (int j = (int)kSteps - 1; j >= 0; --j) A = mul(b.a[j], A), b.step(j, live, E);
+            }
+            e = crew_state<V>(s_crew, n, A, E, first);
+            if (on) {
+                const Row<V> sum = b.emit(g, p, t0, live, e);
+                if (!b.kEvery)
+#pragma unroll
+                    for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
+            }
+            crew_done<V>(s_crew, n, e);
+        });
+    if (!p.on) return;
+    if (g.dh0 && warp + 1 == kCrew) store<float, V>(g.dh0 + p.i, e);
+    if (g.partial) {
+        Row<V> sum;
+#pragma unroll
+        for (int q = 0; q < V; ++q) sum.v[q] = (float)total[q];
+        put_partial(g, p, b.gates, warp, sum);
+    }
+}
+
 // ---- single step ----
 // A row of the pool is updated by the threads of the first row that names
 // it, which also do the later rows that name it, in order. To know, every CTA
@@ -693,35 +893,41 @@ cudaError_t step_narrow(cudaStream_t s, const Form &f, const StepArgs &a, dim3 g
     return wide ? launch_step<X, X, float>(s, f, a, grid) : launch_step<X, X, X>(s, f, a, grid);
 }
 
+// grid CTAs of `warps` warps, each with `feed` bytes of shared memory, beside `fixed` bytes of the kernel's own.
 template <typename K>
-cudaError_t start(K kernel, cudaStream_t s, const Args &a, uint32_t slot) {
-    const uint32_t smem = kWarps * kDepth * slot;
-    if (smem > 48 * 1024) {
+cudaError_t start(K kernel, cudaStream_t s, const Args &a, uint64_t grid, uint32_t warps, uint32_t feed, uint32_t fixed = 0) {
+    const uint32_t smem = warps * feed;
+    if (smem + fixed > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    const uint32_t grid = (uint32_t)(((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps);
-    return launch_early(kernel, grid, kWarps * 32, smem, s, 1, a);
+    return launch_early(kernel, (uint32_t)grid, warps * 32, smem, s, 1, a);
 }
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_scan(cudaStream_t s, const Args &a) {
     constexpr uint32_t slot = Feed<X, V>::kBytes + Feed<G, V>::kBytes;
+    if constexpr (V <= 2)
+        if (a.crew)
+            return start(scan_crew_kernel<X, G, Y, V>, s, a, a.columns, kCrew, crew_depth<V>(slot) * slot, sizeof(Crew<V>));
+    const uint64_t grid = ((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps;
     if (a.segments > 1) {
-        cudaError_t e = start(scan_kernel<X, G, Y, V, true>, s, a, slot);
+        cudaError_t e = start(scan_kernel<X, G, Y, V, true>, s, a, grid, kWarps, kDepth * slot);
         if (e == cudaSuccess) e = carry(s, a, false);
         if (e != cudaSuccess) return e;
     }
-    return start(scan_kernel<X, G, Y, V, false>, s, a, slot);
+    return start(scan_kernel<X, G, Y, V, false>, s, a, grid, kWarps, kDepth * slot);
 }
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_back(cudaStream_t s, const Args &a) {
-    constexpr uint32_t slot = Feed<G, V>::kBytes + Feed<Y, V>::kBytes;
+    constexpr uint32_t maps = Feed<G, V>::kBytes + Feed<Y, V>::kBytes, slot = maps + Feed<X, V>::kBytes + kSavedBytes<V>;
+    if (a.crew) return start(back_crew_kernel<X, G, Y, V>, s, a, a.columns, kCrew, crew_depth<V>(slot) * slot, sizeof(Crew<V>));
+    const uint64_t grid = ((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps;
     if (a.segments > 1) {
-        cudaError_t e = start(back_kernel<X, G, Y, V, true>, s, a, slot);
+        cudaError_t e = start(back_kernel<X, G, Y, V, true>, s, a, grid, kWarps, kDepth * maps);
         if (e == cudaSuccess) e = carry(s, a, true);
         if (e != cudaSuccess) return e;
     }
-    return start(back_kernel<X, G, Y, V, false>, s, a, slot + Feed<X, V>::kBytes + kSavedBytes<V>);
+    return start(back_kernel<X, G, Y, V, false>, s, a, grid, kWarps, kDepth * slot);
 }
 template <typename X, typename G, typename Y>
 cudaError_t launch(cudaStream_t s, const Form &f, const Args &a, bool back) {

@@ -9,6 +9,11 @@ HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 # each, quotient 2 units of 2^-23), the input's two products and the fused
 # update together stay below 2^-20 of the magnitudes they combine.
 STEP = 2.0 ** -20
+# A rounding to 32 bits is off by half a unit of the result, that is by a share
+# of 2^-24 of it, but never by less than half of the smallest subnormal, 2^-150,
+# where the result is subnormal. A step has at most four roundings that reach its
+# state (two of the input's products, one each of a product and a sum).
+TINY = 4 * 2.0 ** -150
 
 
 def mx4_parts(x):
@@ -94,7 +99,7 @@ class LeakyRef:
             self.before[:, i], self.before_err[:, i] = h, err
             a = self.a[:, i]
             nbig = np.abs(a) * big + np.abs(u[:, i])
-            big, err = np.where(on, nbig, big), np.where(on, np.abs(a) * err + STEP * nbig, err)
+            big, err = np.where(on, nbig, big), np.where(on, np.abs(a) * err + STEP * nbig + TINY, err)
             h = np.where(on, a * h + u[:, i], h)
             self.y[:, i], self.y_err[:, i] = np.where(on, h, 0), np.where(on, err, 0)
         self.h_last, self.h_last_err = h, err
@@ -110,19 +115,19 @@ class LeakyRef:
             on = live[:, i]
             a = self.a[:, i]
             step, nbig = dy[:, i] + e, np.abs(dy[:, i]) + big
-            serr = err + STEP * nbig
+            serr = err + STEP * nbig + TINY
             d[:, i], derr[:, i] = np.where(on, step, 0), np.where(on, serr, 0)
             e, big = np.where(on, a * step, e), np.where(on, np.abs(a) * nbig, big)
-            err = np.where(on, np.abs(a) * serr + STEP * big, err)
+            err = np.where(on, np.abs(a) * serr + STEP * big + TINY, err)
         self.dh0, self.dh0_err = e, err
         f = self.scale * (self.rest if self.complement else 1.0)
         self.dx = d * f
-        self.dx_err = np.abs(f) * (derr + STEP * np.abs(d))
+        self.dx_err = np.abs(f) * (derr + STEP * np.abs(d)) + TINY
         k = self.before - self.sx if self.complement else self.before
         kmag = np.abs(self.before) + (np.abs(self.sx) if self.complement else 0.0)
         s = self.a * self.rest if self.logit else 1.0
         dg = d * k * s
-        derr = np.abs(s) * (derr * np.abs(k) + (np.abs(d) + derr) * (self.before_err + STEP * kmag)) + STEP * np.abs(dg)
+        derr = np.abs(s) * (derr * np.abs(k) + (np.abs(d) + derr) * (self.before_err + STEP * kmag)) + STEP * np.abs(dg) + TINY
         if self.gate is None:
             return
         g = np.asarray(self.gate)

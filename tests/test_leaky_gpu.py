@@ -140,6 +140,15 @@ def test_uneven_lengths(src, gate, logit):
     Problem(2, 5000, 34, src, gate, "f32", None, logit, False, lengths=[4000, 2048], seed=5).verify()
 
 
+@pytest.mark.parametrize("src,gate,gate_type,out", [("bf16", "step", "bf16", "bf16"), ("f32", "step", "f32", "f32"),
+                                                    ("bf16", "step", "f32", "f32"), ("f16", "channel", "f32", "f16"),
+                                                    ("u8", "channel", "f32", "f32"), ("u8", "step", "f32", "f32")])
+@pytest.mark.parametrize("b,t,c,lengths", [(3, 300, 1500, None), (4, 129, 1026, [129, 0, 128, 57]), (70, 135, 61, None)])
+def test_columns_in_the_hundreds(b, t, c, lengths, src, gate, gate_type, out):
+    """Enough channels for whole rows of CTAs, too few for a warp each."""
+    Problem(b, t, c, src, gate, gate_type, out, True, True, 0.5, lengths, seed=18).verify()
+
+
 def test_many_sequences_take_the_same_values():
     """How the work is split does not show: rows of a large batch against a small one."""
     p = Problem(2000, 25, 130, "u8", "channel", time_major=True, seed=6)

@@ -36,93 +36,102 @@ struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
 
-// Arithmetic on a thread's channels, two at a time where there are two: the
-// kernels' instruction count, not their arithmetic, is what is scarce.
+// A thread's channels of one step, in 32 bits. Two of them share a register pair
+// and an instruction: the instructions, not the arithmetic, are what is scarce.
 template <int V>
-using Row = Vec<float, V>;
-template <int V>
-__device__ __forceinline__ uint64_t two(const Row<V> &a, int q) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[q]), "f"(a.v[q + 1]));
-    return r;
-}
-template <int V>
-__device__ __forceinline__ void split(uint64_t r, Row<V> &o, int q) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(o.v[q]), "=f"(o.v[q + 1]) : "l"(r));
-}
+struct Row {
+    uint64_t r[V / 2];
+    __device__ __forceinline__ float lo(int i) const {
+        float f;
+        asm("{\n .reg .b32 h;\n mov.b64 {%0, h}, %1;\n}" : "=f"(f) : "l"(r[i]));
+        return f;
+    }
+    __device__ __forceinline__ float hi(int i) const {
+        float f;
+        asm("{\n .reg .b32 l;\n mov.b64 {l, %0}, %1;\n}" : "=f"(f) : "l"(r[i]));
+        return f;
+    }
+    __device__ __forceinline__ float operator[](int q) const { return q % 2 ? hi(q / 2) : lo(q / 2); }
+    // Element q is f(q).
+    template <typename F>
+    static __device__ __forceinline__ Row of(F f) {
+        Row o;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float l = f(2 * i), h = f(2 * i + 1);
+            asm("mov.b64 %0, {%1, %2};" : "=l"(o.r[i]) : "f"(l), "f"(h));
+        }
+        return o;
+    }
+};
+template <>
+struct Row<1> {
+    float f;
+    __device__ __forceinline__ float operator[](int) const { return f; }
+    template <typename F>
+    static __device__ __forceinline__ Row of(F g) {
+        return {g(0)};
+    }
+};
 template <int V>
 __device__ __forceinline__ Row<V> fma(const Row<V> &a, const Row<V> &b, const Row<V> &c) {
-    Row<V> o;
     if constexpr (V == 1) {
-        o.v[0] = __fmaf_rn(a.v[0], b.v[0], c.v[0]);
+        return {__fmaf_rn(a.f, b.f, c.f)};
     } else {
+        Row<V> o;
 #pragma unroll
-        for (int q = 0; q < V; q += 2) {
-            uint64_t r;
-            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(two(a, q)), "l"(two(b, q)), "l"(two(c, q)));
-            split(r, o, q);
-        }
+        for (int i = 0; i < V / 2; ++i) asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o.r[i]) : "l"(a.r[i]), "l"(b.r[i]), "l"(c.r[i]));
+        return o;
     }
-    return o;
 }
 template <int V>
 __device__ __forceinline__ Row<V> mul(const Row<V> &a, const Row<V> &b) {
-    Row<V> o;
     if constexpr (V == 1) {
-        o.v[0] = __fmul_rn(a.v[0], b.v[0]);
+        return {__fmul_rn(a.f, b.f)};
     } else {
+        Row<V> o;
 #pragma unroll
-        for (int q = 0; q < V; q += 2) {
-            uint64_t r;
-            asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a, q)), "l"(two(b, q)));
-            split(r, o, q);
-        }
+        for (int i = 0; i < V / 2; ++i) asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o.r[i]) : "l"(a.r[i]), "l"(b.r[i]));
+        return o;
     }
-    return o;
 }
 template <int V>
 __device__ __forceinline__ Row<V> add(const Row<V> &a, const Row<V> &b) {
-    Row<V> o;
     if constexpr (V == 1) {
-        o.v[0] = __fadd_rn(a.v[0], b.v[0]);
+        return {__fadd_rn(a.f, b.f)};
     } else {
+        Row<V> o;
 #pragma unroll
-        for (int q = 0; q < V; q += 2) {
-            uint64_t r;
-            asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(two(a, q)), "l"(two(b, q)));
-            split(r, o, q);
-        }
+        for (int i = 0; i < V / 2; ++i) asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o.r[i]) : "l"(a.r[i]), "l"(b.r[i]));
+        return o;
     }
-    return o;
 }
 template <int V>
 __device__ __forceinline__ Row<V> all(float f) {
-    Row<V> o;
-#pragma unroll
-    for (int q = 0; q < V; ++q) o.v[q] = f;
-    return o;
+    return Row<V>::of([&](int) { return f; });
 }
 template <typename T, int V>
 __device__ __forceinline__ Row<V> widen(const Vec<T, V> &a) {
-    Row<V> o;
-#pragma unroll
-    for (int q = 0; q < V; ++q) o.v[q] = to_float(a.v[q]);
-    return o;
+    if constexpr (V > 1 && std::is_same<T, __nv_bfloat16>::value) {  // the halves of a word, without taking them apart
+        return Row<V>::of([&](int q) {
+            const uint32_t w = reinterpret_cast<const uint32_t *>(&a)[q / 2];
+            return __uint_as_float(q % 2 ? w & 0xffff0000u : w << 16);
+        });
+    }
+    return Row<V>::of([&](int q) { return to_float(a.v[q]); });
 }
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> narrow(const Row<V> &a) {
     Vec<T, V> o;
     if constexpr (V > 1 && std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-        for (int q = 0; q < V; q += 2)
-            *reinterpret_cast<__nv_bfloat162 *>(&o.v[q]) = __floats2bfloat162_rn(a.v[q], a.v[q + 1]);
+        for (int q = 0; q < V; q += 2) *reinterpret_cast<__nv_bfloat162 *>(&o.v[q]) = __floats2bfloat162_rn(a[q], a[q + 1]);
     } else if constexpr (V > 1 && std::is_same<T, __half>::value) {
 #pragma unroll
-        for (int q = 0; q < V; q += 2)
-            *reinterpret_cast<__half2 *>(&o.v[q]) = __floats2half2_rn(a.v[q], a.v[q + 1]);
+        for (int q = 0; q < V; q += 2) *reinterpret_cast<__half2 *>(&o.v[q]) = __floats2half2_rn(a[q], a[q + 1]);
     } else {
 #pragma unroll
-        for (int q = 0; q < V; ++q) o.v[q] = from_float<T>(a.v[q]);
+        for (int q = 0; q < V; ++q) o.v[q] = from_float<T>(a[q]);
     }
     return o;
 }
@@ -138,30 +147,38 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
 // No gate array, or one without a step stride: the gate is a constant of the thread.
 struct Fixed {};
 
-struct Leak {
-    float a, rest;  // the gate and one minus it
-};
-// Both from one exponential of a non-positive number, so that neither is a
-// difference of nearly equal values. A 16-bit logit has a rounding of 2^-9 of
-// itself, so for it the product with log2(e) is rounded once to 32 bits (2^-20
-// of the exponential up to logits of 22).
-template <typename G, bool Logit>
-__device__ __forceinline__ Leak leak_of(G gate) {
-    const float z = to_float(gate);
-    if (!Logit) return {z, __fsub_rn(1.0f, z)};
-    float t, r;
-    if (sizeof(G) == 2) {
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(__fmul_rn(fabsf(z), -1.44269504f)));
+// The gate and one minus it from gates z. Of logits, both come from one
+// exponential of a non-positive number, so that neither is a difference of
+// nearly equal values. A 16-bit logit has a rounding of 2^-9 of itself, so for it
+// the product with log2(e) is rounded once to 32 bits (2^-20 of the exponential
+// up to logits of 22).
+template <typename G, bool Logit, int V>
+__device__ __forceinline__ void leak_of(const Vec<G, V> &z, Row<V> &a, Row<V> &rest) {
+    if constexpr (!Logit) {
+        a = widen(z);
+        rest = fma(a, all<V>(-1.0f), all<V>(1.0f));
     } else {
-        t = expf(-fabsf(z));
+        const Row<V> f = widen(z);
+        const Row<V> t = Row<V>::of([&](int q) {
+            const float m = fabsf(f[q]);
+            if constexpr (sizeof(G) == 2) {
+                float e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(m, -1.44269504f)));
+                return e;
+            } else {
+                return expf(-m);
+            }
+        });
+        const Row<V> one = add(t, all<V>(1.0f));
+        const Row<V> r = Row<V>::of([&](int q) {
+            float i;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(i) : "f"(one[q]));
+            return i;
+        });
+        const Row<V> s = mul(t, r);
+        a = Row<V>::of([&](int q) { return f[q] >= 0.0f ? r[q] : s[q]; });
+        rest = Row<V>::of([&](int q) { return f[q] >= 0.0f ? s[q] : r[q]; });
     }
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, t)));
-    const float q = __fmul_rn(t, r);
-    return z >= 0.0f ? Leak{r, q} : Leak{q, r};
-}
-template <typename G>
-__device__ __forceinline__ Leak leak_from(G z, int logit) {
-    return logit ? leak_of<G, true>(z) : leak_of<G, false>(z);
 }
 
 // f(logit, complement) with the call's flags as constants: a test for every
@@ -227,7 +244,7 @@ struct Feed {
     static constexpr uint32_t kOwn = (uint32_t)sizeof(T) * V;           // bytes of a thread's piece of a row
     static constexpr uint32_t kRow = 32 * kOwn, kBytes = kRow * kSteps;  // of a row, of a block
     static constexpr uint32_t kAcross = kRow / 16, kAtOnce = 32 / kAcross;  // lanes on a row, rows of a copy
-    const T *p, *q;  // the thread's piece, the one it copies
+    const T *p, *q;  // the thread's piece, the first one it copies
     int64_t stride;
     uint32_t len;  // of the sequence it copies from
     bool wide;
@@ -240,7 +257,8 @@ struct Feed {
         if (wide) {
             const uint64_t i = column * 32 * V + (threadIdx.x & 31) % kAcross * (16 / sizeof(T));
             const int64_t b = i < g.flat ? (int64_t)(i / g.channels) : 0;
-            q = (const T *)base + b * sb + (int64_t)(i - (uint64_t)b * g.channels);
+            q = (const T *)base + b * sb + (int64_t)(i - (uint64_t)b * g.channels) +
+                (int64_t)((threadIdx.x & 31) / kAcross) * st;
             len = i >= g.flat ? 0u : g.lengths ? min(g.lengths[b], g.steps) : g.steps;
         } else {
             q = p;
@@ -259,11 +277,10 @@ struct Feed {
         const int live = live_steps(len, t0);
         const T *row = q + (int64_t)t0 * stride;
         if (wide) {
+            const int left = live - (int)(lane / kAcross);  // of the rows from this lane's first on
 #pragma unroll
-            for (uint32_t j = 0; j < kSteps; j += kAtOnce) {
-                const uint32_t r = j + lane / kAcross;
-                if ((int)r < live) copy<16>(at + (j * kAcross + lane) * 16, row + r * stride);
-            }
+            for (uint32_t j = 0; j < kSteps; j += kAtOnce, row += kAtOnce * stride)
+                if ((int)j < left) copy<16>(at + (j * kAcross + lane) * 16, row);
         } else if constexpr (kOwn >= 4) {
 #pragma unroll
             for (int j = 0; j < (int)kSteps; ++j)
@@ -329,24 +346,20 @@ struct Gates {
     }
     template <bool Logit>
     __device__ __forceinline__ void at(int j, Row<V> &a, Row<V> &rest) const {
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            const Leak l = leak_of<G, Logit>(raw[j].v[q]);
-            a.v[q] = l.a, rest.v[q] = l.rest;
-        }
+        leak_of<G, Logit, V>(raw[j], a, rest);
     }
 };
 template <int V>
 struct Gates<Fixed, V> {
     Row<V> a_, rest_;
     __device__ __forceinline__ void init(const Args &g, const Place &p) {
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            const Leak l = !g.gate ? Leak{g.decay, __fsub_rn(1.0f, g.decay)}
-                           : p.on  ? leak_from(((const float *)g.gate)[p.b * g.gb + p.c + q], g.logit)
-                                   : Leak{1.0f, 0.0f};
-            a_.v[q] = l.a, rest_.v[q] = l.rest;
+        if (!g.gate) {
+            a_ = all<V>(g.decay), rest_ = all<V>(__fsub_rn(1.0f, g.decay));
+            return;
         }
+        const Vec<float, V> z = p.on ? load<float, V>((const float *)g.gate + p.b * g.gb + p.c) : Vec<float, V>{};
+        if (g.logit) leak_of<float, true, V>(z, a_, rest_);
+        else leak_of<float, false, V>(z, a_, rest_);
     }
     __device__ __forceinline__ void take(const Feed<Fixed, V> &, const uint8_t *, uint32_t, int) {}
     template <bool Logit>
@@ -356,27 +369,23 @@ struct Gates<Fixed, V> {
 };
 
 template <int V>
-__device__ __forceinline__ Row<V> load_state(const float *p, uint64_t i) {
-    return p ? load<float, V>(p + i) : all<V>(0.0f);
+__device__ __forceinline__ Row<V> load_row(const float *p) {
+    return widen(load<float, V>(p));
 }
 template <int V>
-__device__ __forceinline__ void load_map(const float2 *p, Row<V> &A, Row<V> &H) {
-#pragma unroll
-    for (int q = 0; q < V; q += 2) {
-        if constexpr (V == 1) {
-            A.v[0] = p->x, H.v[0] = p->y;
-        } else {
-            const float4 m = *reinterpret_cast<const float4 *>(p + q);
-            A.v[q] = m.x, H.v[q] = m.y, A.v[q + 1] = m.z, H.v[q + 1] = m.w;
-        }
-    }
+__device__ __forceinline__ void store_row(float *p, const Row<V> &a) {
+    store<float, V>(p, narrow<float, V>(a));
+}
+template <int V>
+__device__ __forceinline__ Row<V> load_state(const float *p, uint64_t i) {
+    return p ? load_row<V>(p + i) : all<V>(0.0f);
 }
 template <int V>
 __device__ __forceinline__ void store_map(float2 *p, const Row<V> &A, const Row<V> &H) {
 #pragma unroll
     for (int q = 0; q < V; q += 2) {
-        if constexpr (V == 1) *p = make_float2(A.v[0], H.v[0]);
-        else *reinterpret_cast<float4 *>(p + q) = make_float4(A.v[q], H.v[q], A.v[q + 1], H.v[q + 1]);
+        if constexpr (V == 1) *p = make_float2(A[0], H[0]);
+        else *reinterpret_cast<float4 *>(p + q) = make_float4(A[q], H[q], A[q + 1], H[q + 1]);
     }
 }
 
@@ -445,29 +454,34 @@ __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_const
                     h = fma(a, h, u);
                 });
             } else if (p.on) {
-                if (g.saved) store<float, V>(saved_at(g, p, t0), h);
+                if (g.saved) store_row<V>(saved_at(g, p, t0), h);
                 Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
-                each_step<X, G, V>(g, gates, x, live, [&](int j, const Row<V> &a, const Row<V> &u) {
+                each_step<X, G, V>(g, gates, x, live, [&](int, const Row<V> &a, const Row<V> &u) {
                     h = fma(a, h, u);
-                    store<Y, V>(y + j * g.yt, narrow<Y, V>(h));
+                    store<Y, V>(y, narrow<Y, V>(h));
+                    y += g.yt;
                 });
                 if (live < (int)kSteps)
-                    for (int j = live; j < (int)min(w.t1 - t0, kSteps); ++j) store<Y, V>(y + j * g.yt, Vec<Y, V>{});
+                    for (int j = live; j < (int)min(w.t1 - t0, kSteps); ++j, y += g.yt) store<Y, V>(y, Vec<Y, V>{});
             }
         });
     if (!p.on) return;
     if constexpr (Maps) {
         store_map<V>(g.maps + w.segment * g.flat + p.i, A, h);
     } else {
-        if (g.h_last && w.segment + 1 == g.segments) store<float, V>(g.h_last + p.i, h);
+        if (g.h_last && w.segment + 1 == g.segments) store_row<V>(g.h_last + p.i, h);
     }
 }
 
 // ---- crews ----
 template <int V>
+struct alignas(2 * sizeof(Row<V>)) Map {
+    Row<V> A, H;
+};
+template <int V>
 struct Crew {
-    float2 map[2][kCrew][32 * V];  // of this round and the one before
-    float state[2][32 * V];        // behind a round
+    Map<V> map[2][kCrew][32];  // of this round and the one before
+    Row<V> state[2][32];       // behind a round
 };
 // Blocks under way or at hand for each warp, as shared memory allows.
 template <int V>
@@ -503,21 +517,20 @@ __device__ __forceinline__ void walk_rounds(uint32_t steps, Fetch fetch, Work wo
 template <int V>
 __device__ __forceinline__ Row<V> crew_state(Crew<V> &c, uint32_t n, const Row<V> &A, const Row<V> &H, const Row<V> &first) {
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, turn = n & 1;
-    store_map<V>(&c.map[turn][warp][lane * V], A, H);
+    c.map[turn][warp][lane] = {A, H};
     __syncthreads();
-    Row<V> h = n ? load<float, V>(&c.state[turn ^ 1][lane * V]) : first;
-#pragma unroll
-    for (uint32_t w = 0; w + 1 < kCrew; ++w) {
-        if (w >= warp) break;
-        Row<V> a, b;
-        load_map<V>(&c.map[turn][w][lane * V], a, b);
-        h = fma(a, h, b);
+    Row<V> h = n ? c.state[turn ^ 1][lane] : first;
+    const Map<V> *m = &c.map[turn][0][lane];
+#pragma unroll 4
+    for (uint32_t w = 0; w < warp; ++w) {
+        const Map<V> v = m[w * 32];
+        h = fma(v.A, h, v.H);
     }
     return h;
 }
 template <int V>
 __device__ __forceinline__ void crew_done(Crew<V> &c, uint32_t n, const Row<V> &h) {
-    if (threadIdx.x / 32 + 1 == kCrew) store<float, V>(&c.state[n & 1][(threadIdx.x & 31) * V], h);
+    if (threadIdx.x / 32 + 1 == kCrew) c.state[n & 1][threadIdx.x & 31] = h;
 }
 
 template <typename X, typename G, typename Y, int V>
@@ -561,25 +574,25 @@ __global__ void __launch_bounds__(kCrew * 32) scan_crew_kernel(const __grid_cons
             }
             h = crew_state<V>(s_crew, n, A, H, first);
             if (on && p.on) {
-                if (g.saved) store<float, V>(saved_at(g, p, t0), h);
+                if (g.saved) store_row<V>(saved_at(g, p, t0), h);
                 Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
                 if (live == (int)kSteps) {
 #pragma unroll
-                    for (int j = 0; j < (int)kSteps; ++j) {
+                    for (int j = 0; j < (int)kSteps; ++j, y += g.yt) {
                         h = fma(a[j], h, u[j]);
-                        store<Y, V>(y + j * g.yt, narrow<Y, V>(h));
+                        store<Y, V>(y, narrow<Y, V>(h));
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < (int)kSteps; ++j) {
+                    for (int j = 0; j < (int)kSteps; ++j, y += g.yt) {
                         if (j < live) h = fma(a[j], h, u[j]);
-                        if (t0 + j < g.steps) store<Y, V>(y + j * g.yt, j < live ? narrow<Y, V>(h) : Vec<Y, V>{});
+                        if (t0 + j < g.steps) store<Y, V>(y, j < live ? narrow<Y, V>(h) : Vec<Y, V>{});
                     }
                 }
             }
             crew_done<V>(s_crew, n, h);
         });
-    if (g.h_last && p.on && warp + 1 == kCrew) store<float, V>(g.h_last + p.i, h);
+    if (g.h_last && p.on && warp + 1 == kCrew) store_row<V>(g.h_last + p.i, h);
 }
 
 // ---- gradient ----
@@ -641,19 +654,20 @@ struct Back {
     template <bool Whole>
     __device__ __forceinline__ Row<V> walk(const Args &g, const Place &p, uint32_t t0, int live, Row<V> &e) {
         using D = typename GradientOf<X>::type;
-        D *dx = (D *)g.dx + p.b * g.dxb + (int64_t)t0 * g.dxt + p.c;
-        G *dz = (G *)g.dgate + p.b * g.dgb + (int64_t)t0 * g.dgt + p.c;
+        const uint32_t end = t0 + kSteps - 1;
+        D *dx = (D *)g.dx + p.b * g.dxb + (int64_t)end * g.dxt + p.c;
+        G *dz = (G *)g.dgate + p.b * g.dgb + (int64_t)end * g.dgt + p.c;
         const int rows = t0 >= g.steps ? 0 : (int)min(g.steps - t0, kSteps);
         Row<V> sum = all<V>(0.0f);
 #pragma unroll
-        for (int j = (int)kSteps - 1; j >= 0; --j) {
+        for (int j = (int)kSteps - 1; j >= 0; --j, dx -= g.dxt, dz -= g.dgt) {
             const bool on = Whole || j < live;
             const Row<V> d = step(j, Whole ? (int)kSteps : live, e);
             if (!kEvery && on) sum = fma(d, fz[j], sum);
             if (!Whole && j >= rows) continue;
-            if (g.dx) store<D, V>(dx + j * g.dxt, on ? narrow<D, V>(mul(fx[j], d)) : Vec<D, V>{});
+            if (g.dx) store<D, V>(dx, on ? narrow<D, V>(mul(fx[j], d)) : Vec<D, V>{});
             if constexpr (kEvery)
-                if (g.dgate) store<G, V>(dz + j * g.dgt, on ? narrow<G, V>(mul(d, fz[j])) : Vec<G, V>{});
+                if (g.dgate) store<G, V>(dz, on ? narrow<G, V>(mul(d, fz[j])) : Vec<G, V>{});
         }
         return sum;
     }
@@ -666,7 +680,7 @@ struct Back {
 template <int V>
 __device__ __forceinline__ void put_partial(const Args &g, const Place &p, const Gates<Fixed, V> &gates, uint32_t segment,
                                             const Row<V> &sum) {
-    store<float, V>(g.partial + segment * g.flat + p.i, g.logit ? mul(sum, mul(gates.a_, gates.rest_)) : sum);
+    store_row<V>(g.partial + segment * g.flat + p.i, g.logit ? mul(sum, mul(gates.a_, gates.rest_)) : sum);
 }
 template <typename G, int V>
 __device__ __forceinline__ void put_partial(const Args &, const Place &, const Gates<G, V> &, uint32_t,
@@ -725,25 +739,23 @@ __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const _
                         }
                 });
             } else {
-                const Row<V> h = reinterpret_cast<const Row<V> *>(mine + slot * kSlot + kS)[threadIdx.x & 31];
+                const Row<V> h = load_row<V>((const float *)(mine + slot * kSlot + kS) + (threadIdx.x & 31) * V);
                 Vec<X, V> x[kSteps];
                 fx.take(mine + slot * kSlot + kZ, t0, live, x);
                 b.maps(g, x, h, live);
                 const Row<V> sum = b.emit(g, p, t0, live, e);
                 if (!b.kEvery)
 #pragma unroll
-                    for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
+                    for (int q = 0; q < V; ++q) total[q] += (double)sum[q];
             }
         });
     if (!p.on) return;
     if constexpr (Maps) {
         store_map<V>(g.maps + w.segment * g.flat + p.i, A, e);
     } else {
-        if (g.dh0 && w.segment == 0) store<float, V>(g.dh0 + p.i, e);
+        if (g.dh0 && w.segment == 0) store_row<V>(g.dh0 + p.i, e);
         if (g.partial) {
-            Row<V> sum;
-#pragma unroll
-            for (int q = 0; q < V; ++q) sum.v[q] = (float)total[q];
+            const Row<V> sum = Row<V>::of([&](int q) { return (float)total[q]; });
             put_partial(g, p, b.gates, w.segment, sum);
         }
     }
@@ -790,7 +802,7 @@ __global__ void __launch_bounds__(kCrew * 32) back_crew_kernel(const __grid_cons
                 b.gates.take(fz, mine + slot * kSlot + kY, t0, live);
                 fy.take(mine + slot * kSlot, t0, live, b.dy);
                 fx.take(mine + slot * kSlot + kZ, t0, live, x);
-                b.maps(g, x, reinterpret_cast<const Row<V> *>(mine + slot * kSlot + kS)[threadIdx.x & 31], live);
+                b.maps(g, x, load_row<V>((const float *)(mine + slot * kSlot + kS) + (threadIdx.x & 31) * V), live);
 #pragma unroll
                 for (int j = (int)kSteps - 1; j >= 0; --j) A = mul(b.a[j], A), b.step(j, live, E);
             }
@@ -799,16 +811,14 @@ __global__ void __launch_bounds__(kCrew * 32) back_crew_kernel(const __grid_cons
                 const Row<V> sum = b.emit(g, p, t0, live, e);
                 if (!b.kEvery)
 #pragma unroll
-                    for (int q = 0; q < V; ++q) total[q] += (double)sum.v[q];
+                    for (int q = 0; q < V; ++q) total[q] += (double)sum[q];
             }
             crew_done<V>(s_crew, n, e);
         });
     if (!p.on) return;
-    if (g.dh0 && warp + 1 == kCrew) store<float, V>(g.dh0 + p.i, e);
+    if (g.dh0 && warp + 1 == kCrew) store_row<V>(g.dh0 + p.i, e);
     if (g.partial) {
-        Row<V> sum;
-#pragma unroll
-        for (int q = 0; q < V; ++q) sum.v[q] = (float)total[q];
+        const Row<V> sum = Row<V>::of([&](int q) { return (float)total[q]; });
         put_partial(g, p, b.gates, warp, sum);
     }
 }
@@ -850,30 +860,28 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
     const bool padding = slot < 0 || slot >= (int64_t)g.slot_count;
     for (uint64_t c = ((uint64_t)blockIdx.y * across + threadIdx.x % across) * V; c < g.channels;
          c += (uint64_t)gridDim.y * across * V) {
-        Vec<Y, V> o = {};
         if (padding) {
-            *reinterpret_cast<Vec<Y, V> *>((Y *)g.y + row * g.ys + c) = o;
+            store<Y, V>((Y *)g.y + row * g.ys + c, Vec<Y, V>{});
             continue;
         }
-        Vec<float, V> *state = reinterpret_cast<Vec<float, V> *>(g.pool + slot * g.ps + c);
-        Vec<float, V> h = *state;
+        float *state = g.pool + slot * g.ps + c;
+        Row<V> h = load_row<V>(state);
         for (uint32_t r = row; r < g.batch; ++r) {
             if (r != row && g.slots[r] != (int32_t)slot) continue;
-            const Vec<X, V> x = *reinterpret_cast<const Vec<X, V> *>((const X *)g.x + r * g.xs + c);
-            Vec<G, V> z = {};
-            if (g.gate) z = *reinterpret_cast<const Vec<G, V> *>((const G *)g.gate + r * g.gs + c);
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                const Leak l = g.gate ? leak_from(z.v[q], g.logit) : Leak{g.decay, __fsub_rn(1.0f, g.decay)};
-                float u = __fmul_rn(g.scale, to_float(x.v[q]));
-                if (g.complement) u = __fmul_rn(u, l.rest);
-                h.v[q] = __fmaf_rn(l.a, h.v[q], u);
-                o.v[q] = from_float<Y>(h.v[q]);
+            const Vec<X, V> x = load<X, V>((const X *)g.x + r * g.xs + c);
+            Row<V> a = all<V>(g.decay), rest = all<V>(__fsub_rn(1.0f, g.decay));
+            if (g.gate) {
+                const Vec<G, V> z = load<G, V>((const G *)g.gate + r * g.gs + c);
+                if (g.logit) leak_of<G, true, V>(z, a, rest);
+                else leak_of<G, false, V>(z, a, rest);
             }
-            *reinterpret_cast<Vec<Y, V> *>((Y *)g.y + r * g.ys + c) = o;
+            Row<V> u = mul(all<V>(g.scale), widen(x));
+            if (g.complement) u = mul(u, rest);
+            h = fma(a, h, u);
+            store<Y, V>((Y *)g.y + r * g.ys + c, narrow<Y, V>(h));
             if (!again) break;
         }
-        *state = h;
+        store_row<V>(state, h);
     }
 }
 

@@ -111,13 +111,15 @@ snn_status_t check_common(int device, const snn_b200_leaky_t *q, const void *x, 
 struct Plan {
     uint64_t flat, columns;
     uint32_t segments, segment_steps, partials;  // partials: sums of a shared gate's gradient a channel
-    bool crew;
+    uint32_t crew;
     uint64_t maps, states, partial, bytes;
 };
 // Warps that walk whole sequences, or where those would be too few to keep the
 // loads of 148 SMs under way, crews, or where even those are too few, segments
-// (64 steps at least).
-constexpr uint64_t kFewWalks = 148 * 5, kFewCrews = 64, kManyWalks = 148 * 48;
+// (64 steps at least). A crew has 16 warps where it has an SM to itself, else 8
+// (8192 steps, bf16, 128 columns: 104 against 127 us, 256 columns of 4096: 105 against
+// 90 us); 64 columns take 102 us in crews and about 70 in segments.
+constexpr uint64_t kFewWalks = 148 * 5, kFewCrews = 104, kManyWalks = 148 * 48;
 constexpr uint32_t kLeastSegment = 64;
 Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     Plan p = {};
@@ -125,14 +127,14 @@ Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     p.columns = (p.flat + 32 * width - 1) / (32 * width);
     p.segments = 1, p.segment_steps = (uint32_t)q.steps;
     if (p.columns && p.columns < kFewWalks && q.steps >= 2 * kLeastSegment) {
-        p.crew = width <= 2 && p.columns >= kFewCrews;
+        p.crew = width > 2 || p.columns < kFewCrews ? 0 : p.columns <= 148 ? 16 : 8;
         if (!p.crew) {
             const uint64_t want = std::max<uint64_t>(kLeastSegment, q.steps * p.columns / kManyWalks);
             p.segment_steps = (uint32_t)((want + kSteps - 1) / kSteps * kSteps);
             p.segments = (uint32_t)((q.steps + p.segment_steps - 1) / p.segment_steps);
         }
     }
-    p.partials = p.crew ? kCrew : p.segments;
+    p.partials = p.crew ? p.crew : p.segments;
     const auto round = [](uint64_t v) { return (v + 255) / 256 * 256; };
     const uint64_t cut = p.segments > 1 ? p.segments * p.flat : 0;
     p.maps = 0;

@@ -478,24 +478,24 @@ template <int V>
 struct alignas(2 * sizeof(Row<V>)) Map {
     Row<V> A, H;
 };
-template <int V>
+template <int V, uint32_t N>
 struct Crew {
-    Map<V> map[2][kCrew][32];  // of this round and the one before
+    Map<V> map[2][N][32];      // of this round and the one before
     Row<V> state[2][32];       // behind a round
 };
 // Blocks under way or at hand for each warp, as shared memory allows.
-template <int V>
+template <int V, uint32_t N>
 constexpr uint32_t crew_depth(uint32_t slot) {
-    return 3 * kCrew * slot + (uint32_t)sizeof(Crew<V>) <= 227 * 1024 ? 3 : 2;
+    return 3 * N * slot + (uint32_t)sizeof(Crew<V, N>) <= 227 * 1024 ? 3 : 2;
 }
 // The next rounds of a crew's warp: fetch(t0, slot) and work(n, t0, slot) of
 // its block in each; a block behind the last one is only worked on (on = false).
-template <bool Reverse, uint32_t Depth, typename Fetch, typename Work>
+template <bool Reverse, uint32_t N, uint32_t Depth, typename Fetch, typename Work>
 __device__ __forceinline__ void walk_rounds(uint32_t steps, Fetch fetch, Work work) {
     const uint32_t warp = threadIdx.x / 32, blocks = (steps + kSteps - 1) / kSteps;
-    const uint32_t rounds = (blocks + kCrew - 1) / kCrew;
-    const auto at = [&](uint32_t n) { return (Reverse ? blocks - 1 - (n * kCrew + warp) : n * kCrew + warp) * kSteps; };
-    const auto on = [&](uint32_t n) { return n * kCrew + warp < blocks; };
+    const uint32_t rounds = (blocks + N - 1) / N;
+    const auto at = [&](uint32_t n) { return (Reverse ? blocks - 1 - (n * N + warp) : n * N + warp) * kSteps; };
+    const auto on = [&](uint32_t n) { return n * N + warp < blocks; };
 #pragma unroll
     for (uint32_t n = 0; n < Depth - 1; ++n) {
         if (on(n)) fetch(at(n), n);
@@ -514,8 +514,8 @@ __device__ __forceinline__ void walk_rounds(uint32_t steps, Fetch fetch, Work wo
 }
 // Shares a block's map and folds the state before it. The last warp's walk of the
 // round before has left the state there.
-template <int V>
-__device__ __forceinline__ Row<V> crew_state(Crew<V> &c, uint32_t n, const Row<V> &A, const Row<V> &H, const Row<V> &first) {
+template <int V, uint32_t N>
+__device__ __forceinline__ Row<V> crew_state(Crew<V, N> &c, uint32_t n, const Row<V> &A, const Row<V> &H, const Row<V> &first) {
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x & 31, turn = n & 1;
     c.map[turn][warp][lane] = {A, H};
     __syncthreads();
@@ -528,20 +528,20 @@ __device__ __forceinline__ Row<V> crew_state(Crew<V> &c, uint32_t n, const Row<V
     }
     return h;
 }
-template <int V>
-__device__ __forceinline__ void crew_done(Crew<V> &c, uint32_t n, const Row<V> &h) {
-    if (threadIdx.x / 32 + 1 == kCrew) c.state[n & 1][threadIdx.x & 31] = h;
+template <int V, uint32_t N>
+__device__ __forceinline__ void crew_done(Crew<V, N> &c, uint32_t n, const Row<V> &h) {
+    if (threadIdx.x / 32 + 1 == N) c.state[n & 1][threadIdx.x & 31] = h;
 }
 
-template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(kCrew * 32) scan_crew_kernel(const __grid_constant__ Args g) {
+template <typename X, typename G, typename Y, int V, uint32_t N>
+__global__ void __launch_bounds__(N * 32) scan_crew_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
-    __shared__ Crew<V> s_crew;
+    __shared__ Crew<V, N> s_crew;
     after_previous();
     const uint32_t warp = threadIdx.x / 32;
     const Place p = place_of<V>(g, blockIdx.x);
     constexpr uint32_t kX = Feed<X, V>::kBytes, kSlot = kX + Feed<G, V>::kBytes;
-    constexpr uint32_t kDeep = crew_depth<V>(kSlot);
+    constexpr uint32_t kDeep = crew_depth<V, N>(kSlot);
     uint8_t *mine = s_feed + warp * (kDeep * kSlot);
     Feed<X, V> fx;
     Feed<G, V> fz;
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(kCrew * 32) scan_crew_kernel(const __grid_cons
     fz.init(g, g.gate, p, blockIdx.x, g.gb, g.gt);
     const Row<V> first = p.on ? load_state<V>(g.h0, p.i) : all<V>(0.0f);
     Row<V> h = first;
-    walk_rounds<false, kDeep>(
+    walk_rounds<false, N, kDeep>(
         g.steps,
         [&](uint32_t t0, uint32_t slot) {
             fz.fetch(mine + slot * kSlot + kX, t0);
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kCrew * 32) scan_crew_kernel(const __grid_cons
                     H = fma(aj, H, uj);
                 });
             }
-            h = crew_state<V>(s_crew, n, A, H, first);
+            h = crew_state<V, N>(s_crew, n, A, H, first);
             if (on && p.on) {
                 if (g.saved) store_row<V>(saved_at(g, p, t0), h);
                 Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
@@ -590,9 +590,9 @@ __global__ void __launch_bounds__(kCrew * 32) scan_crew_kernel(const __grid_cons
                     }
                 }
             }
-            crew_done<V>(s_crew, n, h);
+            crew_done<V, N>(s_crew, n, h);
         });
-    if (g.h_last && p.on && warp + 1 == kCrew) store_row<V>(g.h_last + p.i, h);
+    if (g.h_last && p.on && warp + 1 == N) store_row<V>(g.h_last + p.i, h);
 }
 
 // ---- gradient ----
@@ -761,16 +761,16 @@ __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const _
     }
 }
 
-template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(kCrew * 32) back_crew_kernel(const __grid_constant__ Args g) {
+template <typename X, typename G, typename Y, int V, uint32_t N>
+__global__ void __launch_bounds__(N * 32) back_crew_kernel(const __grid_constant__ Args g) {
     extern __shared__ __align__(16) uint8_t s_feed[];
-    __shared__ Crew<V> s_crew;
+    __shared__ Crew<V, N> s_crew;
     after_previous();
     const uint32_t warp = threadIdx.x / 32;
     const Place p = place_of<V>(g, blockIdx.x);
     constexpr uint32_t kY = Feed<Y, V>::kBytes, kZ = kY + Feed<G, V>::kBytes, kS = kZ + Feed<X, V>::kBytes,
                        kSlot = kS + kSavedBytes<V>;
-    constexpr uint32_t kDeep = crew_depth<V>(kSlot);
+    constexpr uint32_t kDeep = crew_depth<V, N>(kSlot);
     uint8_t *mine = s_feed + warp * (kDeep * kSlot);
     Feed<X, V> fx;
     Feed<G, V> fz;
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kCrew * 32) back_crew_kernel(const __grid_cons
     const Row<V> first = p.on ? load_state<V>(g.dh_last, p.i) : all<V>(0.0f);
     Row<V> e = first;
     double total[V] = {};
-    walk_rounds<true, kDeep>(
+    walk_rounds<true, N, kDeep>(
         g.steps,
         [&](uint32_t t0, uint32_t slot) {
             fy.fetch(mine + slot * kSlot, t0);
@@ -806,17 +806,17 @@ __global__ void __launch_bounds__(kCrew * 32) back_crew_kernel(const __grid_cons
 #pragma unroll
                 for (int j = (int)kSteps - 1; j >= 0; --j) A = mul(b.a[j], A), b.step(j, live, E);
             }
-            e = crew_state<V>(s_crew, n, A, E, first);
+            e = crew_state<V, N>(s_crew, n, A, E, first);
             if (on) {
                 const Row<V> sum = b.emit(g, p, t0, live, e);
                 if (!b.kEvery)
 #pragma unroll
                     for (int q = 0; q < V; ++q) total[q] += (double)sum[q];
             }
-            crew_done<V>(s_crew, n, e);
+            crew_done<V, N>(s_crew, n, e);
         });
     if (!p.on) return;
-    if (g.dh0 && warp + 1 == kCrew) store_row<V>(g.dh0 + p.i, e);
+    if (g.dh0 && warp + 1 == N) store_row<V>(g.dh0 + p.i, e);
     if (g.partial) {
         const Row<V> sum = Row<V>::of([&](int q) { return (float)total[q]; });
         put_partial(g, p, b.gates, warp, sum);
@@ -914,9 +914,14 @@ cudaError_t start(K kernel, cudaStream_t s, const Args &a, uint64_t grid, uint32
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_scan(cudaStream_t s, const Args &a) {
     constexpr uint32_t slot = Feed<X, V>::kBytes + Feed<G, V>::kBytes;
-    if constexpr (V <= 2)
+    if constexpr (V <= 2) {
+        if (a.crew == 16)
+            return start(scan_crew_kernel<X, G, Y, V, 16>, s, a, a.columns, 16, crew_depth<V, 16>(slot) * slot,
+                         sizeof(Crew<V, 16>));
         if (a.crew)
-            return start(scan_crew_kernel<X, G, Y, V>, s, a, a.columns, kCrew, crew_depth<V>(slot) * slot, sizeof(Crew<V>));
+            return start(scan_crew_kernel<X, G, Y, V, 8>, s, a, a.columns, 8, crew_depth<V, 8>(slot) * slot,
+                         sizeof(Crew<V, 8>));
+    }
     const uint64_t grid = ((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps;
     if (a.segments > 1) {
         cudaError_t e = start(scan_kernel<X, G, Y, V, true>, s, a, grid, kWarps, kDepth * slot);
@@ -928,7 +933,12 @@ cudaError_t launch_scan(cudaStream_t s, const Args &a) {
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_back(cudaStream_t s, const Args &a) {
     constexpr uint32_t maps = Feed<G, V>::kBytes + Feed<Y, V>::kBytes, slot = maps + Feed<X, V>::kBytes + kSavedBytes<V>;
-    if (a.crew) return start(back_crew_kernel<X, G, Y, V>, s, a, a.columns, kCrew, crew_depth<V>(slot) * slot, sizeof(Crew<V>));
+    if (a.crew == 16)
+        return start(back_crew_kernel<X, G, Y, V, 16>, s, a, a.columns, 16, crew_depth<V, 16>(slot) * slot,
+                     sizeof(Crew<V, 16>));
+    if (a.crew)
+        return start(back_crew_kernel<X, G, Y, V, 8>, s, a, a.columns, 8, crew_depth<V, 8>(slot) * slot,
+                     sizeof(Crew<V, 8>));
     const uint64_t grid = ((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps;
     if (a.segments > 1) {
         cudaError_t e = start(back_kernel<X, G, Y, V, true>, s, a, grid, kWarps, kDepth * maps);

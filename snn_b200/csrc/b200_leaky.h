@@ -10,7 +10,6 @@ namespace leaky {
 constexpr uint32_t kSteps = SNN_B200_LEAKY_BLOCK;  // steps worked on at a time, and of a saved state
 constexpr uint32_t kWarps = 4;                     // of a CTA
 constexpr uint32_t kDepth = 4;                     // blocks of steps under way or at hand
-constexpr uint32_t kCrew = 16;                     // warps of a crew
 
 struct Args {
     uint64_t flat;  // batch * channels
@@ -26,7 +25,7 @@ struct Args {
     int wide;                          // rows of x, gate and dy can be read in pieces of 16 bytes
     uint32_t columns;                  // warps' widths across the channels
     uint32_t segments, segment_steps;  // along the steps
-    int crew;                          // a CTA of kCrew warps a column
+    uint32_t crew;                     // a CTA of 16 or 8 warps a column, 0: none
     float2 *maps;                      // [segments][flat], (A, H) of h -> A h + H
     float *states;                     // [segments][flat], before each (backward: behind each)
     float *partial;                    // backward: sums of a shared gate's gradient, [segments, or warps of a crew][flat]

@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(N * 32) back_crew_kernel(const __grid_constant
 // it, which also do the later rows that name it, in order. To know, every CTA
 // looks through the slots once, for all of its rows at a time.
 template <typename X, typename G, typename Y, int V>
-__global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
+__global__ void __launch_bounds__(256, 4) step_kernel(StepArgs g) {
     __shared__ uint32_t s_before[8], s_after[8];  // rows named before, rows named again
     const uint32_t across = 256 / g.rows, mine = threadIdx.x / across;
     const uint32_t row = blockIdx.x * g.rows + mine;
@@ -842,13 +842,20 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
             const uint32_t n = blockIdx.x * g.rows + r;
             named[r] = r < g.rows && n < g.batch ? g.slots[n] : -1;
         }
-        for (uint32_t n = threadIdx.x; n < g.batch; n += 256) {
-            const int32_t s = g.slots[n];
-            if (s < 0) continue;
+        for (uint32_t n0 = threadIdx.x; n0 < g.batch; n0 += 8 * 256) {
+            int32_t s[8];
 #pragma unroll
-            for (uint32_t r = 0; r < 8; ++r) {
-                const uint32_t of = blockIdx.x * g.rows + r;
-                if (s == named[r] && n != of) (n < of ? s_before : s_after)[r] = 1u;
+            for (uint32_t i = 0; i < 8; ++i) s[i] = n0 + i * 256 < g.batch ? g.slots[n0 + i * 256] : -1;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                bool hit = false;
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) hit |= s[i] == named[r];
+                if (!hit || s[i] < 0) continue;
+                for (uint32_t r = 0; r < g.rows; ++r) {
+                    const uint32_t n = n0 + i * 256, of = blockIdx.x * g.rows + r;
+                    if (of < g.batch && s[i] == g.slots[of] && n != of) (n < of ? s_before : s_after)[r] = 1u;
+                }
             }
         }
         __syncthreads();
@@ -858,30 +865,59 @@ __global__ void __launch_bounds__(256) step_kernel(StepArgs g) {
     const bool again = g.slots && g.batch > 1 && s_after[mine];
     const int64_t slot = g.slots ? (int64_t)g.slots[row] : (int64_t)row;
     const bool padding = slot < 0 || slot >= (int64_t)g.slot_count;
-    for (uint64_t c = ((uint64_t)blockIdx.y * across + threadIdx.x % across) * V; c < g.channels;
-         c += (uint64_t)gridDim.y * across * V) {
-        if (padding) {
-            store<Y, V>((Y *)g.y + row * g.ys + c, Vec<Y, V>{});
-            continue;
+    const uint64_t c0 = ((uint64_t)blockIdx.y * across + threadIdx.x % across) * V, jump = (uint64_t)gridDim.y * across * V;
+    Y *y = (Y *)g.y + row * g.ys;
+    if (padding) {
+        for (uint64_t c = c0; c < g.channels; c += jump) store<Y, V>(y + c, Vec<Y, V>{});
+        return;
+    }
+    float *state = g.pool + slot * g.ps;
+    const auto one = [&](const Vec<X, V> &x, const Vec<G, V> &z, Row<V> &h) {
+        Row<V> a = all<V>(g.decay), rest = all<V>(__fsub_rn(1.0f, g.decay));
+        if (g.gate) {
+            if (g.logit) leak_of<G, true, V>(z, a, rest);
+            else leak_of<G, false, V>(z, a, rest);
         }
-        float *state = g.pool + slot * g.ps + c;
-        Row<V> h = load_row<V>(state);
-        for (uint32_t r = row; r < g.batch; ++r) {
-            if (r != row && g.slots[r] != (int32_t)slot) continue;
-            const Vec<X, V> x = load<X, V>((const X *)g.x + r * g.xs + c);
-            Row<V> a = all<V>(g.decay), rest = all<V>(__fsub_rn(1.0f, g.decay));
-            if (g.gate) {
-                const Vec<G, V> z = load<G, V>((const G *)g.gate + r * g.gs + c);
-                if (g.logit) leak_of<G, true, V>(z, a, rest);
-                else leak_of<G, false, V>(z, a, rest);
-            }
-            Row<V> u = mul(all<V>(g.scale), widen(x));
-            if (g.complement) u = mul(u, rest);
-            h = fma(a, h, u);
-            store<Y, V>((Y *)g.y + r * g.ys + c, narrow<Y, V>(h));
-            if (!again) break;
+        Row<V> u = mul(all<V>(g.scale), widen(x));
+        if (g.complement) u = mul(u, rest);
+        h = fma(a, h, u);
+        return narrow<Y, V>(h);
+    };
+    const X *xs = (const X *)g.x;
+    const G *zs = (const G *)g.gate;
+    if (again) {
+        for (uint64_t c = c0; c < g.channels; c += jump) {
+            Row<V> h = load_row<V>(state + c);
+            for (uint32_t r = row; r < g.batch; ++r)
+                if (g.slots[r] == (int32_t)slot)
+                    store<Y, V>((Y *)g.y + r * g.ys + c,
+                                one(load<X, V>(xs + r * g.xs + c), zs ? load<G, V>(zs + r * g.gs + c) : Vec<G, V>{}, h));
+            store_row<V>(state + c, h);
         }
-        store_row<V>(state, h);
+        return;
+    }
+    xs += row * g.xs;
+    if (zs) zs += row * g.gs;
+    constexpr uint32_t kAtOnce = 4;  // pieces whose loads are under way together
+    for (uint64_t c = c0; c < g.channels; c += kAtOnce * jump) {
+        Vec<X, V> x[kAtOnce];
+        Vec<G, V> z[kAtOnce];
+        Row<V> h[kAtOnce];
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+            const uint64_t at = c + i * jump;
+            if (at >= g.channels) break;
+            x[i] = load<X, V>(xs + at);
+            z[i] = zs ? load<G, V>(zs + at) : Vec<G, V>{};
+            h[i] = load_row<V>(state + at);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+            const uint64_t at = c + i * jump;
+            if (at >= g.channels) break;
+            store<Y, V>(y + at, one(x[i], z[i], h[i]));
+            store_row<V>(state + at, h[i]);
+        }
     }
 }
 

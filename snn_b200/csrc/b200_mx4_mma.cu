@@ -214,7 +214,9 @@ constexpr uint32_t kNoValue = 0x7fffffffu;
 // rows, and the instructions read x from both. What a CTA loads for a tile is
 // the bound (about 11 TB/s come out of L2 for all SMs; 256 rows of x a CTA took
 // 309 us at 8192x8192x8192), and this halves x's part of it.
-constexpr uint32_t kPairN = 256, kPairStages = 6, kPairThreads = 384;
+constexpr uint32_t kPairN = 256, kPairStages = 6;
+constexpr uint32_t kReaders = 16;  // warps that read and write accumulators: four share the lanes, kReaders / 4 the columns
+constexpr uint32_t kPairThreads = 128 + kReaders * 32, kReadN = kPairN / (kReaders / 4);
 constexpr uint32_t kPairX = 128 * kStageBytes, kPairW = kRows * kStageBytes;
 // A stage: weights, x, the scales of the CTA's weights, of all of x's rows.
 constexpr uint32_t kPairAtX = kPairW, kPairAtWScales = kPairW + kPairX, kPairAtXScales = kPairAtWScales + 2 * kScaleTile;
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < kPairStages; ++s) bar_init(&s_full[s], 1), bar_init(&s_empty[s], 1);
         bar_init(&s_ready, 1);
-        bar_init(&s_free, 16);  // the warps that read accumulators, of both CTAs
+        bar_init(&s_free, 2 * kReaders);  // of both CTAs
         tma::bar_init_done();
     }
     if (warp == 0) {
@@ -323,32 +325,31 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
         }
     } else if (warp >= 4) {
-        // Four warps share the lanes, two share the columns.
-        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+        const uint32_t quarter = warp & 3, part = (warp - 4) / 4;
         const uint32_t free = in_cta(smem_of(&s_free), 0);
         uint32_t count = 0;
         for (uint32_t tile = pair; tile < tiles; tile += pairs, ++count) {
             const uint32_t j = tile % p.tiles_n * 256 + rank * 128 + quarter * 32 + lane;
-            const uint32_t i0 = tile / p.tiles_n * kPairN + half * (kPairN / 2);
+            const uint32_t i0 = tile / p.tiles_n * kPairN + part * kReadN;
             const float bias = p.bias && j < p.n ? p.bias[j] : 0.0f;
             ok = ok && bar_wait(&s_ready, count & 1);
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
-            float v[kPairN / 2 / 16][16];
+            float v[kReadN / 16][16];
 #pragma unroll
-            for (uint32_t c = 0; c < kPairN / 2 / 16; ++c)
-                read_columns(tmem + (quarter * 32 << 16) + half * (kPairN / 2) + c * 16, v[c]);
+            for (uint32_t c = 0; c < kReadN / 16; ++c)
+                read_columns(tmem + (quarter * 32 << 16) + part * kReadN + c * 16, v[c]);
             read_done();
 #pragma unroll
-            for (uint32_t c = 0; c < kPairN / 2 / 16; ++c) settle(v[c]);
+            for (uint32_t c = 0; c < kReadN / 16; ++c) settle(v[c]);
             fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(free) : "memory");
             if (j < p.n) {
                 T *to = (T *)p.out + (int64_t)i0 * p.row_stride + j;
-                const uint32_t rows = i0 < p.m ? min(p.m - i0, kPairN / 2) : 0;
+                const uint32_t rows = i0 < p.m ? min(p.m - i0, kReadN) : 0;
 #pragma unroll
-                for (uint32_t c = 0; c < kPairN / 2 / 16; ++c)
+                for (uint32_t c = 0; c < kReadN / 16; ++c)
 #pragma unroll
                     for (uint32_t q = 0; q < 16; ++q) {
                         if (c * 16 + q < rows)

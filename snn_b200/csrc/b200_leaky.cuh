@@ -170,11 +170,13 @@ __device__ __forceinline__ void leak_of(const Vec<G, V> &z, Row<V> &a, Row<V> &r
             }
         });
         const Row<V> one = add(t, all<V>(1.0f));
-        const Row<V> r = Row<V>::of([&](int q) {
+        const Row<V> near = Row<V>::of([&](int q) {
             float i;
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(i) : "f"(one[q]));
             return i;
         });
+        // A step of Newton's, as an error of the gate grows by 1 / (1 - a) on its way into the state.
+        const Row<V> r = fma(near, fma(mul(one, all<V>(-1.0f)), near, all<V>(1.0f)), near);
         const Row<V> s = mul(t, r);
         a = Row<V>::of([&](int q) { return f[q] >= 0.0f ? r[q] : s[q]; });
         rest = Row<V>::of([&](int q) { return f[q] >= 0.0f ? s[q] : r[q]; });

@@ -16,10 +16,11 @@ __device__ __forceinline__ void store_any(void *p, int dtype, int64_t i, float v
 // 128 rows x 4 blocks: the unit of the packers' CTAs, and one tile of scales.
 constexpr uint32_t kTileRows = 128, kTileCols = 128;
 
-// Rows of neighbouring elements that can be read 16 bytes at a time. Lanes lie
-// across a row, each with the elements of one 16-byte load, and find their
-// block's largest magnitude by shuffles, so loads and stores are whole runs.
-template <typename T>
+// Rows of neighbouring elements. Lanes lie across a row, each with 16 bytes of
+// it, and find their block's largest magnitude by shuffles, so loads and
+// stores are whole runs. Rows that do not start on 16 bytes are read element
+// by element, out of lines that the lanes share in L1.
+template <typename T, bool Aligned>
 __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, uint32_t rows, uint32_t cols, int64_t rs,
                                                                 uint8_t *codes, uint8_t *scales, uint32_t tiles) {
     constexpr uint32_t kOwn = 16 / sizeof(T), kAcross = kTileCols / kOwn;  // elements of a lane, lanes on a row
@@ -36,7 +37,7 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, ui
 #pragma unroll
         for (uint32_t i = 0; i < kHeld; ++i) {
             const uint32_t r = r0 + (pass + i) * kRowsAtOnce + first;
-            if (r < rows && c < cols) v[i] = load_piece(src + (int64_t)r * rs + c, cols - c);
+            if (r < rows && c < cols) v[i] = load_piece<Aligned>(src + (int64_t)r * rs + c, cols - c);
             else v[i] = Piece<T>{};
         }
 #pragma unroll
@@ -56,8 +57,8 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, ui
             reinterpret_cast<const uint4 *>(s_scales)[threadIdx.x];
 }
 
-// Any strides: a thread a block, lanes along the rows, so a transposed source
-// is read in whole runs too.
+// Other strides: a thread a block, lanes along the rows, so a transposed source
+// is read in whole runs.
 template <typename T>
 __global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uint32_t rows, uint32_t cols, int64_t rs,
                                                                int64_t cs, uint8_t *codes, uint8_t *scales,
@@ -90,47 +91,58 @@ __global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uin
             reinterpret_cast<const uint4 *>(s_scales)[threadIdx.x];
 }
 
-// A thread 8 elements: 4 bytes of codes, written as whole 16-byte pieces where
-// the rows allow it.
-template <typename T>
+// A CTA 16 rows of 512 elements at a time, a thread 8 elements (4 bytes of
+// codes) of four rows. Whole: they are written in 16-byte pieces; else they go
+// through shared memory and leave element by element, lanes side by side, so
+// that rows that do not start on 16 bytes are written in whole runs too.
+template <typename T, bool Whole>
 __global__ void __launch_bounds__(256) mx4_dequantize_kernel(const uint8_t *codes, const uint8_t *scales, uint32_t rows,
-                                                             uint32_t cols, uint32_t tiles, T *dst, int64_t rs,
-                                                             bool pieces) {
+                                                             uint32_t cols, uint32_t tiles, T *dst, int64_t rs) {
+    __shared__ __align__(16) T s_row[Whole ? 1 : 16][Whole ? 8 : 512];
     const uint64_t pitch = blocks_of(cols) * 16;
-    const uint32_t c = (blockIdx.x * 64 + threadIdx.x % 64) * 8;
+    const uint32_t first = blockIdx.x * 512, lane = threadIdx.x % 64, c = first + lane * 8, b = c / kBlock;
     after_previous();
-    if (c >= cols) return;
-    const uint32_t b = c / kBlock;
-    for (uint64_t r0 = (uint64_t)blockIdx.y * 16 + threadIdx.x / 64; r0 < rows; r0 += (uint64_t)gridDim.y * 16) {
-        uint32_t w[4], s[4];
+    for (uint64_t base = (uint64_t)blockIdx.y * 16; base < rows; base += (uint64_t)gridDim.y * 16) {
+        const uint64_t r0 = base + threadIdx.x / 64;
+        uint32_t w[4] = {}, s[4] = {};
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             const uint64_t r = r0 + 4 * i;
-            w[i] = s[i] = 0;
-            if (r < rows) {
-                w[i] = *reinterpret_cast<const uint32_t *>(codes + r * pitch + c / 2);
-                s[i] = scales[512 * ((r / kTileRows) * tiles + b / 4) + scale_slot((uint32_t)(r % kTileRows), b % 4)];
-            }
+            if (r >= rows || c >= cols) continue;
+            w[i] = *reinterpret_cast<const uint32_t *>(codes + r * pitch + c / 2);
+            s[i] = scales[512 * ((r / kTileRows) * tiles + b / 4) + scale_slot((uint32_t)(r % kTileRows), b % 4)];
         }
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             const uint64_t r = r0 + 4 * i;
-            if (r >= rows) continue;
             float v[8];
             decode8(w[i], scale_value(s[i]), v);
-            T *to = dst + (int64_t)r * rs + c;
-            if (pieces && c + 8 <= cols) {
-                Eight<T> o;
+            Eight<T> o;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) o.v[q] = from_float<T>(v[q]);
+            for (int q = 0; q < 8; ++q) o.v[q] = from_float<T>(v[q]);
+            T *to = Whole ? dst + (int64_t)r * rs + c : &s_row[threadIdx.x / 64 + 4 * i][lane * 8];
+            if (Whole && (r >= rows || c >= cols)) continue;
+            if (!Whole || c + 8 <= cols) {
 #pragma unroll
                 for (uint32_t q = 0; q < sizeof(T) / 2; ++q)
                     reinterpret_cast<uint4 *>(to)[q] = reinterpret_cast<const uint4 *>(&o)[q];
             } else {
 #pragma unroll
                 for (uint32_t q = 0; q < 8; ++q)
-                    if (c + q < cols) to[q] = from_float<T>(v[q]);
+                    if (c + q < cols) to[q] = o.v[q];
             }
+        }
+        if constexpr (!Whole) {
+            __syncthreads();
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint64_t r = r0 + 4 * i;
+                if (r >= rows) break;
+                T *to = dst + (int64_t)r * rs + first;
+#pragma unroll
+                for (uint32_t q = 0; q < 8; ++q)
+                    if (first + q * 64 + lane < cols) to[q * 64 + lane] = s_row[threadIdx.x / 64 + 4 * i][q * 64 + lane];
+            }
+            __syncthreads();
         }
     }
 }
@@ -176,7 +188,9 @@ void quantize_as(cudaStream_t s, const void *src, uint64_t rows, uint64_t cols, 
         const T *from = (const T *)src + (int64_t)r0 * rs;
         uint8_t *c = codes + code_bytes(r0, cols), *x = scales + scale_bytes(r0, cols);
         if (cs == 1 && aligned_to(src, 16) && rs * (int64_t)sizeof(T) % 16 == 0)
-            launch_early(mx4_quantize_rows_kernel<T>, grid, 256, 0, s, 1, from, n, cols, rs, c, x, tiles);
+            launch_early(mx4_quantize_rows_kernel<T, true>, grid, 256, 0, s, 1, from, n, cols, rs, c, x, tiles);
+        else if (cs == 1)
+            launch_early(mx4_quantize_rows_kernel<T, false>, grid, 256, 0, s, 1, from, n, cols, rs, c, x, tiles);
         else
             launch_early(mx4_quantize_any_kernel<T>, grid, 512, 0, s, 1, from, n, cols, rs, cs, c, x, tiles);
     }
@@ -196,8 +210,9 @@ void dequantize_as(cudaStream_t s, const void *codes, const void *scales, uint64
                    int64_t rs) {
     const uint64_t high = (rows + 15) / 16;
     const dim3 grid((uint32_t)((cols + 511) / 512), (uint32_t)(high < 65535 ? high : 65535));
-    launch_early(mx4_dequantize_kernel<T>, grid, 256, 0, s, 1, (const uint8_t *)codes, (const uint8_t *)scales, rows, cols,
-                 scale_tiles(cols), (T *)dst, rs, aligned_to(dst, 16) && rs * (int64_t)sizeof(T) % 16 == 0);
+    const bool whole = aligned_to(dst, 16) && rs * (int64_t)sizeof(T) % 16 == 0;
+    launch_early(whole ? mx4_dequantize_kernel<T, true> : mx4_dequantize_kernel<T, false>, grid, 256, 0, s, 1,
+                 (const uint8_t *)codes, (const uint8_t *)scales, rows, cols, scale_tiles(cols), (T *)dst, rs);
 }
 
 cudaError_t enqueue_matmul(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, const float *bias,

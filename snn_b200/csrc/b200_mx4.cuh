@@ -99,11 +99,12 @@ struct Piece<Spike> {
         if (on) *reinterpret_cast<uint2 *>(to) = make_uint2(four(raw.x) | four(raw.y) << 16, four(raw.z) | four(raw.w) << 16);
     }
 };
-// The piece at p, of which n elements are left in the row; Again: others read it too.
-template <bool Again = false, typename T>
+// The piece at p, of which n elements are left in the row. Aligned: p is a
+// multiple of 16 bytes. Again: others read it too.
+template <bool Aligned, bool Again = false, typename T>
 __device__ __forceinline__ Piece<T> load_piece(const T *p, uint32_t n) {
     Piece<T> v;
-    if (n >= Piece<T>::kOwn) {
+    if (Aligned && n >= Piece<T>::kOwn) {
         v.raw = Again ? *reinterpret_cast<const uint4 *>(p) : __ldcs(reinterpret_cast<const uint4 *>(p));
     } else {
         __align__(16) T e[Piece<T>::kOwn];

@@ -406,7 +406,7 @@ __device__ __forceinline__ void pack_stage(const Problem &p, uint32_t slot, uint
 #pragma unroll
             for (uint32_t q = 0; q < kPieces; ++q) {
                 const uint32_t e = c + q * Piece<X>::kOwn;
-                v[h][q] = r < p.m && e < p.k ? load_piece<true>((const X *)p.x + r * p.x_stride + e, p.k - e) : Piece<X>{};
+                v[h][q] = r < p.m && e < p.k ? load_piece<true, true>((const X *)p.x + r * p.x_stride + e, p.k - e) : Piece<X>{};
             }
         }
 #pragma unroll

@@ -114,6 +114,8 @@ Tensor state(const Tensor &t, at::IntArrayRef shape, const char *text) {
     require(t.scalar_type() == at::kFloat && t.sizes() == shape, text);
     return t.contiguous();
 }
+// A dimension's stride, or `single` where the dimension is one long and its stride says nothing.
+int64_t stride(const Tensor &t, int64_t d, int64_t single) { return t.size(d) > 1 ? t.stride(d) : single; }
 // With neighbouring elements along the last dimension.
 Tensor rows(const Tensor &t) { return t.size(-1) > 1 && t.stride(-1) != 1 ? t.contiguous() : t; }
 
@@ -227,13 +229,15 @@ struct Sequence {
     bool every = false;
 
     // x, gate, decay, lengths, logit, complement, input_scale from argument i on.
-    Sequence(const Args &a, int i) : x(a.tensor(i)), gate(a.tensor(i + 1, true)), lengths(a.tensor(i + 3, true)) {
+    // A gate expanded over the sequences or the steps is read where it is; for
+    // its gradient (whole) it becomes an array with an element for each of them.
+    Sequence(const Args &a, int i, bool whole) : x(a.tensor(i)), gate(a.tensor(i + 1, true)), lengths(a.tensor(i + 3, true)) {
         dev = shared_device(x, gate, lengths);
         require(x.dim() == 3, "leaky: [batch, steps, channels] expected");
         x = rows(x);
         q.batch = x.size(0), q.steps = x.size(1), q.channels = x.size(2);
         q.x_dtype = code(x);
-        q.x_batch_stride = x.stride(0), q.x_step_stride = x.stride(1);
+        q.x_batch_stride = stride(x, 0, 0), q.x_step_stride = stride(x, 1, 0);
         q.logit = a.flag(i + 4), q.complement = a.flag(i + 5), q.input_scale = (float)a.number(i + 6);
         require(gate.defined() != !a.none(i + 2), "leaky: either a gate array or a decay is needed");
         if (gate.defined()) {
@@ -242,8 +246,11 @@ struct Sequence {
                         (d < 3 || gate.size(1) == x.size(1)),
                     "leaky: a gate of shape [channels], [batch, channels] or [batch, steps, channels] expected");
             gate = rows(gate);
+            const int64_t c = x.size(2) ? x.size(2) : 1;  // of a dimension that is one long: not shared
+            if (whole && d > 1 && (stride(gate, 0, c) == 0 || (d > 2 && stride(gate, 1, c) == 0)))
+                gate = gate.clone(at::MemoryFormat::Contiguous);
             q.gate_dtype = code(gate);
-            q.gate_batch_stride = d > 1 ? gate.stride(0) : 0, q.gate_step_stride = d > 2 ? gate.stride(1) : 0;
+            q.gate_batch_stride = d > 1 ? stride(gate, 0, c) : 0, q.gate_step_stride = d > 2 ? stride(gate, 1, c) : 0;
             every = q.gate_step_stride != 0;
         } else {
             q.decay = (float)a.number(i + 2);
@@ -263,7 +270,7 @@ struct Sequence {
 
 // (x, gate, decay, lengths, logit, complement, input_scale, h0, dtype, save)
 PyObject *scan(Args a) {
-    Sequence s(a, 0);
+    Sequence s(a, 0, false);
     const int64_t b = s.x.size(0), c = s.x.size(2);
     const Tensor given = a.tensor(7, true);
     if (given.defined()) shared_device(s.x, given);
@@ -284,7 +291,7 @@ PyObject *scan(Args a) {
 
 // (x, gate, decay, lengths, logit, complement, input_scale, dy, saved, dh_last)
 PyObject *scan_backward(Args a) {
-    Sequence s(a, 0);
+    Sequence s(a, 0, true);
     const int64_t b = s.x.size(0), c = s.x.size(2);
     Tensor dy = a.tensor(7);
     const Tensor saved = a.tensor(8), given = a.tensor(9, true);
@@ -304,7 +311,7 @@ PyObject *scan_backward(Args a) {
         dgate = s.gate.dim() > 1 ? empty({b, c}, at::kFloat, s.x) : empty({c}, at::kFloat, s.x);
         q.dgate_batch_stride = q.gate_batch_stride ? c : 0;
     }
-    q.y_dtype = code(dy), q.dy_batch_stride = dy.stride(0), q.dy_step_stride = dy.stride(1);
+    q.y_dtype = code(dy), q.dy_batch_stride = stride(dy, 0, 0), q.dy_step_stride = stride(dy, 1, 0);
     q.dx_batch_stride = dx.stride(0), q.dx_step_stride = dx.stride(1);
     snn_size_t need;
     const Tensor ws = s.workspace(&need);
@@ -334,7 +341,7 @@ PyObject *step(Args a) {
         require((d == 1 || (d == 2 && gate0.size(0) == b)) && gate0.size(-1) == c,
                 "leaky_step: a gate of shape [channels] or [batch, channels] expected");
         gate = rows(gate0);
-        gate_stride = d == 2 ? gate.stride(0) : 0, gate_type = code(gate);
+        gate_stride = d == 2 ? stride(gate, 0, c ? c : 1) : 0, gate_type = code(gate);
     }
     if (slots.defined())
         require(slots.scalar_type() == at::kInt && slots.dim() == 1 && slots.size(0) == b && slots.is_contiguous(),

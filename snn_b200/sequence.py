@@ -134,8 +134,9 @@ def leaky_scan_backward(dy, x, gate=None, saved=None, *, dh_last=None, decay: fl
                         logit: bool = False, complement: bool = False, input_scale: float = 1.0):
     """The gradients (dx, dgate, dh0) of leaky_scan from those of its outputs:
     dy (h's type) and dh_last (None: zero); `saved` is what leaky_scan(...,
-    save=True) returned for the same inputs. dgate is shaped like the gate,
-    float32 where the gate is shared over the steps, None without a gate."""
+    save=True) returned for the same inputs. dgate is shaped like the gate (an
+    expanded gate's has an element for each of its own), float32 for a gate of
+    [channels] or [batch, channels], None without a gate."""
     return (_OPS or _ops()).scan_backward(x, gate, decay, lengths, logit, complement, input_scale, dy, saved, dh_last)
 
 

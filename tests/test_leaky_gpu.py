@@ -158,13 +158,49 @@ def test_many_sequences_take_the_same_values():
 
 
 @pytest.mark.parametrize("t", [1, 40, 1500])
-def test_gates_shared_over_sequences(t):
-    p = Problem(3, t, 50, "bf16", "shared", "bf16", None, True, True, seed=7)
-    p.verify(gradient=False)
-    _, _, saved = p.forward(save=True)
-    with pytest.raises(sb.SnnError) as e:
-        p.backward(saved)
-    assert e.value.status == sb.SNN_ERR_UNSUPPORTED
+def test_gates_expanded_over_sequences_or_steps(t):
+    """An expanded gate is read where it is; its gradient has an element for each of its own."""
+    Problem(3, t, 50, "bf16", "shared", "bf16", None, True, True, seed=7).verify()
+    for shape in ((3, 1, 50), (1, 1, 50)):
+        p = Problem(3, t, 50, "f32", "step", logit=True, seed=7)
+        p.gate = p.leak(True, *shape).cuda().expand(3, t, 50)
+        p.verify()
+    p = Problem(3, t, 50, "f32", "sequence", logit=True, seed=7)
+    p.gate = p.leak(True, 1, 50).cuda().expand(3, 50)
+    p.verify()
+
+
+def test_dependent_calls_without_a_wait():
+    """Kernels that start while their predecessors end still wait for what those
+    write: a chain of calls, each on the last one's results, against the same
+    chain with a wait after every call."""
+    g = torch.Generator().manual_seed(3)
+    w = [sb.mx4_quantize(torch.randn(256, 256, generator=g).cuda() / 16) for _ in range(2)]
+    z = torch.randn(2, 300, 256, generator=g).cuda()
+    start = torch.randn(2, 300, 256, generator=g).cuda()
+
+    def chain(wait):
+        x, pool = start, torch.zeros(2, 256, device="cuda")
+        for i in range(6):
+            for f in (lambda: sb.mx4_linear(x, w[i % 2]), lambda: sb.leaky_scan(x, z, logit=True, complement=True)[0],
+                      lambda: sb.mx4_dequantize(sb.mx4_quantize(x.view(-1, 256))).view(2, 300, 256),
+                      lambda: sb.mx4_linear(x[:, :7], w[0])):
+                out = f()
+                if wait:
+                    torch.cuda.synchronize()
+                if out.shape == x.shape:
+                    x = out
+            y, last, saved = sb.leaky_scan(x, z, logit=True, save=True)
+            x, dz, _ = sb.leaky_scan_backward(y, x, z, saved, logit=True)
+            x = x / x.abs().amax()
+            sb.leaky_step(out[:, 0], None, pool, decay=0.5)
+            if wait:
+                torch.cuda.synchronize()
+        return x, dz, pool
+
+    want = chain(True)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
 
 
 def test_extreme_gates_and_inputs():

@@ -11,35 +11,42 @@ namespace {
 // ---- states between segments ----
 // states[s] = the state before segment s, folded in order from `first` (or
 // zero) and the maps of the segments before it (backward: behind it). A CTA takes
-// 32 channels; each of its warps composes the maps of one run of segments,
-// folds those of the runs before onto the first state, and walks its run again.
-constexpr uint32_t kCarryWarps = 16;
+// 32 channels; each of its warps composes the maps of one run of segments, folds
+// those of the runs before onto the first state, and walks its run again. Runs of
+// up to kHeld maps stay in registers, all of them under way at once.
+constexpr uint32_t kCarryWarps = 32, kHeld = 16;
 __global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *maps, uint32_t segments, uint64_t flat,
                                                                  const float *first, float *states, bool back) {
     __shared__ float2 s_run[kCarryWarps][32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     const uint64_t i = (uint64_t)blockIdx.x * 32 + lane;
     const uint32_t run = (segments + kCarryWarps - 1) / kCarryWarps;
-    const uint32_t from = min(segments, warp * run), to = min(segments, from + run);
+    const uint32_t from = min(segments, warp * run), to = i < flat ? min(segments, from + run) : from;
     const auto at = [&](uint32_t n) { return (uint64_t)(back ? segments - 1 - n : n) * flat + i; };
     after_previous();
-    float2 m = make_float2(1.0f, 0.0f);
-    if (i < flat)
-#pragma unroll 8
-        for (uint32_t n = from; n < to; ++n) {
-            const float2 v = maps[at(n)];
-            m = make_float2(__fmul_rn(v.x, m.x), __fmaf_rn(v.x, m.y, v.y));
-        }
+    float2 m = make_float2(1.0f, 0.0f), held[kHeld];
+    for (uint32_t n0 = from; n0 < to; n0 += kHeld) {
+#pragma unroll
+        for (uint32_t n = 0; n < kHeld; ++n) held[n] = n0 + n < to ? maps[at(n0 + n)] : make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (uint32_t n = 0; n < kHeld; ++n)
+            m = make_float2(__fmul_rn(held[n].x, m.x), __fmaf_rn(held[n].x, m.y, held[n].y));
+    }
     s_run[warp][lane] = m;
+    float h = i < flat && first ? first[i] : 0.0f;
     __syncthreads();
     if (i >= flat) return;
-    float h = first ? first[i] : 0.0f;
     for (uint32_t w = 0; w < warp; ++w) h = __fmaf_rn(s_run[w][lane].x, h, s_run[w][lane].y);
-#pragma unroll 8
-    for (uint32_t n = from; n < to; ++n) {
-        const float2 v = maps[at(n)];
-        states[at(n)] = h;
-        h = __fmaf_rn(v.x, h, v.y);
+    for (uint32_t n0 = from; n0 < to; n0 += kHeld) {
+        if (run > kHeld)
+#pragma unroll
+            for (uint32_t n = 0; n < kHeld; ++n) held[n] = n0 + n < to ? maps[at(n0 + n)] : make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (uint32_t n = 0; n < kHeld; ++n)
+            if (n0 + n < to) {
+                states[at(n0 + n)] = h;
+                h = __fmaf_rn(held[n].x, h, held[n].y);
+            }
     }
 }
 

@@ -159,14 +159,14 @@ __device__ __forceinline__ void leak_of(const Vec<G, V> &z, Row<V> &a, Row<V> &r
         rest = fma(a, all<V>(-1.0f), all<V>(1.0f));
     } else {
         const Row<V> f = widen(z);
+        const Row<V> m = sizeof(G) == 2 ? mul(f, all<V>(1.44269504f)) : f;
         const Row<V> t = Row<V>::of([&](int q) {
-            const float m = fabsf(f[q]);
             if constexpr (sizeof(G) == 2) {
                 float e;
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(m, -1.44269504f)));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-fabsf(m[q])));
                 return e;
             } else {
-                return expf(-m);
+                return expf(-fabsf(m[q]));
             }
         });
         const Row<V> one = add(t, all<V>(1.0f));

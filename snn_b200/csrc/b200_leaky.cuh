@@ -5,22 +5,22 @@
 // thread each V of them, with the state in registers, so every access is one
 // run of 32 V elements. What limits it is how much it keeps under way: the next
 // blocks of kSteps steps are copied to shared memory (cp.async) while one is
-// worked on; a thread reads only what it copied itself, so nothing waits for
-// another warp.
+// worked on. 1024 sequences of 64 steps and 1024 channels, bf16 with logits: 66 us
+// (6.1 TB/s), the gradient 112 us (6.3 TB/s).
 //
 // Fewer channels than keep the GPU busy that way are walked by crews: the warps
 // of a CTA take the next blocks of one column side by side. Steps compose as
 // affine maps h -> A h + H; each warp shares its block's map, folds those before
-// its own onto the state, and then walks its block.
+// its own onto the state, and then walks its block. 4 x 8192 x 2048 (128 columns):
+// 104 us, the gradient 155 us; the SMs' issue slots are the bound, with 30 and 49
+// instructions an element.
 //
-// Where even crews are too few, the steps are cut into
-// segments: one kernel walks each segment for its map, one folds them in order
-// into the state before each segment, and the walk itself then starts
-// everywhere at once. The inputs are
-// read twice; the second walk goes through the segments in the opposite order
-// and so finds the last ones in L2. (Measured against one pass whose tiles wait
-// for the maps of the tiles before them: 1 x 65536 x 1024 bf16 took 0.37 to 0.45 ms
-// that way, as the tiles under way are too few to cover the waits.)
+// Where even crews are too few, the steps are cut into segments: one kernel
+// walks each segment for its map, one folds them in order into the state before
+// each segment, and the walk itself then starts everywhere at once. The inputs
+// are read twice. 1 x 65536 x 1024: 127 to 132 us, the gradient 178 us. (One pass
+// whose tiles publish maps and wait for the ones before them took 370 to 450 us
+// there: the tiles under way are too few to cover the waits.)
 #pragma once
 
 #include "b200_leaky.h"
@@ -828,7 +828,10 @@ __global__ void __launch_bounds__(N * 32) back_crew_kernel(const __grid_constant
 // ---- single step ----
 // A row of the pool is updated by the threads of the first row that names
 // it, which also do the later rows that name it, in order. To know, every CTA
-// looks through the slots once, for all of its rows at a time.
+// looks through the slots once, for all of its rows at a time. 2000 rows of 1000
+// channels out of 4096: 7 us a call, 28 MB; the look was most of it (10.5 us) while
+// every slot was compared with all that a decision needs instead of first with
+// the rows' own.
 template <typename X, typename G, typename Y, int V>
 __global__ void __launch_bounds__(256, 4) step_kernel(StepArgs g) {
     __shared__ uint32_t s_before[8], s_after[8];  // rows named before, rows named again

@@ -208,12 +208,19 @@ __device__ __forceinline__ void put(const Problem &p, uint32_t i, uint32_t j, fl
 
 constexpr uint32_t kNoValue = 0x7fffffffu;
 
-// ---- wide form ----
+// ---- pairs ----
 // A pair of CTAs (cta_group::2) works on 256 weight rows and 256 rows of x: each
 // CTA holds 128 of both in shared memory and the accumulators of its weight
-// rows, and the instructions read x from both. What a CTA loads for a tile is
-// the bound (about 11 TB/s come out of L2 for all SMs; 256 rows of x a CTA took
-// 309 us at 8192x8192x8192), and this halves x's part of it.
+// rows, and the instructions read x from both, so an SM loads 35 KB for 256 of k
+// where a CTA of its own with 256 rows of x would load 52.
+//
+// 8192 x 8192 x 8192: 193 us, 5.7 PFLOP/s, the tensor pipe active 72% of the
+// time. The bound was the issue (347 us while one lane of a divergent warp put
+// the descriptors together; leaving out the loads or the stores changed nothing,
+// leaving out the scale copies gave 277). 50000 x 784 x 1000 to f32: 50 us, of
+// which the writes of 200 MB are 30; 16 warps read the accumulators there, as
+// with 8 (43 against 33 us at 768 of k to bf16) a tile's writes took longer than
+// its instructions.
 constexpr uint32_t kPairN = 256, kPairStages = 6;
 constexpr uint32_t kReaders = 16;  // warps that read and write accumulators: four share the lanes, kReaders / 4 the columns
 constexpr uint32_t kPairThreads = 128 + kReaders * 32, kReadN = kPairN / (kReaders / 4);
@@ -370,6 +377,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ---- skinny form ----
+// Four parts of k of 4 x 8192 x 8192 are one wave of 256 CTAs, two an SM: 9 us a
+// launch among others, of which the 36 MB of weights are 5.5; the rest is set-up
+// and the joining of the parts. Packing x on the way takes 16 rows in 12.3 us where
+// a packing kernel before it takes 12.6 + 4, 32 rows in 22.7 against 14.6 + 4, so
+// 16 rows are the most.
 constexpr uint32_t kMostSplits = 8;
 template <uint32_t BN>
 struct Skinny {

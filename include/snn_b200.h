@@ -466,7 +466,8 @@ snn_status_t snn_b200_step_noalloc(int device, void *stream, snn_size_t neuron_c
  * writes only what it still defines. Counts above 2^31 - 1 (and batch x
  * channels above it) return SNN_ERR_OVERFLOW, a combination of element types that is not listed
  * SNN_ERR_UNSUPPORTED, everything else that is wrong with an argument
- * SNN_ERR_INVALID_ARGUMENT. */
+ * SNN_ERR_INVALID_ARGUMENT. The kernels' shared memory limits are raised once
+ * a device: do not make these calls on a device after cudaDeviceReset. */
 typedef enum snn_b200_dtype {
     SNN_B200_F32 = 0,
     SNN_B200_F16 = 1,
@@ -515,8 +516,10 @@ snn_status_t snn_b200_mx4_matmul_async(int device, void *stream, const void *x_c
 
 /* The same with x (m x k, any snn_b200_dtype_t, strides as for quantize)
  * packed on the way: equal to quantize followed by matmul. The workspace holds
- * snn_b200_mx4_linear_workspace(m, k) bytes, 16-byte aligned. */
-snn_size_t snn_b200_mx4_linear_workspace(snn_size_t m, snn_size_t k);
+ * as many bytes as snn_b200_mx4_linear_workspace says, 16-byte aligned (none
+ * for up to 16 rows that start on 16 bytes). */
+snn_size_t snn_b200_mx4_linear_workspace(const void *x, int x_dtype, snn_size_t m, snn_size_t k, int64_t x_row_stride,
+                                         int64_t x_col_stride);
 snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, int x_dtype, snn_size_t m,
                                        snn_size_t k, int64_t x_row_stride, int64_t x_col_stride, const void *w_codes,
                                        const void *w_scales, snn_size_t n, const float *bias, void *out,
@@ -568,8 +571,8 @@ typedef struct snn_b200_leaky {
  * 8th step, floats [batch, ceil(steps / 8), channels]. */
 #define SNN_B200_LEAKY_BLOCK 8u
 snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_size_t channels);
-/* Bytes of workspace (16-byte aligned) of the forward and of the backward call. */
-snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *leaky);
+/* Bytes of workspace (16-byte aligned) of a forward or a backward call, often none. */
+snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *leaky, int backward);
 
 /* h0 may be NULL (zero); h_last and saved may be NULL (not wanted). */
 snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,

@@ -159,11 +159,11 @@ ENTRY_POINTS = [
     ("snn_b200_mx4_quantize_async", C.c_int, [C.c_int, P, P, C.c_int, u64, u64, i64, i64, P, P]),
     ("snn_b200_mx4_dequantize_async", C.c_int, [C.c_int, P, P, P, u64, u64, P, C.c_int, i64]),
     ("snn_b200_mx4_matmul_async", C.c_int, [C.c_int, P, P, P, u64, P, P, u64, u64, P, P, C.c_int, i64]),
-    ("snn_b200_mx4_linear_workspace", u64, [u64, u64]),
+    ("snn_b200_mx4_linear_workspace", u64, [P, C.c_int, u64, u64, i64, i64]),
     ("snn_b200_mx4_linear_async", C.c_int, [C.c_int, P, P, C.c_int, u64, u64, i64, i64, P, P, u64, P, P, C.c_int,
                                             i64, P, u64]),
     ("snn_b200_leaky_saved_floats", u64, [u64, u64, u64]),
-    ("snn_b200_leaky_workspace", u64, [P]),
+    ("snn_b200_leaky_workspace", u64, [P, C.c_int]),
     ("snn_b200_leaky_scan_async", C.c_int, [C.c_int, P, P, P, P, P, P, P, P, P, P, u64]),
     ("snn_b200_leaky_scan_backward_async", C.c_int, [C.c_int, P, P, P, P, P, P, P, P, P, P, P, P, u64]),
     ("snn_b200_leaky_step_async", C.c_int, [C.c_int, P, u64, u64, u64, P, C.c_int, i64, P, C.c_int, i64, C.c_int,

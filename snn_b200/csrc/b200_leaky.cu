@@ -129,7 +129,7 @@ struct Plan {
 // 90 us); 64 columns take 102 us in crews and about 70 in segments.
 constexpr uint64_t kFewWalks = 148 * 5, kFewCrews = 104, kManyWalks = 148 * 48;
 constexpr uint32_t kLeastSegment = 64;
-Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
+Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
     Plan p = {};
     p.flat = q.batch * q.channels;
     p.columns = (p.flat + 32 * width - 1) / (32 * width);
@@ -148,7 +148,7 @@ Plan plan_of(const snn_b200_leaky_t &q, uint32_t width) {
     p.maps = 0;
     p.states = p.maps + round(cut * 8);
     p.partial = p.states + round(cut * 4);
-    p.bytes = p.partial + round(p.partials * p.flat * 4);
+    p.bytes = p.partial + (back && !q.gate_step_stride ? round(p.partials * p.flat * 4) : 0);
     return p;
 }
 
@@ -213,9 +213,9 @@ snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_s
     return batch * ((steps + kSteps - 1) / kSteps) * channels;
 }
 
-snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *q) {
+snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *q, int backward) {
     if (q == nullptr || q->batch > kMaxCount || q->steps > kMaxCount || q->channels > kMaxCount) return 0;
-    return std::max({plan_of(*q, 1).bytes, plan_of(*q, 2).bytes, plan_of(*q, 4).bytes});
+    return std::max({plan_of(*q, 1, backward).bytes, plan_of(*q, 2, backward).bytes, plan_of(*q, 4, backward).bytes});
 }
 
 snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,
@@ -227,8 +227,9 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
     if (!floats_ok(h0) || !floats_ok(h_last) || !floats_ok(saved)) return SNN_ERR_INVALID_ARGUMENT;
     if (q.batch == 0 || q.channels == 0) return SNN_OK;
     if (q.steps && !output_ok(y, q.y_dtype, q, q.y_batch_stride, q.y_step_stride)) return SNN_ERR_INVALID_ARGUMENT;
-    const uint64_t need = snn_b200_leaky_workspace(leaky);
-    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)) return SNN_ERR_INVALID_ARGUMENT;
+    const uint64_t need = snn_b200_leaky_workspace(leaky, 0);
+    if (need && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)))
+        return SNN_ERR_INVALID_ARGUMENT;
     if (q.batch * q.channels > kMaxCount) return SNN_ERR_OVERFLOW;
     DeviceScope scope(device);
     if (scope.error() != cudaSuccess) return op_status(scope.error(), __func__);
@@ -249,7 +250,7 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
     const uint32_t width = q.x_dtype == SNN_B200_SPIKES && holds(4) ? 4 : holds(2) ? 2 : 1;
     Args g = {};
     g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
-    const cudaError_t e = run(s, q, g, plan_of(q, width), width, false, workspace);
+    const cudaError_t e = run(s, q, g, plan_of(q, width, false), width, false, workspace);
     return op_status(e, __func__);
 }
 
@@ -276,7 +277,7 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
     if (dgate && !every && !shared &&
         (!offset_fits(q.batch, q.dgate_batch_stride) || !disjoint_runs(q.batch, q.dgate_batch_stride, 1, 0, q.channels)))
         return SNN_ERR_INVALID_ARGUMENT;
-    const uint64_t need = snn_b200_leaky_workspace(leaky);
+    const uint64_t need = snn_b200_leaky_workspace(leaky, 1);
     if (need && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)))
         return SNN_ERR_INVALID_ARGUMENT;
     if (q.batch * q.channels > kMaxCount) return SNN_ERR_OVERFLOW;
@@ -304,7 +305,7 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
     g.x = x, g.gate = gate, g.lengths = lengths, g.saved = const_cast<float *>(saved), g.dy = dy;
     g.dh_last = dh_last, g.dx = dx, g.dgate = every ? dgate : nullptr, g.dh0 = dh0;
     const uint32_t width = even ? 2 : 1;
-    const Plan p = plan_of(q, width);
+    const Plan p = plan_of(q, width, true);
     g.partial = sums ? (float *)((char *)workspace + p.partial) : nullptr;
     cudaError_t e = run(s, q, g, p, width, true, workspace);
     if (e == cudaSuccess && sums) {

@@ -942,51 +942,51 @@ cudaError_t step_narrow(cudaStream_t s, const Form &f, const StepArgs &a, dim3 g
     return wide ? launch_step<X, X, float>(s, f, a, grid) : launch_step<X, X, X>(s, f, a, grid);
 }
 
-// grid CTAs of `warps` warps, each with `feed` bytes of shared memory, beside `fixed` bytes of the kernel's own.
-template <typename K>
-cudaError_t start(K kernel, cudaStream_t s, const Args &a, uint64_t grid, uint32_t warps, uint32_t feed, uint32_t fixed = 0) {
-    const uint32_t smem = warps * feed;
-    if (smem + fixed > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+// grid CTAs of Warps warps, each with Feed bytes of shared memory, beside Fixed bytes of the kernel's own.
+template <auto Kernel, uint32_t Warps, uint32_t FeedBytes, uint32_t FixedBytes = 0>
+cudaError_t start(cudaStream_t s, const Args &a, uint64_t grid) {
+    constexpr uint32_t smem = Warps * FeedBytes;
+    if constexpr (smem + FixedBytes > 48 * 1024) {
+        const cudaError_t e = allow_smem<Kernel>(smem);
         if (e != cudaSuccess) return e;
     }
-    return launch_early(kernel, (uint32_t)grid, warps * 32, smem, s, 1, a);
+    return launch_early(Kernel, (uint32_t)grid, Warps * 32, smem, s, 1, a);
 }
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_scan(cudaStream_t s, const Args &a) {
     constexpr uint32_t slot = Feed<X, V>::kBytes + Feed<G, V>::kBytes;
     if constexpr (V <= 2) {
         if (a.crew == 16)
-            return start(scan_crew_kernel<X, G, Y, V, 16>, s, a, a.columns, 16, crew_depth<V, 16>(slot) * slot,
-                         sizeof(Crew<V, 16>));
+            return start<scan_crew_kernel<X, G, Y, V, 16>, 16, crew_depth<V, 16>(slot) * slot, sizeof(Crew<V, 16>)>(
+                s, a, a.columns);
         if (a.crew)
-            return start(scan_crew_kernel<X, G, Y, V, 8>, s, a, a.columns, 8, crew_depth<V, 8>(slot) * slot,
-                         sizeof(Crew<V, 8>));
+            return start<scan_crew_kernel<X, G, Y, V, 8>, 8, crew_depth<V, 8>(slot) * slot, sizeof(Crew<V, 8>)>(
+                s, a, a.columns);
     }
     const uint64_t grid = ((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps;
     if (a.segments > 1) {
-        cudaError_t e = start(scan_kernel<X, G, Y, V, true>, s, a, grid, kWarps, kDepth * slot);
+        cudaError_t e = start<scan_kernel<X, G, Y, V, true>, kWarps, kDepth * slot>(s, a, grid);
         if (e == cudaSuccess) e = carry(s, a, false);
         if (e != cudaSuccess) return e;
     }
-    return start(scan_kernel<X, G, Y, V, false>, s, a, grid, kWarps, kDepth * slot);
+    return start<scan_kernel<X, G, Y, V, false>, kWarps, kDepth * slot>(s, a, grid);
 }
 template <typename X, typename G, typename Y, int V>
 cudaError_t launch_back(cudaStream_t s, const Args &a) {
     constexpr uint32_t maps = Feed<G, V>::kBytes + Feed<Y, V>::kBytes, slot = maps + Feed<X, V>::kBytes + kSavedBytes<V>;
     if (a.crew == 16)
-        return start(back_crew_kernel<X, G, Y, V, 16>, s, a, a.columns, 16, crew_depth<V, 16>(slot) * slot,
-                     sizeof(Crew<V, 16>));
+        return start<back_crew_kernel<X, G, Y, V, 16>, 16, crew_depth<V, 16>(slot) * slot, sizeof(Crew<V, 16>)>(
+            s, a, a.columns);
     if (a.crew)
-        return start(back_crew_kernel<X, G, Y, V, 8>, s, a, a.columns, 8, crew_depth<V, 8>(slot) * slot,
-                     sizeof(Crew<V, 8>));
+        return start<back_crew_kernel<X, G, Y, V, 8>, 8, crew_depth<V, 8>(slot) * slot, sizeof(Crew<V, 8>)>(s, a,
+                                                                                                              a.columns);
     const uint64_t grid = ((uint64_t)a.columns * a.segments + kWarps - 1) / kWarps;
     if (a.segments > 1) {
-        cudaError_t e = start(back_kernel<X, G, Y, V, true>, s, a, grid, kWarps, kDepth * maps);
+        cudaError_t e = start<back_kernel<X, G, Y, V, true>, kWarps, kDepth * maps>(s, a, grid);
         if (e == cudaSuccess) e = carry(s, a, true);
         if (e != cudaSuccess) return e;
     }
-    return start(back_kernel<X, G, Y, V, false>, s, a, grid, kWarps, kDepth * slot);
+    return start<back_kernel<X, G, Y, V, false>, kWarps, kDepth * slot>(s, a, grid);
 }
 template <typename X, typename G, typename Y>
 cudaError_t launch(cudaStream_t s, const Form &f, const Args &a, bool back) {

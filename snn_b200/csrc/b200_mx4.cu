@@ -62,8 +62,9 @@ __global__ void __launch_bounds__(256) mx4_quantize_rows_kernel(const T *src, ui
 }
 
 // Other strides: a thread a block, lanes along the rows, so a transposed source
-// is read in whole runs (3873 x 34654 transposed: f32 108 us, bf16, whose runs
-// are 64 bytes, 250 us).
+// is read in whole runs; all of a block's elements are on their way before the
+// first is looked at (3873 x 34654 transposed: f32 109 us, bf16 110 us, 250 us with
+// the magnitude taken on the way; the two rows of a word in a thread took 327).
 template <typename T>
 __global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uint32_t rows, uint32_t cols, int64_t rs,
                                                                int64_t cs, uint8_t *codes, uint8_t *scales,
@@ -71,24 +72,25 @@ __global__ void __launch_bounds__(512) mx4_quantize_any_kernel(const T *src, uin
     __shared__ __align__(16) uint8_t s_scales[512];
     const uint32_t tile = blockIdx.x, at = threadIdx.x % kTileRows, b = threadIdx.x / kTileRows;
     const uint64_t r = (uint64_t)blockIdx.y * kTileRows + at, c = (uint64_t)tile * kTileCols + b * kBlock;
-    uint32_t s = 0;
+    const uint32_t n = r < rows && c < cols ? min(kBlock, (uint32_t)(cols - c)) : 0;
+    const T *p = src + (int64_t)r * rs + (int64_t)c * cs;
+    T e[kBlock];
     after_previous();
-    if (r < rows && c < cols) {
-        const T *p = src + (int64_t)r * rs + (int64_t)c * cs;
-        const uint32_t n = min(kBlock, (uint32_t)(cols - c));
-        float v[kBlock];
-        uint32_t top = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < kBlock; ++k) v[k] = k < n ? to_float(p[(int64_t)k * cs]) : 0.0f;
+    for (uint32_t k = 0; k < kBlock; ++k) e[k] = k < n ? p[(int64_t)k * cs] : T{};
+    uint32_t top = 0, w[4];
 #pragma unroll
-        for (uint32_t k = 0; k < kBlock; ++k) top = max(top, __float_as_uint(fabsf(v[k])));
-        s = scale_byte(top);
-        const float inv = inverse_scale(s);
-        uint32_t w[4];
+    for (uint32_t k = 0; k < kBlock; ++k) top = max(top, __float_as_uint(fabsf(to_float(e[k]))));
+    const uint32_t s = scale_byte(top);
+    const float inv = inverse_scale(s);
 #pragma unroll
-        for (uint32_t q = 0; q < 4; ++q) w[q] = s == 255u ? 0u : encode8(v + 8 * q, inv);
-        reinterpret_cast<uint4 *>(codes)[r * blocks_of(cols) + c / kBlock] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (uint32_t q = 0; q < 4; ++q) {
+        float v[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) v[k] = to_float(e[8 * q + k]);
+        w[q] = s == 255u ? 0u : encode8(v, inv);
     }
+    if (n) reinterpret_cast<uint4 *>(codes)[r * blocks_of(cols) + c / kBlock] = make_uint4(w[0], w[1], w[2], w[3]);
     s_scales[scale_slot(at, b)] = (uint8_t)s;
     __syncthreads();
     if (threadIdx.x < 32)
@@ -300,8 +302,9 @@ snn_status_t snn_b200_mx4_matmul_async(int device, void *stream, const void *x_c
                      __func__);
 }
 
-snn_size_t snn_b200_mx4_linear_workspace(snn_size_t m, snn_size_t k) {
-    if (m > kMaxCount || k > kMaxCount) return 0;
+snn_size_t snn_b200_mx4_linear_workspace(const void *x, int x_dtype, snn_size_t m, snn_size_t k, int64_t x_row_stride,
+                                         int64_t x_col_stride) {
+    if (m > kMaxCount || k > kMaxCount || packs_on_the_way(x, x_dtype, m, x_row_stride, x_col_stride)) return 0;
     return code_bytes(m, k) + scale_bytes(m, k);
 }
 
@@ -315,7 +318,7 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
     if (st == SNN_OK) st = check_packed(w_codes, w_scales, n, k);
     if (st == SNN_OK) st = check_rows(out, out_dtype, m, n, out_row_stride);
     if (st != SNN_OK || device < 0 || !aligned_to(bias, 4)) return st != SNN_OK ? st : SNN_ERR_INVALID_ARGUMENT;
-    const uint64_t need = snn_b200_mx4_linear_workspace(m, k);
+    const uint64_t need = snn_b200_mx4_linear_workspace(x, x_dtype, m, k, x_row_stride, x_col_stride);
     if (need && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)))
         return SNN_ERR_INVALID_ARGUMENT;
     if (m == 0 || n == 0) return SNN_OK;

@@ -590,7 +590,7 @@ cudaError_t launch_pairs(int device, cudaStream_t s, const Packed &x, const Pack
     if (e == cudaSuccess) e = map_of(&m.x, x, k, 128);
     if (e == cudaSuccess) e = scale_map_of(&m.w_scales, w, k, 1);
     if (e == cudaSuccess) e = scale_map_of(&m.x_scales, x, k, 2);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+    if (e == cudaSuccess) e = allow_smem<pair_kernel<T>>(kPairSmem);
     if (e != cudaSuccess) return e;
     const uint64_t tiles = (uint64_t)p.tiles_n * p.tiles_m, most = (uint64_t)sm_count(device) / 2;
     return launch_early(pair_kernel<T>, 2 * (uint32_t)std::min(tiles, most), kPairThreads, kPairSmem, s, 2, m, p);
@@ -599,8 +599,8 @@ cudaError_t launch_pairs(int device, cudaStream_t s, const Packed &x, const Pack
 template <typename T, uint32_t BN, typename X>
 cudaError_t launch_skinny(cudaStream_t s, const CUtensorMap &wm, const CUtensorMap &xm, const Problem &p) {
     using K = Skinny<BN>;
-    const auto kernel = skinny_kernel<T, BN, X>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kSmem);
+    constexpr auto kernel = skinny_kernel<T, BN, X>;
+    const cudaError_t e = allow_smem<kernel>(K::kSmem);
     if (e != cudaSuccess) return e;
     const uint32_t threads = std::is_same<X, None>::value ? 128 : 256;
     return launch_early(kernel, p.tiles_n * p.tiles_m * p.splits, threads, K::kSmem, s, p.splits, wm, xm, p);

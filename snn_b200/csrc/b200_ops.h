@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace b200 {
@@ -81,6 +82,18 @@ cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
     c.attrs = at;
     c.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+// Lets a kernel have that much dynamic shared memory on the current device;
+// asked for once a device.
+template <auto Kernel>
+cudaError_t allow_smem(uint32_t bytes) {
+    static std::atomic<uint64_t> asked{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 64 && asked.load(std::memory_order_acquire) >> device & 1)) return e;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 64) asked.fetch_or(1ull << device, std::memory_order_release);
+    return e;
 }
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;"); }

@@ -105,6 +105,9 @@ void *stream_of(int device) { return c10::cuda::getCurrentCUDAStream((c10::Devic
 Tensor empty(at::IntArrayRef sizes, at::ScalarType t, const Tensor &like) {
     return at::empty(sizes, like.options().dtype(t).memory_format(c10::nullopt));
 }
+Tensor scratch(snn_size_t bytes, const Tensor &like) {
+    return bytes ? empty({(int64_t)bytes}, at::kByte, like) : Tensor();
+}
 const void *data(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *out(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
@@ -200,8 +203,9 @@ PyObject *linear(Args a) {
     for (int64_t d = 0; d + 1 < x.dim(); ++d) m *= x.size(d);
     const Tensor flat = x.dim() == 2 ? x : x.reshape({m, w.cols});
     Tensor y = empty({m, w.rows}, a.dtype(6, result_type(x)), x);
-    const snn_size_t need = snn_b200_mx4_linear_workspace(m, w.cols);
-    const Tensor ws = empty({(int64_t)need}, at::kByte, x);
+    const snn_size_t need =
+        snn_b200_mx4_linear_workspace(data(flat), type, m, w.cols, flat.stride(0), flat.stride(1));
+    const Tensor ws = scratch(need, x);
     check(snn_b200_mx4_linear_async(dev, stream_of(dev), data(flat), type, m, w.cols, flat.stride(0), flat.stride(1),
                                     data(w.codes), data(w.scales), w.rows, bias_of(bias, w.rows), out(y), code(y),
                                     w.rows, out(ws), need),
@@ -262,9 +266,9 @@ struct Sequence {
     }
     const uint32_t *length() const { return (const uint32_t *)data(lengths); }
     int64_t blocks() const { return ((int64_t)q.steps + SNN_B200_LEAKY_BLOCK - 1) / SNN_B200_LEAKY_BLOCK; }
-    Tensor workspace(snn_size_t *need) const {
-        *need = snn_b200_leaky_workspace(&q);
-        return empty({(int64_t)*need}, at::kByte, x);
+    Tensor workspace(snn_size_t *need, bool backward) const {
+        *need = snn_b200_leaky_workspace(&q, backward);
+        return scratch(*need, x);
     }
 };
 
@@ -280,7 +284,7 @@ PyObject *scan(Args a) {
     if (save) saved = empty({b, s.blocks(), c}, at::kFloat, s.x);
     s.q.y_dtype = code(y), s.q.y_batch_stride = y.stride(0), s.q.y_step_stride = y.stride(1);
     snn_size_t need;
-    const Tensor ws = s.workspace(&need);
+    const Tensor ws = s.workspace(&need, false);
     check(snn_b200_leaky_scan_async(s.dev, stream_of(s.dev), &s.q, data(s.x), data(s.gate), (const float *)data(h0),
                                     s.length(), out(y), (float *)out(h_last), (float *)out(saved), out(ws), need),
           "snn_b200_leaky_scan_async");
@@ -314,7 +318,7 @@ PyObject *scan_backward(Args a) {
     q.y_dtype = code(dy), q.dy_batch_stride = stride(dy, 0, 0), q.dy_step_stride = stride(dy, 1, 0);
     q.dx_batch_stride = dx.stride(0), q.dx_step_stride = dx.stride(1);
     snn_size_t need;
-    const Tensor ws = s.workspace(&need);
+    const Tensor ws = s.workspace(&need, true);
     check(snn_b200_leaky_scan_backward_async(s.dev, stream_of(s.dev), &q, data(s.x), data(s.gate), s.length(),
                                              (const float *)data(saved), data(dy), (const float *)data(dh_last), out(dx),
                                              out(dgate), (float *)out(dh0), out(ws), need),

@@ -273,7 +273,7 @@ def test_rows_inside_wider_arrays():
     q = sb.Leaky(b, t, c, 2, 0, 2, 1, 0, 0.0, 1.0, t * w, w, t * w, w, t * w, w)
     L = sb.lib()
     import ctypes as C
-    need = L.snn_b200_leaky_workspace(C.byref(q))
+    need = L.snn_b200_leaky_workspace(C.byref(q), 0)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
     st = L.snn_b200_leaky_scan_async(0, torch.cuda.current_stream().cuda_stream, C.byref(q), xs.data_ptr(),
                                      zs.data_ptr(), None, None, ys.data_ptr(), None, None, ws.data_ptr(), need)

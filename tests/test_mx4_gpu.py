@@ -36,13 +36,17 @@ def unpacked(q):
 SHAPES = [(1, 1), (1, 31), (3, 32), (5, 33), (127, 128), (128, 129), (129, 784), (1000, 784), (257, 1027), (33, 4100)]
 
 
-@pytest.mark.parametrize("order", ["rows", "cols", "wide"])
+@pytest.mark.parametrize("order", ["rows", "cols", "words", "wide"])
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16", "u8"])
 @pytest.mark.parametrize("rows,cols", SHAPES)
 def test_pack_matches_definition(rows, cols, kind, order):
     x = draw((rows, cols), kind, rows * 7 + cols, spread=8 if kind != "u8" else 0)
     if order == "cols":
         view = x.t().contiguous().t()
+    elif order == "words":  # columns of a whole number of words
+        big = torch.zeros(cols, (rows + 7) // 4 * 4, dtype=x.dtype, device="cuda")
+        view = big[:, :rows].t()
+        view.copy_(x)
     elif order == "wide":  # every third element of wider rows, at an odd offset
         big = torch.zeros(rows, cols * 3 + 5, dtype=x.dtype, device="cuda")
         view = big[:, 1:1 + cols * 3:3]
@@ -172,7 +176,7 @@ def test_linear_strides_and_rows_behind():
     assert torch.equal(sb.mx4_linear(x, w), want)
     assert torch.equal(sb.mx4_linear(x.t().contiguous().t(), w), want)
     out = torch.full((m + 2, n + 13), -7.0, dtype=torch.float16, device="cuda")
-    need = sb.lib().snn_b200_mx4_linear_workspace(m, k)
+    need = sb.lib().snn_b200_mx4_linear_workspace(x.data_ptr(), 1, m, k, x.stride(0), 1)
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
     st = sb.lib().snn_b200_mx4_linear_async(0, torch.cuda.current_stream().cuda_stream, x.data_ptr(), 1, m, k,
                                             x.stride(0), 1, w.codes.data_ptr(), w.scales.data_ptr(), n, None,

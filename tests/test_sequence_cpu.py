@@ -25,9 +25,12 @@ def test_sizes():
     assert e.value.status == OVER
     L = sb.lib()
     assert L.snn_b200_mx4_sizes(1, 1, None, None) == BAD
-    assert L.snn_b200_mx4_linear_workspace(2, 784) == sum(sb.mx4_sizes(2, 784))
+    assert L.snn_b200_mx4_linear_workspace(P, F32, 17, 784, 784, 1) == sum(sb.mx4_sizes(17, 784))
+    assert L.snn_b200_mx4_linear_workspace(P, F32, 16, 784, 784, 1) == 0  # packed by the product's kernel
+    assert L.snn_b200_mx4_linear_workspace(P + 4, F32, 16, 784, 784, 1) == sum(sb.mx4_sizes(16, 784))
+    assert L.snn_b200_mx4_linear_workspace(P, F32, 16, 783, 783, 1) == sum(sb.mx4_sizes(16, 783))
     assert L.snn_b200_leaky_saved_floats(3, 33, 5) == 3 * 5 * 5
-    assert L.snn_b200_leaky_workspace(None) == 0
+    assert L.snn_b200_leaky_workspace(None, 0) == L.snn_b200_leaky_workspace(None, 1) == 0
 
 
 QUANT = dict(device=0, stream=None, src=P, dtype=F32, rows=4, cols=64, rs=64, cs=1, codes=P, scales=P)
@@ -64,22 +67,22 @@ def test_matmul_refusals(change, status):
     assert sb.lib().snn_b200_mx4_matmul_async(*{**MATMUL, **change}.values()) == status
 
 
-LINEAR = dict(device=0, stream=None, x=P, x_dtype=BF16, m=4, k=64, xrs=64, xcs=1, wc=P, ws=P, n=8, bias=None, out=P,
+LINEAR = dict(device=0, stream=None, x=P, x_dtype=BF16, m=20, k=64, xrs=64, xcs=1, wc=P, ws=P, n=8, bias=None, out=P,
               dtype=F32, rs=8, work=P, work_bytes=1 << 20)
 
 
 @pytest.mark.parametrize("change,status", [
     (dict(device=-1), BAD), (dict(x=None), BAD), (dict(x=P + 1), BAD), (dict(x_dtype=9), BAD), (dict(xrs=-1), BAD),
     (dict(wc=None), BAD), (dict(out=None), BAD), (dict(rs=7), BAD), (dict(work=None), BAD), (dict(work=P + 8), BAD),
-    (dict(work_bytes=sum(sb.mx4_sizes(4, 64)) - 1), BAD), (dict(m=BIG), OVER), (dict(k=BIG), OVER), (dict(m=0), OK)])
+    (dict(work_bytes=sum(sb.mx4_sizes(20, 64)) - 1), BAD), (dict(m=BIG), OVER), (dict(k=BIG), OVER), (dict(m=0), OK)])
 def test_linear_refusals(change, status):
     assert sb.lib().snn_b200_mx4_linear_async(*{**LINEAR, **change}.values()) == status
 
 
-SHAPE = dict(batch=2, steps=40, channels=8, x_dtype=BF16, gate_dtype=BF16, y_dtype=BF16, logit=0, complement=0,
-             decay=0.5, input_scale=1.0, x_batch_stride=320, x_step_stride=8, gate_batch_stride=320,
-             gate_step_stride=8, y_batch_stride=320, y_step_stride=8, dy_batch_stride=320, dy_step_stride=8,
-             dx_batch_stride=320, dx_step_stride=8, dgate_batch_stride=320, dgate_step_stride=8)
+SHAPE = dict(batch=2, steps=400, channels=8, x_dtype=BF16, gate_dtype=BF16, y_dtype=BF16, logit=0, complement=0,
+             decay=0.5, input_scale=1.0, x_batch_stride=3200, x_step_stride=8, gate_batch_stride=3200,
+             gate_step_stride=8, y_batch_stride=3200, y_step_stride=8, dy_batch_stride=3200, dy_step_stride=8,
+             dx_batch_stride=3200, dx_step_stride=8, dgate_batch_stride=3200, dgate_step_stride=8)
 SCAN = dict(x=P, gate=P, h0=P, lengths=P, y=P, h_last=P, saved=P, work=P, work_bytes=1 << 30)
 BACK = dict(x=P, gate=P, lengths=P, saved=P, dy=P, dh_last=P, dx=P, dgate=P, dh0=P, work=P, work_bytes=1 << 30)
 
@@ -103,7 +106,7 @@ COMMON = [
 
 @pytest.mark.parametrize("change,status", COMMON + [
     (dict(y=None), BAD), (dict(y=P + 1), BAD), (dict(h0=P + 2), BAD), (dict(h_last=P + 1), BAD), (dict(saved=P + 2), BAD),
-    (dict(y_step_stride=7), BAD), (dict(y_batch_stride=319), BAD), (dict(y_batch_stride=8, y_step_stride=8), BAD),
+    (dict(y_step_stride=7), BAD), (dict(y_batch_stride=3199), BAD), (dict(y_batch_stride=8, y_step_stride=8), BAD),
     (dict(y_step_stride=0), BAD)])
 def test_scan_refusals(change, status):
     assert call("snn_b200_leaky_scan_async", SHAPE, SCAN, change) == status
@@ -112,7 +115,7 @@ def test_scan_refusals(change, status):
 @pytest.mark.parametrize("change,status", COMMON + [
     (dict(saved=None), BAD), (dict(saved=P + 2), BAD), (dict(dy=None), BAD), (dict(dy=P + 1), BAD),
     (dict(dh_last=P + 2), BAD), (dict(dh0=P + 1), BAD), (dict(dx=P + 1), BAD), (dict(dgate=P + 1), BAD),
-    (dict(dx_step_stride=7), BAD), (dict(dgate_batch_stride=319), BAD), (dict(gate=None), BAD),
+    (dict(dx_step_stride=7), BAD), (dict(dgate_batch_stride=3199), BAD), (dict(gate=None), BAD),
     (dict(gate_batch_stride=0), UNSUP), (dict(gate_dtype=F32, gate_step_stride=0, dgate_batch_stride=7), BAD)])
 def test_backward_refusals(change, status):
     assert call("snn_b200_leaky_scan_backward_async", SHAPE, BACK, change) == status

@@ -285,8 +285,8 @@ struct Feed {
                 if ((int)j < left) copy<16>(at + (j * kAcross + lane) * 16, row);
         } else if constexpr (kOwn >= 4) {
 #pragma unroll
-            for (int j = 0; j < (int)kSteps; ++j)
-                if (j < live) copy<kOwn>(at + j * kRow + lane * kOwn, row + j * stride);
+            for (int j = 0; j < (int)kSteps; ++j, row += stride)
+                if (j < live) copy<kOwn>(at + j * kRow + lane * kOwn, row);
         }
     }
     // The block's rows; those behind the live ones are anything.
@@ -298,7 +298,7 @@ struct Feed {
         } else {
             const T *row = p + (int64_t)t0 * stride;
 #pragma unroll
-            for (int j = 0; j < (int)kSteps; ++j) r[j] = j < live ? load<T, V>(row + j * stride) : Vec<T, V>{};
+            for (int j = 0; j < (int)kSteps; ++j, row += stride) r[j] = j < live ? load<T, V>(row) : Vec<T, V>{};
         }
     }
 };

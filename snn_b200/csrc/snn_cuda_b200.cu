@@ -2055,7 +2055,10 @@ snn_status_t group_step(snn_cuda_context_t *g, const float *ext, uint8_t *spikes
 //                              C ABI
 // ======================================================================
 namespace b200 {
-snn_status_t op_status(cudaError_t e, const char *where) { return cuda_status_at(e, where); }
+snn_status_t op_status(cudaError_t e, const char *where) {
+    if (e != cudaSuccess) cudaGetLastError();  // reported here, not by whoever asks the runtime next
+    return cuda_status_at(e, where);
+}
 }  // namespace b200
 
 extern "C" {

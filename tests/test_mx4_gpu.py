@@ -235,3 +235,18 @@ def test_two_products_at_once(m, k, n):
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % 2])
+
+
+def test_a_device_that_is_not_there_and_the_callers_own():
+    """A device index beyond the last one is an error of the call alone; the caller's current device stays."""
+    x = torch.ones(4, 64, device="cuda")
+    q = sb.mx4_quantize(x)
+    L = sb.lib()
+    args = (None, x.data_ptr(), 0, 4, 64, 64, 1, q.codes.data_ptr(), q.scales.data_ptr())
+    before = torch.cuda.current_device()
+    assert L.snn_b200_mx4_quantize_async(torch.cuda.device_count() + 7, *args) == sb.SNN_ERR_CUDA
+    assert sb.last_error()
+    assert torch.cuda.current_device() == before
+    assert L.snn_b200_mx4_quantize_async(before, *args) == sb.SNN_OK
+    assert torch.equal(sb.mx4_dequantize(q), x)
+    torch.cuda.synchronize()

@@ -122,21 +122,29 @@ struct Plan {
     uint32_t crew;
     uint64_t maps, states, partial, bytes;
 };
-// Warps that walk whole sequences, or where those would be too few to keep the
-// loads of 148 SMs under way, crews, or where even those are too few, segments
-// (64 steps at least). A crew has 16 warps where it has an SM to itself, else 8
-// (8192 steps, bf16, 128 columns: 104 against 127 us, 256 columns of 4096: 105 against
-// 90 us); 64 columns take 102 us in crews and about 70 in segments.
+// Warps that walk whole sequences; where those would be too few to keep the loads
+// of 148 SMs under way, crews; where even crews are too few and the sequences
+// long, segments (64 steps at least), which cost three launches.
+// Measured in us, forward and gradient (f32 with a leak a channel):
+//   512 channels:   32 steps  128        512         1024        2048
+//     whole         3.1, 5.5  7.4, 11.7  23.9, 36.0  45.6, 68.4
+//     crews                   3.1, 5.5   6.4, 10.0   11.1, 16.2  20.4, 28.8
+//     segments                11.2, 14.1 11.5, 14.7  12.0, 15.3  12.6, 16.2
+//   8192 steps of 64 columns: crews 102, segments about 70 (bf16), of 128: 104, 140;
+//   1024 columns of 1024 steps: whole 101, segments 139.
+// A crew has 16 warps where it has an SM to itself, else 8 (8192 steps, bf16, 128
+// columns: 104 against 127 us, 256 columns of 4096: 105 against 90 us).
 constexpr uint64_t kFewWalks = 148 * 5, kFewCrews = 104, kManyWalks = 148 * 48;
-constexpr uint32_t kLeastSegment = 64;
+constexpr uint32_t kShort = 1024, kLeastSegment = 64;
 Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
     Plan p = {};
     p.flat = q.batch * q.channels;
     p.columns = (p.flat + 32 * width - 1) / (32 * width);
     p.segments = 1, p.segment_steps = (uint32_t)q.steps;
-    if (p.columns && p.columns < kFewWalks && q.steps >= 2 * kLeastSegment) {
-        p.crew = width > 2 || p.columns < kFewCrews ? 0 : p.columns <= 148 ? 16 : 8;
-        if (!p.crew) {
+    if (p.columns && p.columns < kFewWalks && q.steps > 2 * kSteps) {
+        if (width <= 2 && (p.columns >= kFewCrews || q.steps <= kShort)) {
+            p.crew = p.columns <= 148 ? 16 : 8;
+        } else if (q.steps >= 2 * kLeastSegment) {
             const uint64_t want = std::max<uint64_t>(kLeastSegment, q.steps * p.columns / kManyWalks);
             p.segment_steps = (uint32_t)((want + kSteps - 1) / kSteps * kSteps);
             p.segments = (uint32_t)((q.steps + p.segment_steps - 1) / p.segment_steps);
@@ -240,14 +248,15 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
                                  : cudaMemsetAsync(h_last, 0, q.batch * q.channels * 4, s);
         return op_status(e, __func__);
     }
-    // Two channels a thread where every array can be read so; four of a raster.
+    // Two channels a thread where every array can be read so; four of a raster
+    // that no crew walks.
     const auto holds = [&](uint32_t n) {
         return q.channels % n == 0 && pieces(n, x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
                pieces(n, gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
                pieces(n, y, dtype_bytes(q.y_dtype), q.y_batch_stride, q.y_step_stride) && float_pieces(n, h0) &&
                float_pieces(n, h_last) && float_pieces(n, saved);
     };
-    const uint32_t width = q.x_dtype == SNN_B200_SPIKES && holds(4) ? 4 : holds(2) ? 2 : 1;
+    const uint32_t width = q.x_dtype == SNN_B200_SPIKES && !plan_of(q, 2, false).crew && holds(4) ? 4 : holds(2) ? 2 : 1;
     Args g = {};
     g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
     const cudaError_t e = run(s, q, g, plan_of(q, width, false), width, false, workspace);

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                     for (uint32_t q = 0; q < 16; ++q) {
                         if (c * 16 + q < rows)
-                            *to = from_float<T>(ok ? __fadd_rn(v[c][q], bias) : __uint_as_float(kNoValue));
+                            __stcs(to, from_float<T>(ok ? __fadd_rn(v[c][q], bias) : __uint_as_float(kNoValue)));
                         to += p.row_stride;
                     }
             }

@@ -131,17 +131,18 @@ struct Plan {
 //     crews                   3.1, 5.5   6.4, 10.0   11.1, 16.2  20.4, 28.8
 //     segments                11.2, 14.1 11.5, 14.7  12.0, 15.3  12.6, 16.2
 //   8192 steps of 64 columns: crews 102, segments about 70 (bf16), of 128: 104, 140;
-//   1024 columns of 1024 steps: whole 101, segments 139.
+//   of 1024 steps (bf16): 768 columns in crews 76, whole 109, 1024 columns 89, 108,
+//   1600 columns 135, 129; 64 steps of 1024 columns: crews 11.1, whole 9.2.
 // A crew has 16 warps where it has an SM to itself, else 8 (8192 steps, bf16, 128
 // columns: 104 against 127 us, 256 columns of 4096: 105 against 90 us).
-constexpr uint64_t kFewWalks = 148 * 5, kFewCrews = 104, kManyWalks = 148 * 48;
-constexpr uint32_t kShort = 1024, kLeastSegment = 64;
+constexpr uint64_t kFewWalks = 148 * 8, kFewShortWalks = 148 * 5, kFewCrews = 104, kManyWalks = 148 * 48;
+constexpr uint32_t kVeryShort = 256, kShort = 1024, kLeastSegment = 64;
 Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
     Plan p = {};
     p.flat = q.batch * q.channels;
     p.columns = (p.flat + 32 * width - 1) / (32 * width);
     p.segments = 1, p.segment_steps = (uint32_t)q.steps;
-    if (p.columns && p.columns < kFewWalks && q.steps > 2 * kSteps) {
+    if (p.columns && p.columns < (q.steps > kVeryShort ? kFewWalks : kFewShortWalks) && q.steps > 2 * kSteps) {
         if (width <= 2 && (p.columns >= kFewCrews || q.steps <= kShort)) {
             p.crew = p.columns <= 148 ? 16 : 8;
         } else if (q.steps >= 2 * kLeastSegment) {

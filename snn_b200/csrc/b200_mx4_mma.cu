@@ -621,9 +621,14 @@ void split_k(int device, Problem &p) {
 template <typename T>
 cudaError_t run(int device, cudaStream_t s, const Packed &x, const Packed &w, uint64_t k, Problem &p) {
     p.x_scales = x.scales;
-    // Pairs of CTAs where their tiles fill the SMs, else narrower tiles with k split.
+    // Pairs of CTAs for more than 64 rows of x, except where a long k and few
+    // tiles gain by splitting it. Measured in us, pairs and split tiles (rows of x,
+    // k, rows of w): 128 x 784 x 1000: 7.0, 12.1; 1024 x 2048 x 2048: 8.2, 14.4;
+    // 256 x 8192 x 8192: 16.0, 19.3; but 128 x 8192 x 8192: 15.9, 13.9;
+    // 300 x 8192 x 256: 15.8, 9.5; 64 x 2048 x 2048: 7.5, 6.6.
+    constexpr uint32_t kShortStages = 12;
     const uint64_t across = (w.rows + 255) / 256, high = (x.rows + kPairN - 1) / kPairN;
-    if (x.rows > 128 && w.rows > 128 && across * high * 8 >= (uint64_t)sm_count(device) * 3) {
+    if (x.rows > 64 && (p.stages <= kShortStages || (x.rows > 128 && across * high * 8 >= (uint64_t)sm_count(device)))) {
         p.tiles_n = (uint32_t)across, p.tiles_m = (uint32_t)high, p.splits = 1;
         return launch_pairs<T>(device, s, x, w, k, p);
     }

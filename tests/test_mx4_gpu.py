@@ -113,7 +113,7 @@ def product_bound(x, w):
 LINEAR = [(1, 1, 1), (1, 784, 1000), (2, 32, 8), (3, 33, 129), (4, 8192, 256), (7, 1000, 10), (16, 500, 300),
           (17, 256, 128), (31, 64, 1), (33, 1027, 200), (64, 2048, 136), (100, 128, 128), (128, 4100, 257),
           (129, 96, 130), (257, 640, 384), (300, 784, 1000), (1, 40000, 3), (1000, 1000, 10), (513, 31, 127),
-          (3300, 200, 1300), (4097, 300, 1025), (20000, 64, 250), (130, 300, 19000)]
+          (3300, 200, 1300), (4097, 300, 1025), (20000, 64, 250), (130, 300, 19000), (300, 4100, 200), (70, 5000, 130)]
 
 
 @pytest.mark.parametrize("m,k,n", LINEAR)

@@ -306,7 +306,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
             uint32_t n = 0, count = 0, s = 0, parity = 0;
             for (uint32_t tile = pair; ok && tile < tiles; tile += pairs, ++count) {
-                ok = count == 0 || bar_wait(&s_free, (count - 1) & 1);
+                // Lanes give up one by one, and the warp goes on as a whole.
+                ok = __all_sync(0xffffffffu, count == 0 || bar_wait(&s_free, (count - 1) & 1));
                 fence_after();
                 for (uint32_t at = 0; ok && at < p.stages; ++at, ++n) {
                     ok = __all_sync(0xffffffffu, bar_wait(&s_full[s], parity));

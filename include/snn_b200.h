@@ -547,7 +547,9 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
  * Types (x, gate, y): SPIKES, F32, F32; F32, F32, F32; and for T of F16 and
  * BF16: T with gate T or F32 and y T or F32. A gate without step stride is F32.
  * States, sums and products are in 32 bits. Products of gates over
- * consecutive steps are formed, so gates above one must not overflow there;
+ * consecutive steps are formed, so gates above one must not overflow there
+ * (products that become too small do no harm: an infinite state stays infinite
+ * until it meets a gate of zero);
  * of 16-bit logits beyond 87 the smaller of a and 1 - a is zero. How the work
  * is split depends on the counts, the types and the arrays' alignment, so the
  * last bits do too; the same call gives the same bits. */

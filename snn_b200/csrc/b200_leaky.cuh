@@ -338,6 +338,14 @@ __device__ __forceinline__ void walk_blocks(uint32_t t0, uint32_t t1, Fetch fetc
     }
 }
 
+// Maps hold products of gates. One that has become zero although no gate is zero
+// stays at the smallest magnitude, with its sign: times zero, an infinite state
+// would turn into NaN, where step by step it stays infinite. It adds at most 2^-149
+// of a finite state, which is what the rounding of a product so small may add too.
+__device__ __forceinline__ float kept(float product, bool zero) {
+    return product == 0.0f && !zero ? copysignf(__uint_as_float(1u), product) : product;
+}
+
 // The gates of a thread's steps. Fixed gates are kept once, and so is their
 // product over a block: each block's map has the same one, so its error acts as
 // another decay would and adds up over a long memory. Rounded once from 64 bits
@@ -373,7 +381,7 @@ struct Gates<Fixed, V> {
         static_assert(kSteps == 8, "a block's product is three squares");
         block_ = Row<V>::of([&](int q) {
             const double two = (double)a_[q] * a_[q], four = two * two;
-            return (float)(four * four);
+            return kept((float)(four * four), a_[q] == 0.0f);
         });
     }
     __device__ __forceinline__ void step_into(Row<V> &A, const Row<V> &a, int live) const {
@@ -388,6 +396,44 @@ struct Gates<Fixed, V> {
         a = a_, rest = rest_;
     }
 };
+
+template <int V>
+__device__ __forceinline__ bool any_zero(const Row<V> &A) {
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < V; ++q) any |= A[q] == 0.0f;
+    return any;
+}
+// The product P of a block's `live` gates gate(j).
+template <int V, typename Gate>
+__device__ __forceinline__ void keep(Row<V> &P, int live, Gate gate) {
+    if (!any_zero(P)) return;
+    uint32_t zero = 0;
+#pragma unroll
+    for (int j = 0; j < (int)kSteps; ++j) {
+        const Row<V> a = gate(j);
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+            if (j < live && a[q] == 0.0f) zero |= 1u << q;
+    }
+    P = Row<V>::of([&](int q) { return kept(P[q], zero >> q & 1u); });
+}
+// A map's product A joined with that of a block, whose gates are looked at again where it matters.
+template <typename G, int V>
+__device__ __forceinline__ void join(const Args &g, const Gates<G, V> &gates, Row<V> &A, Row<V> P, int live) {
+    const Row<V> both = mul(P, A);
+    if (any_zero(both)) {
+        keep<V>(P, live, [&](int j) {
+            Row<V> a, rest;
+            if (g.logit) gates.template at<true>(j, a, rest);
+            else gates.template at<false>(j, a, rest);
+            return a;
+        });
+        A = Row<V>::of([&](int q) { return kept(__fmul_rn(P[q], A[q]), P[q] == 0.0f || A[q] == 0.0f); });
+    } else {
+        A = both;
+    }
+}
 
 template <int V>
 __device__ __forceinline__ Row<V> load_row(const float *p) {
@@ -470,11 +516,13 @@ __global__ void __launch_bounds__(kWarps * 32, 6) scan_kernel(const __grid_const
             gates.take(fz, mine + slot * kSlot + kX, t0, live);
             fx.take(mine + slot * kSlot, t0, live, x);
             if constexpr (Maps) {
+                Row<V> P = all<V>(1.0f);
                 each_step<X, G, V>(g, gates, x, live, [&](int, const Row<V> &a, const Row<V> &u) {
-                    gates.step_into(A, a, live);
+                    gates.step_into(P, a, live);
                     h = fma(a, h, u);
                 });
-                gates.block_into(A, live);
+                gates.block_into(P, live);
+                join(g, gates, A, P, live);
             } else if (p.on) {
                 if (g.saved) store_row<V>(saved_at(g, p, t0), h);
                 Y *y = (Y *)g.y + p.b * g.yb + (int64_t)t0 * g.yt + p.c;
@@ -595,6 +643,7 @@ __global__ void __launch_bounds__(N * 32) scan_crew_kernel(const __grid_constant
                 });
                 gates.block_into(A, live);
             }
+            keep<V>(A, live, [&](int j) { return a[j]; });
             h = crew_state<V, N>(s_crew, n, A, H, first);
             if (on && p.on) {
                 if (g.saved) store_row<V>(saved_at(g, p, t0), h);
@@ -751,17 +800,19 @@ __global__ void __launch_bounds__(kWarps * 32, Maps ? 6 : 4) back_kernel(const _
             b.gates.take(fz, mine + slot * kSlot + kY, t0, live);
             fy.take(mine + slot * kSlot, t0, live, b.dy);
             if constexpr (Maps) {
+                Row<V> P = all<V>(1.0f);
                 with_flags(g, [&](auto logit, auto) {
 #pragma unroll
                     for (int j = (int)kSteps - 1; j >= 0; --j)
                         if (j < live) {
                             Row<V> a, rest;
                             b.gates.template at<logit.value>(j, a, rest);
-                            b.gates.step_into(A, a, live);
+                            b.gates.step_into(P, a, live);
                             e = mul(a, add(widen(b.dy[j]), e));
                         }
                 });
-                b.gates.block_into(A, live);
+                b.gates.block_into(P, live);
+                join(g, b.gates, A, P, live);
             } else {
                 const Row<V> h = load_row<V>((const float *)(mine + slot * kSlot + kS) + (threadIdx.x & 31) * V);
                 Vec<X, V> x[kSteps];
@@ -830,6 +881,7 @@ __global__ void __launch_bounds__(N * 32) back_crew_kernel(const __grid_constant
 #pragma unroll
                 for (int j = (int)kSteps - 1; j >= 0; --j) b.gates.step_into(A, b.a[j], live), b.step(j, live, E);
                 b.gates.block_into(A, live);
+                keep<V>(A, live, [&](int j) { return b.a[j]; });
             }
             e = crew_state<V, N>(s_crew, n, A, E, first);
             if (on) {

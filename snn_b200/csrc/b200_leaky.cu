@@ -172,6 +172,9 @@ Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
     p.states = p.maps + round(cut * 8);
     p.partial = p.states + round(cut * 4);
     p.bytes = p.partial + (back && !q.gate_step_stride ? round(p.partials * p.flat * 4) : 0);
+    // Crews need no workspace of their own, but a call that they walk is refused without
+    // one all the same: it stays so, with the least there is.
+    if (p.crew) p.bytes = std::max<uint64_t>(p.bytes, 256);
     return p;
 }
 
@@ -238,7 +241,9 @@ snn_size_t snn_b200_leaky_saved_floats(snn_size_t batch, snn_size_t steps, snn_s
 
 snn_size_t snn_b200_leaky_workspace(const snn_b200_leaky_t *q, int backward) {
     if (q == nullptr || q->batch > kMaxCount || q->steps > kMaxCount || q->channels > kMaxCount) return 0;
-    return std::max({plan_of(*q, 1, backward).bytes, plan_of(*q, 2, backward).bytes, plan_of(*q, 4, backward).bytes});
+    const uint64_t need = std::max(plan_of(*q, 1, backward).bytes, plan_of(*q, 2, backward).bytes);
+    // Four channels a thread walk rasters only, and forward only.
+    return q->x_dtype == SNN_B200_SPIKES && !backward ? std::max(need, plan_of(*q, 4, false).bytes) : need;
 }
 
 snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_leaky_t *leaky, const void *x,

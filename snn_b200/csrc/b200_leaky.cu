@@ -149,6 +149,9 @@ struct Plan {
 //   1600 columns 135, 129; 64 steps of 1024 columns: crews 11.1, whole 9.2.
 // A crew has 16 warps where it has an SM to itself, else 8 (8192 steps, bf16, 128
 // columns: 104 against 127 us, 256 columns of 4096: 105 against 90 us).
+// Walks are counted two channels a thread, also of the rasters that four are walked of
+// (1000 channels, a leak each, whole and in segments: 64 sequences of 200 steps 15, 51 us,
+// 128 of 400 steps 49, 124 us).
 constexpr uint64_t kFewWalks = 148 * 8, kFewShortWalks = 148 * 5, kFewCrews = 104, kManyWalks = 148 * 48;
 constexpr uint32_t kVeryShort = 256, kShort = 1024, kLeastSegment = 64;
 Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
@@ -156,8 +159,9 @@ Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
     p.flat = q.batch * q.channels;
     p.columns = (p.flat + 32 * width - 1) / (32 * width);
     p.segments = 1, p.segment_steps = (uint32_t)q.steps;
-    if (p.columns && p.columns < (q.steps > kVeryShort ? kFewWalks : kFewShortWalks) && q.steps > 2 * kSteps) {
-        if (width <= 2 && (p.columns >= kFewCrews || q.steps <= kShort)) {
+    const uint64_t walks = width == 4 ? (p.flat + 63) / 64 : p.columns;
+    if (walks && walks < (q.steps > kVeryShort ? kFewWalks : kFewShortWalks) && q.steps > 2 * kSteps) {
+        if (walks >= kFewCrews || q.steps <= kShort) {
             p.crew = p.columns <= 148 ? 16 : 8;
         } else if (q.steps >= 2 * kLeastSegment) {
             const uint64_t want = std::max<uint64_t>(kLeastSegment, q.steps * p.columns / kManyWalks);
@@ -203,14 +207,19 @@ bool wide_rows(const void *p, int dtype, uint64_t channels, int64_t sb, int64_t 
     return channels % n == 0 && pieces(n, p, dtype_bytes(dtype), sb, st);
 }
 
+// Of x, of a gate for every step and, backward, of dy.
+bool wide_rows(const snn_b200_leaky_t &q, const Args &g, bool back) {
+    return wide_rows(g.x, q.x_dtype, q.channels, q.x_batch_stride, q.x_step_stride) &&
+           (!(g.gate && q.gate_step_stride) ||
+            wide_rows(g.gate, q.gate_dtype, q.channels, q.gate_batch_stride, q.gate_step_stride)) &&
+           (!back || wide_rows(g.dy, q.y_dtype, q.channels, q.dy_batch_stride, q.dy_step_stride));
+}
+
 cudaError_t run(cudaStream_t s, const snn_b200_leaky_t &q, Args &g, const Plan &p, uint32_t width, bool back,
                 void *workspace) {
     fill(g, q, p, workspace);
-    const bool every = g.gate && q.gate_step_stride;
-    g.wide = wide_rows(g.x, q.x_dtype, q.channels, q.x_batch_stride, q.x_step_stride) &&
-             (!every || wide_rows(g.gate, q.gate_dtype, q.channels, q.gate_batch_stride, q.gate_step_stride)) &&
-             (!back || wide_rows(g.dy, q.y_dtype, q.channels, q.dy_batch_stride, q.dy_step_stride));
-    const Form f = {q.gate_dtype, q.y_dtype, every, width};
+    g.wide = wide_rows(q, g, back);
+    const Form f = {q.gate_dtype, q.y_dtype, g.gate && q.gate_step_stride, width};
     switch (q.x_dtype) {
         case SNN_B200_F32: return back ? backward_f32(s, f, g) : forward_f32(s, f, g);
         case SNN_B200_F16: return back ? backward_f16(s, f, g) : forward_f16(s, f, g);
@@ -268,17 +277,21 @@ snn_status_t snn_b200_leaky_scan_async(int device, void *stream, const snn_b200_
                                  : cudaMemsetAsync(h_last, 0, q.batch * q.channels * 4, s);
         return op_status(e, __func__);
     }
-    // Two channels a thread where every array can be read so; four of a raster
-    // that no crew walks.
+    Args g = {};
+    g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
+    // Two channels a thread where every array can be read so; four of a raster that no
+    // crew walks, as two of them are too few bytes to be copied ahead (2000 x 25 x 1000: 46
+    // against 82 us). Not with a gate for every step where rows are copied in pieces of 16
+    // bytes anyway (762 x 200 x 1008: 311 against 229 us; of 1000 channels 348, 345).
     const auto holds = [&](uint32_t n) {
         return q.channels % n == 0 && pieces(n, x, dtype_bytes(q.x_dtype), q.x_batch_stride, q.x_step_stride) &&
                pieces(n, gate, dtype_bytes(q.gate_dtype), q.gate_batch_stride, q.gate_step_stride) &&
                pieces(n, y, dtype_bytes(q.y_dtype), q.y_batch_stride, q.y_step_stride) && float_pieces(n, h0) &&
                float_pieces(n, h_last) && float_pieces(n, saved);
     };
-    const uint32_t width = q.x_dtype == SNN_B200_SPIKES && !plan_of(q, 2, false).crew && holds(4) ? 4 : holds(2) ? 2 : 1;
-    Args g = {};
-    g.x = x, g.gate = gate, g.h0 = h0, g.lengths = lengths, g.y = y, g.h_last = h_last, g.saved = saved;
+    const bool four = q.x_dtype == SNN_B200_SPIKES && !plan_of(q, 2, false).crew &&
+                      !(gate && q.gate_step_stride && wide_rows(q, g, false)) && holds(4);
+    const uint32_t width = four ? 4 : holds(2) ? 2 : 1;
     const cudaError_t e = run(s, q, g, plan_of(q, width, false), width, false, workspace);
     return op_status(e, __func__);
 }

@@ -35,3 +35,10 @@ def test_crews_ask_for_no_segments(b, t, c, crew):
 def test_segments_ask_for_their_maps_and_states():
     # 64 steps a segment; a map of 8 bytes and a state of 4 a channel and segment.
     assert workspace(1, 6400, 800, F32, True, 0) == 100 * 800 * 12
+
+
+@pytest.mark.parametrize("step_gate", [False, True])
+@pytest.mark.parametrize("b,t,c", [(64, 200, 1000), (128, 400, 1024), (100, 2000, 1000), (46, 200, 1040), (151, 257, 1000)])
+def test_rasters_are_cut_like_other_sequences(b, t, c, step_gate):
+    """Four channels a thread are half the columns, not a reason for segments."""
+    assert workspace(b, t, c, SPIKES, step_gate, 0) == workspace(b, t, c, F32, step_gate, 0) == 0

@@ -233,8 +233,9 @@ struct Sequence {
     bool every = false;
 
     // x, gate, decay, lengths, logit, complement, input_scale from argument i on.
-    // A gate expanded over the sequences or the steps is read where it is; for
-    // its gradient (whole) it becomes an array with an element for each of them.
+    // A gate expanded over the sequences or the steps is read where it is (one of x's
+    // 16-bit type over the steps in 32 bits, as gates without a step stride are); for its gradient
+    // (whole) it becomes an array with an element for each of them.
     Sequence(const Args &a, int i, bool whole) : x(a.tensor(i)), gate(a.tensor(i + 1, true)), lengths(a.tensor(i + 3, true)) {
         dev = shared_device(x, gate, lengths);
         require(x.dim() == 3, "leaky: [batch, steps, channels] expected");
@@ -245,7 +246,7 @@ struct Sequence {
         q.logit = a.flag(i + 4), q.complement = a.flag(i + 5), q.input_scale = (float)a.number(i + 6);
         require(gate.defined() != !a.none(i + 2), "leaky: either a gate array or a decay is needed");
         if (gate.defined()) {
-            const int64_t d = gate.dim();
+            int64_t d = gate.dim();
             require(d >= 1 && d <= 3 && gate.size(-1) == x.size(2) && (d < 2 || gate.size(0) == x.size(0)) &&
                         (d < 3 || gate.size(1) == x.size(1)),
                     "leaky: a gate of shape [channels], [batch, channels] or [batch, steps, channels] expected");
@@ -253,6 +254,8 @@ struct Sequence {
             const int64_t c = x.size(2) ? x.size(2) : 1;  // of a dimension that is one long: not shared
             if (whole && d > 1 && (stride(gate, 0, c) == 0 || (d > 2 && stride(gate, 1, c) == 0)))
                 gate = gate.clone(at::MemoryFormat::Contiguous);
+            if (d > 2 && stride(gate, 1, c) == 0 && q.x_dtype != SNN_B200_SPIKES && gate.scalar_type() == x.scalar_type())
+                gate = gate.select(1, 0).to(at::kFloat), d = 2;
             q.gate_dtype = code(gate);
             q.gate_batch_stride = d > 1 ? stride(gate, 0, c) : 0, q.gate_step_stride = d > 2 ? stride(gate, 1, c) : 0;
             every = q.gate_step_stride != 0;
@@ -345,7 +348,11 @@ PyObject *step(Args a) {
         require((d == 1 || (d == 2 && gate0.size(0) == b)) && gate0.size(-1) == c,
                 "leaky_step: a gate of shape [channels] or [batch, channels] expected");
         gate = rows(gate0);
-        gate_stride = d == 2 ? stride(gate, 0, c ? c : 1) : 0, gate_type = code(gate);
+        gate_stride = d == 2 ? stride(gate, 0, c ? c : 1) : 0;
+        // Expanded over the rows: in 32 bits, as gates without a row stride are.
+        if (d == 2 && gate_stride == 0 && type != SNN_B200_SPIKES && gate.scalar_type() == x.scalar_type())
+            gate = gate.select(0, 0).to(at::kFloat);
+        gate_type = code(gate);
     }
     if (slots.defined())
         require(slots.scalar_type() == at::kInt && slots.dim() == 1 && slots.size(0) == b && slots.is_contiguous(),

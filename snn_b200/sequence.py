@@ -123,9 +123,10 @@ def leaky_scan(x, gate=None, *, decay: float | None = None, h0=None, lengths=Non
                complement: bool = False, input_scale: float = 1.0, dtype=None, save: bool = False):
     """h[t] = a[t] h[t-1] + input_scale x[t] (times 1 - a[t] with
     `complement`) over x [batch, steps, channels]: returns (h, h_last), and
-    with `save` also what leaky_scan_backward needs. The gate ([channels],
-    [batch, channels] or [batch, steps, channels]) holds a, or its logits with
-    `logit`; `decay` is one a for all. h is of x's type (float32 for spikes)
+    with `save` also what leaky_scan_backward needs. The gate ([channels] or
+    [batch, channels] in float32, or [batch, steps, channels], which may be of
+    x's 16-bit type too) holds a, or its logits with `logit`; `decay` is one a
+    for all. h is of x's type (float32 for spikes)
     or of `dtype`; rows at or behind lengths[b] are zero there."""
     return (_OPS or _ops()).scan(x, gate, decay, lengths, logit, complement, input_scale, h0, dtype, save)
 
@@ -145,6 +146,7 @@ def leaky_step(x, gate=None, pool=None, *, slots=None, decay: float | None = Non
     """One step of x [batch, channels]: pool[slots[i]] (pool [slot_count,
     channels], float32, updated in place; without `slots` pool[i]) becomes
     a pool[slots[i]] + input_scale x[i] (times 1 - a with `complement`), which
-    is returned. The gate is [channels] or [batch, channels]. Rows with a slot
-    outside the pool are padding (zero)."""
+    is returned. The gate is [channels] in float32, or [batch, channels], which
+    may be of x's 16-bit type too. Rows with a slot outside the pool are padding
+    (zero)."""
     return (_OPS or _ops()).step(x, gate, pool, slots, decay, logit, complement, input_scale, dtype)

@@ -63,7 +63,15 @@ struct Args {
             return Tensor();
         }
         require(THPVariable_Check(v[i]), "a tensor expected");
-        return THPVariable_Unpack(v[i]);
+        const Tensor &t = THPVariable_Unpack(v[i]);
+        return t.is_neg() ? t.resolve_neg() : t;  // a sign that is only noted is not in memory
+    }
+    // One that is written to.
+    Tensor place(int i) const {
+        require(THPVariable_Check(v[i]), "a tensor expected");
+        const Tensor &t = THPVariable_Unpack(v[i]);
+        require(!t.is_neg(), "a tensor whose sign is only noted cannot be written to");
+        return t;
     }
     bool none(int i) const { return v[i] == Py_None; }
     bool flag(int i) const {
@@ -137,7 +145,7 @@ PyObject *quantize(Args a) {
     if (make) {
         codes = empty({(int64_t)nc}, at::kByte, x), scales = empty({(int64_t)ns}, at::kByte, x);
     } else {
-        codes = a.tensor(1), scales = a.tensor(2);
+        codes = a.place(1), scales = a.place(2);
         shared_device(x, codes, scales);
         require(codes.nbytes() == nc && scales.nbytes() == ns && codes.is_contiguous() && scales.is_contiguous(),
                 "mx4_quantize: `out` is of another shape");
@@ -332,7 +340,7 @@ PyObject *scan_backward(Args a) {
 
 // (x, gate, pool, slots, decay, logit, complement, input_scale, dtype)
 PyObject *step(Args a) {
-    const Tensor x0 = a.tensor(0), gate0 = a.tensor(1, true), pool = a.tensor(2), slots = a.tensor(3, true);
+    const Tensor x0 = a.tensor(0), gate0 = a.tensor(1, true), pool = a.place(2), slots = a.tensor(3, true);
     const int dev = shared_device(x0, gate0, pool, slots), type = code(x0);
     require(x0.dim() == 2 && pool.dim() == 2 && pool.scalar_type() == at::kFloat && pool.size(1) == x0.size(1) &&
                 (pool.stride(1) == 1 || pool.size(1) <= 1),

@@ -176,9 +176,9 @@ Plan plan_of(const snn_b200_leaky_t &q, uint32_t width, bool back) {
     p.states = p.maps + round(cut * 8);
     p.partial = p.states + round(cut * 4);
     p.bytes = p.partial + (back && !q.gate_step_stride ? round(p.partials * p.flat * 4) : 0);
-    // Crews need no workspace of their own, but a call that they walk is refused without
-    // one all the same: it stays so, with the least there is.
-    if (p.crew) p.bytes = std::max<uint64_t>(p.bytes, 256);
+    // Crews need no workspace of their own, but a call of so many steps that they walk is
+    // refused without one all the same: it stays so, with the least there is.
+    if (p.crew && q.steps >= 2 * kLeastSegment) p.bytes = std::max<uint64_t>(p.bytes, 256);
     return p;
 }
 

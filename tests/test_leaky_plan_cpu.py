@@ -32,6 +32,12 @@ def test_crews_ask_for_no_segments(b, t, c, crew):
         assert workspace(b, t, c, x, False, 1) == max(256, (crew * b * c * 4 + 255) // 256 * 256)
 
 
+def test_short_sequences_in_crews_ask_for_none():
+    for b, t, c in ((2, 30, 64), (100, 127, 300)):
+        assert workspace(b, t, c, F32, False, 0) == workspace(b, t, c, SPIKES, True, 0) == 0
+        assert workspace(b, t, c, F32, True, 1) == 0
+
+
 def test_segments_ask_for_their_maps_and_states():
     # 64 steps a segment; a map of 8 bytes and a state of 4 a channel and segment.
     assert workspace(1, 6400, 800, F32, True, 0) == 100 * 800 * 12

@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <Python.h>
@@ -52,6 +54,38 @@ int code(const Tensor &t) {
     const int c = code_of(t.scalar_type());
     require(c >= 0, "element type is not one of float32, float16, bfloat16, uint8, bool");
     return c;
+}
+
+// ---- autograd ----
+// The operators have no autograd formulas: gradients come from calls of their own.
+// A result of tensors that require a gradient says so, and going back through it
+// is an error; without a history it would only leave their gradients empty.
+struct NoFormula : torch::autograd::Node {
+    const char *text;
+    explicit NoFormula(const char *t) : text(t) {}
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&) override {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, text);
+    }
+    std::string name() const override { return "SequenceOperator"; }
+};
+template <typename... T>
+bool wants_gradient(const T &...inputs) {
+    return at::GradMode::is_enabled() && ((inputs.defined() && inputs.requires_grad()) || ...);
+}
+template <typename... T>
+std::shared_ptr<NoFormula> no_formula(const char *text, const T &...inputs) {
+    if (!wants_gradient(inputs...)) return nullptr;
+    std::shared_ptr<NoFormula> f(new NoFormula(text), torch::autograd::deleteNode);
+    f->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    return f;
+}
+Tensor &behind(Tensor &result, const std::shared_ptr<NoFormula> &f) {
+    if (f && result.defined()) torch::autograd::set_history(result, f);
+    return result;
+}
+// What a call has written to in place is another version of itself.
+void written(const Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // Arguments are borrowed; None is an undefined tensor.
@@ -153,7 +187,10 @@ PyObject *quantize(Args a) {
     check(snn_b200_mx4_quantize_async(dev, stream_of(dev), data(x), type, x.size(0), x.size(1), x.stride(0),
                                       x.stride(1), out(codes), out(scales)),
           "snn_b200_mx4_quantize_async");
-    if (!make) Py_RETURN_NONE;
+    if (!make) {
+        written(codes), written(scales);
+        Py_RETURN_NONE;
+    }
     PyObject *c = THPVariable_Wrap(std::move(codes)), *s = THPVariable_Wrap(std::move(scales));
     return Py_BuildValue("(NN)", c, s);
 }
@@ -198,6 +235,7 @@ PyObject *matmul(Args a) {
     check(snn_b200_mx4_matmul_async(dev, stream_of(dev), data(x.codes), data(x.scales), x.rows, data(w.codes),
                                     data(w.scales), w.rows, w.cols, bias_of(bias, w.rows), out(y), code(y), w.rows),
           "snn_b200_mx4_matmul_async");
+    behind(y, no_formula("mx4_matmul has no gradient: pass detached tensors", bias));
     return THPVariable_Wrap(std::move(y));
 }
 
@@ -210,7 +248,9 @@ PyObject *linear(Args a) {
     int64_t m = 1;
     for (int64_t d = 0; d + 1 < x.dim(); ++d) m *= x.size(d);
     const Tensor flat = x.dim() == 2 ? x : x.reshape({m, w.cols});
-    Tensor y = empty({m, w.rows}, a.dtype(6, result_type(x)), x);
+    auto shape = x.sizes().vec();
+    shape.back() = w.rows;
+    Tensor y = empty(shape, a.dtype(6, result_type(x)), x);
     const snn_size_t need =
         snn_b200_mx4_linear_workspace(data(flat), type, m, w.cols, flat.stride(0), flat.stride(1));
     const Tensor ws = scratch(need, x);
@@ -218,11 +258,7 @@ PyObject *linear(Args a) {
                                     data(w.codes), data(w.scales), w.rows, bias_of(bias, w.rows), out(y), code(y),
                                     w.rows, out(ws), need),
           "snn_b200_mx4_linear_async");
-    if (x.dim() != 2) {
-        auto shape = x.sizes().vec();
-        shape.back() = w.rows;
-        y = y.view(shape);
-    }
+    behind(y, no_formula("mx4_linear has no gradient: pass detached tensors", x, bias));
     return THPVariable_Wrap(std::move(y));
 }
 
@@ -230,7 +266,8 @@ PyObject *linear(Args a) {
 // An empty [batch, steps, channels] tensor whose steps come first in memory where x's do.
 Tensor like(const Tensor &x, at::ScalarType t) {
     const int64_t b = x.size(0), n = x.size(1), c = x.size(2);
-    if (b > 1 && n > 1 && x.stride(0) < x.stride(1)) return empty({n, b, c}, t, x).transpose(0, 1);
+    if (b > 1 && n > 1 && x.stride(0) < x.stride(1))
+        return at::empty_strided({b, n, c}, {c, b * c, 1}, x.options().dtype(t).memory_format(c10::nullopt));
     return empty({b, n, c}, t, x);
 }
 
@@ -299,6 +336,9 @@ PyObject *scan(Args a) {
     check(snn_b200_leaky_scan_async(s.dev, stream_of(s.dev), &s.q, data(s.x), data(s.gate), (const float *)data(h0),
                                     s.length(), out(y), (float *)out(h_last), (float *)out(saved), out(ws), need),
           "snn_b200_leaky_scan_async");
+    const auto f = no_formula("leaky_scan has no autograd formula: its gradients come from leaky_scan_backward",
+                              a.tensor(0), a.tensor(1, true), given);
+    behind(y, f), behind(h_last, f);
     PyObject *py = THPVariable_Wrap(std::move(y)), *ph = THPVariable_Wrap(std::move(h_last));
     if (!save) return Py_BuildValue("(NN)", py, ph);
     return Py_BuildValue("(NNN)", py, ph, THPVariable_Wrap(std::move(saved)));
@@ -334,6 +374,9 @@ PyObject *scan_backward(Args a) {
                                              (const float *)data(saved), data(dy), (const float *)data(dh_last), out(dx),
                                              out(dgate), (float *)out(dh0), out(ws), need),
           "snn_b200_leaky_scan_backward_async");
+    // x and the gate ordinarily require a gradient here: this one. Of dy and dh_last it would be a second.
+    const auto f = no_formula("leaky_scan_backward has no gradient of its own", a.tensor(7), given);
+    behind(dx, f), behind(dgate, f), behind(dh0, f);
     PyObject *pz = dgate.defined() ? THPVariable_Wrap(std::move(dgate)) : Py_NewRef(Py_None);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(dx)), pz, THPVariable_Wrap(std::move(dh0)));
 }
@@ -345,6 +388,7 @@ PyObject *step(Args a) {
     require(x0.dim() == 2 && pool.dim() == 2 && pool.scalar_type() == at::kFloat && pool.size(1) == x0.size(1) &&
                 (pool.stride(1) == 1 || pool.size(1) <= 1),
             "leaky_step: x [batch, channels] and a float32 pool [slot_count, channels] with neighbouring channels expected");
+    require(!wants_gradient(pool), "leaky_step: a pool that requires a gradient cannot be updated in place");
     const int64_t b = x0.size(0), c = x0.size(1);
     const Tensor x = rows(x0);
     require(gate0.defined() != !a.none(4), "leaky_step: either a gate array or a decay is needed");
@@ -371,6 +415,8 @@ PyObject *step(Args a) {
                                     gate0.defined() ? 0.0f : (float)a.number(4), (float)a.number(7), (float *)out(pool),
                                     pool.stride(0), (const int32_t *)data(slots), out(y), code(y), c),
           "snn_b200_leaky_step_async");
+    written(pool);
+    behind(y, no_formula("leaky_step has no gradient: pass detached tensors", x0, gate0));
     return THPVariable_Wrap(std::move(y));
 }
 

@@ -9,6 +9,12 @@ A tensor of uint8 or bool is a spike raster (non-zero = one spike).
     current = mx4_linear(raster, w)            # [rows, pre] -> [rows, post]
     y, h_last = leaky_scan(current, decays)    # [batch, steps, channels]
 
+None of them has an autograd formula. A result of tensors that require a
+gradient carries that on, and going back through it raises NotImplementedError:
+gradients come from leaky_scan_backward (in a torch.autograd.Function, say).
+leaky_scan_backward's own results are plain, unless dy or dh_last require a
+gradient. What is updated in place (a pool, `out`) counts as a new version.
+
 The checks and the calls are compiled (csrc/torch/sequence_ops.cpp, built to
 _lib/sequence_ops.so); torch is imported when an operator is first called.
 """

@@ -550,7 +550,8 @@ snn_status_t snn_b200_mx4_linear_async(int device, void *stream, const void *x, 
  * consecutive steps are formed, so gates above one must not overflow there
  * (products that become too small do no harm: an infinite state stays infinite
  * until it meets a gate of zero);
- * of 16-bit logits beyond 87 the smaller of a and 1 - a is zero. How the work
+ * of 16-bit logits the smaller of a and 1 - a is within 2^-19 of itself up to
+ * 22, within 2^-17 up to 87 and zero beyond. How the work
  * is split depends on the counts, the types and the arrays' alignment, so the
  * last bits do too; the same call gives the same bits. */
 typedef struct snn_b200_leaky {

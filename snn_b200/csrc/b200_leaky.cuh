@@ -149,9 +149,12 @@ struct Fixed {};
 
 // The gate and one minus it from gates z. Of logits, both come from one
 // exponential of a non-positive number, so that neither is a difference of
-// nearly equal values. A 16-bit logit has a rounding of 2^-9 of itself, so for it
-// the product with log2(e) is rounded once to 32 bits (2^-20 of the exponential
-// up to logits of 22).
+// nearly equal values. For a 16-bit logit the product with log2(e) is rounded
+// once to 32 bits: half a unit of it is a share of 2^-19.8 of the exponential up to
+// logits of 22 and of 2^-17.9 up to 87, the hardware exponential's own 2^-22.5 with it. The
+// logit's own rounding, 2^-9 of itself in bf16 and 2^-12 in f16, moves the exponential of
+// such logits by shares of 2^-5 and 2^-8; the low part of the product would cost every
+// element two to four instructions of about thirty.
 template <typename G, bool Logit, int V>
 __device__ __forceinline__ void leak_of(const Vec<G, V> &z, Row<V> &a, Row<V> &rest) {
     if constexpr (!Logit) {

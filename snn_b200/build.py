@@ -8,7 +8,8 @@ on which libcudart the host process (e.g. PyTorch) already loaded. NCCL is the
 one the installed PyTorch uses (the nvidia-nccl wheel), found through an
 rpath, so a process that also runs torch.distributed loads a single NCCL.
 snn_b200/_lib/sequence_ops.so, the sequence operators for torch tensors, is
-built beside it with g++ against the installed PyTorch.
+built beside it with g++ against the installed PyTorch, and again when another
+PyTorch or Python is found; without a CUDA build of PyTorch it is left out.
 """
 from __future__ import annotations
 
@@ -64,19 +65,35 @@ def _newer(src_files, target) -> bool:
     return any(os.path.getmtime(f) > t for f in src_files)
 
 
-def torch_dir() -> str:
+def torch_dir() -> str | None:
+    """The installed PyTorch, if it has headers and was built for CUDA."""
     for p in sys.path:
         d = os.path.join(p, "torch")
         if os.path.exists(os.path.join(d, "include", "ATen", "ATen.h")):
-            return d
-    raise RuntimeError("PyTorch's headers not found")
+            return d if os.path.exists(os.path.join(d, "lib", "libc10_cuda.so")) else None
+    return None
+
+
+def torch_stamp(t: str) -> str:
+    """What the binary of the tensor operators depends on beside its sources."""
+    with open(os.path.join(t, "version.py")) as f:
+        return f"{sys.implementation.cache_tag} {t}\n{f.read()}"
 
 
 def build_torch_ops(headers, force: bool, verbose: bool) -> None:
-    src = os.path.join(CSRC, "torch", "sequence_ops.cpp")
-    if not (force or _newer([src] + headers, TORCH_OPS)):
-        return
     t = torch_dir()
+    if t is None:
+        print(f"PyTorch for CUDA not found: {os.path.basename(TORCH_OPS)} (operators on torch tensors) not built",
+              file=sys.stderr)
+        return
+    src = os.path.join(CSRC, "torch", "sequence_ops.cpp")
+    stamp, now = os.path.join(OBJ_DIR, "sequence_ops.stamp"), torch_stamp(t)
+    same = False
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            same = f.read() == now
+    if not (force or not same or _newer([src] + headers, TORCH_OPS)):
+        return
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I", os.path.join(ROOT, "include"),
            "-I", os.path.join(t, "include"), "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"),
@@ -86,6 +103,8 @@ def build_torch_ops(headers, force: bool, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
+    with open(stamp, "w") as f:
+        f.write(now)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

@@ -26,7 +26,6 @@ import os
 from . import HERE, SNN_ERR_CUDA, SnnError, _check, last_error, lib
 
 OPS_PATH = os.path.join(HERE, "_lib", "sequence_ops.so")
-LEAKY_BLOCK = 8  # SNN_B200_LEAKY_BLOCK
 
 _OPS = None
 

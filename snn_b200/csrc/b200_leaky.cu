@@ -15,12 +15,7 @@ namespace {
 // those of the runs before onto the first state, and walks its run again. Runs of
 // up to kHeld maps stay in registers, all of them under way at once (with 8 under
 // way and two passes over them it took 10 us for 444 segments of 1024 channels).
-// The maps' gates stay from zero as in the walks.
 constexpr uint32_t kCarryWarps = 32, kHeld = 16;
-__device__ __forceinline__ float joined(float a, float b) {
-    const float p = __fmul_rn(a, b);
-    return p == 0.0f && a != 0.0f && b != 0.0f ? copysignf(__uint_as_float(1u), p) : p;
-}
 __global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *maps, uint32_t segments, uint64_t flat,
                                                                  const float *first, float *states, bool back) {
     __shared__ float2 s_run[kCarryWarps][32];
@@ -41,9 +36,10 @@ __global__ void __launch_bounds__(kCarryWarps * 32) carry_kernel(const float2 *m
             m.y = __fmaf_rn(held[n].x, m.y, held[n].y);
         }
         if (x == 0.0f) {
-            x = m.x;
+            bool zero = m.x == 0.0f;
 #pragma unroll
-            for (uint32_t n = 0; n < kHeld; ++n) x = joined(held[n].x, x);
+            for (uint32_t n = 0; n < kHeld; ++n) zero |= held[n].x == 0.0f;
+            x = kept(x, zero);
         }
         m.x = x;
     }

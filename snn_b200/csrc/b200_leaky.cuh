@@ -341,14 +341,6 @@ __device__ __forceinline__ void walk_blocks(uint32_t t0, uint32_t t1, Fetch fetc
     }
 }
 
-// Maps hold products of gates. One that has become zero although no gate is zero
-// stays at the smallest magnitude, with its sign: times zero, an infinite state
-// would turn into NaN, where step by step it stays infinite. It adds at most 2^-149
-// of a finite state, which is what the rounding of a product so small may add too.
-__device__ __forceinline__ float kept(float product, bool zero) {
-    return product == 0.0f && !zero ? copysignf(__uint_as_float(1u), product) : product;
-}
-
 // The gates of a thread's steps. Fixed gates are kept once, and so is their
 // product over a block: each block's map has the same one, so its error acts as
 // another decay would and adds up over a long memory. Rounded once from 64 bits
@@ -425,7 +417,9 @@ __device__ __forceinline__ void keep(Row<V> &P, int live, Gate gate) {
 template <typename G, int V>
 __device__ __forceinline__ void join(const Args &g, const Gates<G, V> &gates, Row<V> &A, Row<V> P, int live) {
     const Row<V> both = mul(P, A);
-    if (any_zero(both)) {
+    if constexpr (std::is_same<G, Fixed>::value) {
+        A = Row<V>::of([&](int q) { return kept(both[q], gates.a_[q] == 0.0f); });
+    } else if (any_zero(both)) {
         keep<V>(P, live, [&](int j) {
             Row<V> a, rest;
             if (g.logit) gates.template at<true>(j, a, rest);

@@ -31,6 +31,14 @@ struct Args {
     float *partial;                    // backward: sums of a shared gate's gradient, [segments, or warps of a crew][flat]
 };
 
+// Maps hold products of gates. One that has become zero although no gate is zero
+// stays at the smallest magnitude, with its sign: times zero, an infinite state
+// would turn into NaN, where step by step it stays infinite. It adds at most 2^-149
+// of a finite state, which is what the rounding of a product so small may add too.
+__device__ __forceinline__ float kept(float product, bool zero) {
+    return product == 0.0f && !zero ? copysignf(__uint_as_float(1u), product) : product;
+}
+
 // x's type is the translation unit's; g and y are snn_b200_dtype_t, `every`
 // says that the gate has a value for every step. width: channels a thread
 // holds.

@@ -601,7 +601,9 @@ snn_status_t snn_b200_leaky_scan_backward_async(int device, void *stream, const 
  * the new state to y. x, gate and y rows have their own strides, a
  * gate_row_stride of 0 shares the gate; types as above. Rows whose slot is
  * outside [0, slot_count) are padding: y is zero and no state changes. Rows
- * that name the same slot are applied in row order. */
+ * that name the same slot are applied in row order. With slots the time grows
+ * with the square of the rows, of which there may be 2^22 (SNN_ERR_OVERFLOW
+ * above); without them it does not. */
 snn_status_t snn_b200_leaky_step_async(int device, void *stream, snn_size_t batch, snn_size_t slot_count,
                                        snn_size_t channels, const void *x, int x_dtype, int64_t x_row_stride,
                                        const void *gate, int gate_dtype, int64_t gate_row_stride, int logit,

@@ -93,6 +93,10 @@ __global__ void __launch_bounds__(kSumWarps * 32) gate_sum_kernel(const float *p
     }
 }
 
+// Every CTA of a step looks through all slots, eight rows to a CTA: 131,072 rows take 3.1
+// ms, so this many about three seconds, and as many as other counts may be days.
+constexpr snn_size_t kMostNamedRows = 1ull << 22;
+
 // The listed combinations of types. Without a gate array its type is not looked at.
 bool types_listed(int x, bool has_gate, int gate, int y, bool gate_every_step) {
     if (x == SNN_B200_SPIKES || x == SNN_B200_F32)
@@ -362,6 +366,7 @@ snn_status_t snn_b200_leaky_step_async(int device, void *stream, snn_size_t batc
                                        int64_t y_row_stride) {
     if (device < 0) return SNN_ERR_INVALID_ARGUMENT;
     if (batch > kMaxCount || slot_count > kMaxCount || channels > kMaxCount) return SNN_ERR_OVERFLOW;
+    if (slots && batch > kMostNamedRows) return SNN_ERR_OVERFLOW;
     if (!is_dtype(x_dtype) || !is_float_dtype(y_dtype) || (gate && !is_float_dtype(gate_dtype)))
         return SNN_ERR_INVALID_ARGUMENT;
     if (!types_listed(x_dtype, gate != nullptr, gate_dtype, y_dtype, gate_row_stride != 0)) return SNN_ERR_UNSUPPORTED;

@@ -48,3 +48,11 @@ def test_segments_ask_for_their_maps_and_states():
 def test_rasters_are_cut_like_other_sequences(b, t, c, step_gate):
     """Four channels a thread are half the columns, not a reason for segments."""
     assert workspace(b, t, c, SPIKES, step_gate, 0) == workspace(b, t, c, F32, step_gate, 0) == 0
+
+
+def test_rows_of_a_step_that_name_slots():
+    """As many as are looked through in seconds; rows without slots may be more."""
+    call = lambda batch, slots: sb.lib().snn_b200_leaky_step_async(  # noqa: E731
+        0, None, batch, 1 << 23, 0, 1 << 20, F32, 0, None, F32, 0, 0, 0, 0.5, 1.0, 1 << 20, 0, slots, 1 << 20, F32, 0)
+    assert call(1 << 22, 1 << 20) == call((1 << 22) + 1, None) == sb.SNN_OK  # no channels: nothing is launched
+    assert call((1 << 22) + 1, 1 << 20) == sb.SNN_ERR_OVERFLOW

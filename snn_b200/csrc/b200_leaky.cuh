@@ -5,20 +5,23 @@
 // thread each V of them, with the state in registers, so every access is one
 // run of 32 V elements. What limits it is how much it keeps under way: the next
 // blocks of kSteps steps are copied to shared memory (cp.async) while one is
-// worked on. 1024 sequences of 64 steps and 1024 channels, bf16 with logits: 66 us
-// (6.1 TB/s), the gradient 112 us (6.3 TB/s).
+// worked on. 1024 sequences of 64 steps and 1024 channels, bf16 with logits: 69 us
+// (5.8 TB/s), the gradient 112 us (6.3 TB/s).
 //
 // Fewer channels than keep the GPU busy that way are walked by crews: the warps
 // of a CTA take the next blocks of one column side by side. Steps compose as
 // affine maps h -> A h + H; each warp shares its block's map, folds those before
 // its own onto the state, and then walks its block. 4 x 8192 x 2048 (128 columns):
-// 104 us, the gradient 155 us; the SMs' issue slots are the bound, with 30 and 49
-// instructions an element.
+// 109 us, the gradient 165 us, of a floor of 62 and 105. No one thing is the bound: 20 SMs
+// have no column, the others' schedulers issue (30 and 49 instructions an element) in 62
+// and 63 of 100 cycles, and of the 6.4 cycles a warp takes for an instruction 1.4 are
+// fixed latencies, 0.9 to 1.2 shared memory, 0.4 to 0.7 the barrier of a round, 0.5 to
+// 1.0 a busy arithmetic pipe.
 //
 // Where even crews are too few, the steps are cut into segments: one kernel
 // walks each segment for its map, one folds them in order into the state before
 // each segment, and the walk itself then starts everywhere at once. The inputs
-// are read twice. 1 x 65536 x 1024: 127 to 132 us, the gradient 178 us. (One pass
+// are read twice. 1 x 65536 x 1024: 133 to 144 us, the gradient 180 us. (One pass
 // whose tiles publish maps and wait for the ones before them took 370 to 450 us
 // there: the tiles under way are too few to cover the waits.)
 #pragma once
@@ -903,7 +906,8 @@ __global__ void __launch_bounds__(N * 32) back_crew_kernel(const __grid_constant
 // looks through the slots once, for all of its rows at a time. 2000 rows of 1000
 // channels out of 4096: 7 us a call, 28 MB; the look was most of it (10.5 us) while
 // every slot was compared with all that a decision needs instead of first with
-// the rows' own.
+// the rows' own. It grows with the square of the rows: 8192 take 34 us with slots and 21
+// without, 65,536 844 and 205.
 template <typename X, typename G, typename Y, int V>
 __global__ void __launch_bounds__(256, 4) step_kernel(StepArgs g) {
     __shared__ uint32_t s_before[8], s_after[8];  // rows named before, rows named again

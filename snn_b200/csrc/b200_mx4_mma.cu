@@ -209,10 +209,10 @@ constexpr uint32_t kNoValue = 0x7fffffffu;
 // rows, and the instructions read x from both, so an SM loads 35 KB for 256 of k
 // where a CTA of its own with 256 rows of x would load 52.
 //
-// 8192 x 8192 x 8192: 189 us, 5.8 PFLOP/s, the tensor pipe active 72% of the
+// 8192 x 8192 x 8192: 193 us, 5.7 PFLOP/s, the tensor pipe active 72% of the
 // time. The bound was the issue (347 us while one lane of a divergent warp put
 // the descriptors together; leaving out the loads or the stores changed nothing,
-// leaving out the scale copies gave 277). 50000 x 784 x 1000 to f32: 50 us, of
+// leaving out the scale copies gave 277). 50000 x 784 x 1000 to f32: 49 us, of
 // which the writes of 200 MB are 30; 16 warps read the accumulators there, as
 // with 8 (43 against 33 us at 768 of k to bf16) a tile's writes took longer than
 // its instructions.
@@ -373,11 +373,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ---- skinny form ----
-// Four parts of k of 4 x 8192 x 8192 are one wave of 256 CTAs, two an SM: 9 us a
-// launch among others, of which the 36 MB of weights are 5.5; the rest is set-up
-// and the joining of the parts. Packing x on the way takes 16 rows in 12.3 us where
-// a packing kernel before it takes 12.6 + 4, 32 rows in 22.7 against 14.6 + 4, so
-// 16 rows are the most.
+// Four parts of k of 4 x 8192 x 8192 are one wave of 256 CTAs, two an SM: 8 to 10 us
+// a launch among others, of which the 36 MB of weights are 5.5; the rest is set-up
+// and the joining of the parts. Packing x on the way takes 16 rows in 13.1 us where
+// a packing kernel before it makes 15.6 of 17 rows (the product itself 11.0); 32 rows
+// took 22.7 on the way, 15.9 that way, so 16 rows are the most.
 constexpr uint32_t kMostSplits = 8;
 template <uint32_t BN>
 struct Skinny {

@@ -72,11 +72,17 @@ template <typename... T>
 bool wants_gradient(const T &...inputs) {
     return at::GradMode::is_enabled() && ((inputs.defined() && inputs.requires_grad()) || ...);
 }
+// It leads on to what the inputs come from, but not to the accumulators of leaves: a
+// result that lives on would keep one, with the stream of this call, which a backward
+// pass of the same leaves captured into a graph could not use.
 template <typename... T>
 std::shared_ptr<NoFormula> no_formula(const char *text, const T &...inputs) {
     if (!wants_gradient(inputs...)) return nullptr;
     std::shared_ptr<NoFormula> f(new NoFormula(text), torch::autograd::deleteNode);
-    f->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    const auto lead = [&](const Tensor &t) {
+        if (t.defined() && t.grad_fn()) f->add_next_edge(torch::autograd::impl::gradient_edge(t));
+    };
+    (lead(inputs), ...);
     return f;
 }
 Tensor &behind(Tensor &result, const std::shared_ptr<NoFormula> &f) {

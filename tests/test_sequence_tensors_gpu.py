@@ -93,7 +93,9 @@ def test_results_of_inputs_that_require_a_gradient_say_so():
                 continue
             with pytest.raises(NotImplementedError, match=text):
                 (y.sum() + leaf.sum()).backward()
-            pool.zero_()
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(f(*args).sum(), leaf)
+            args[i] = leaf * 2
             with pytest.raises(NotImplementedError, match=text):
                 torch.autograd.grad(f(*args).sum() + leaf.sum(), leaf)
 
@@ -125,6 +127,17 @@ def test_gradient_calls_under_autograd():
             return sb.leaky_scan_backward(dy, x, z, saved, logit=True)[:2]
 
     Scan.apply(x, z).backward(dy)
+    assert torch.equal(x.grad, by_hand[0]) and torch.equal(z.grad, by_hand[1])
+
+    # The results above live on: they do not tie the leaves to the stream that they were made on.
+    assert y.requires_grad and not y.grad_fn.next_functions
+    x.grad = z.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        Scan.apply(x, z).backward(dy)
+    graph.replay()
+    torch.cuda.synchronize()
     assert torch.equal(x.grad, by_hand[0]) and torch.equal(z.grad, by_hand[1])
 
 
